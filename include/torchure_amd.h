@@ -445,6 +445,99 @@ int tm_ce_grad_w_ld_bf16(uint16_t* d_grad_w, const uint16_t* d_grad_logits, int6
                          const uint16_t* d_hidden, int64_t rows, int64_t vocab, int64_t dim, void* d_ws,
                          size_t ws_bytes, void* stream);
 
+/*
+ * The linear layers of a decoder block (torchure/models/qwen3/qwen3.py:107-113,220-230: projections and
+ * the SwiGLU feed-forward, bf16 matmuls under autocast): bf16 MFMA products with fp32 accumulation and
+ * what follows them, in one launch each (two where K is split). Deterministic. Matrices are row-major
+ * with a row stride in elements; a, b0 and b1 are bf16, 16-byte aligned, with strides that are multiples
+ * of 8 and cover the width's next multiple of 8, the padding zero. One of:
+ *   TM_LIN_FORWARD    o0 (rows x out) = act(a b0^T + bias) + res, rounded once to bf16 or (out_f32) fp32;
+ *                     a rows x inp, b0 out x inp; bias (out) and res (rows x out) bf16 or fp32 or NULL.
+ *                     held: z0 = a b0^T + bias as the backward pass reads it.
+ *   TM_LIN_GATE       o0 (rows x out, bf16, zeros up to the next multiple of 8) =
+ *                     silu(a b0^T) (a b1^T). held: z0, z1 = the two products.
+ *   TM_LIN_GRAD_X     o0 (rows x inp) = a b0, a rows x out, b0 out x inp (the weight as stored). With
+ *                     b1: a's rows are [d0 | d1], each of out columns and zeros up to the next multiple
+ *                     of 64, and o0 = d0 b0 + d1 b1.
+ *   TM_LIN_GATE_GRAD  with d = a b0 (rows x inp; a rows x out, b0 out x inp), g = z0 and u = z1 as held
+ *                     by TM_LIN_GATE (inp columns): o0's rows (bf16) = [d u silu'(g) | d silu(g)], each
+ *                     with zeros up to the next multiple of 64; o1 (bf16, optional, rows ldo1
+ *                     apart, zeros likewise) = silu(g) u.
+ *   TM_LIN_GRAD_W     o0 (out x inp) = a^T b0, a rows x out, b0 rows x inp. With o1: a's rows are
+ *                     [d0 | d1] as in TM_LIN_GRAD_X, o0 = d0^T b0 and o1 = d1^T b0.
+ * held: TM_HELD_BF16, rows of the next multiple of 8 columns; TM_HELD_E4M3, rows of the next multiple of
+ * 32, with exponents s0 and s1 (see tm_quantize_e4m3); padding columns zero.
+ * d_ws holds tm_lin_workspace_bytes(op, rows, inp, out, two) bytes, two: b1 (TM_LIN_GRAD_X) or o1
+ * (TM_LIN_GRAD_W) is given. Calls that share a workspace on one stream are ordered.
+ */
+#define TM_LIN_FORWARD 0
+#define TM_LIN_GATE 1
+#define TM_LIN_GRAD_X 2
+#define TM_LIN_GATE_GRAD 3
+#define TM_LIN_GRAD_W 4
+
+#define TM_ACT_NONE 0
+#define TM_ACT_RELU 1
+#define TM_ACT_SILU 2
+#define TM_ACT_GELU 3      /* z Phi(z) */
+#define TM_ACT_GELU_TANH 4 /* its tanh form */
+
+#define TM_HELD_NOT 0
+#define TM_HELD_BF16 1
+#define TM_HELD_E4M3 2
+
+typedef struct tm_lin {
+  int64_t rows, inp, out;
+  const uint16_t* a;
+  const uint16_t* b0;
+  const uint16_t* b1;
+  int64_t lda, ldb;
+  void* o0;
+  void* o1;
+  int64_t ldo, ldo1;
+  const void* bias;
+  const void* res;
+  int64_t ldr;
+  void* z0;
+  void* z1;
+  uint8_t* s0;
+  uint8_t* s1;
+  int64_t ldz;
+  int32_t op, act, held;
+  int32_t out_f32, bias_f32, res_f32;
+} tm_lin_t;
+
+size_t tm_lin_workspace_bytes(int op, int64_t rows, int64_t inp, int64_t out, int two);
+int tm_lin(const tm_lin_t* h_desc, void* d_ws, size_t ws_bytes, void* stream);
+
+/*
+ * Activations held in 8 bits between forward and backward: e4m3 values (rows ldv apart, ldv = cols' next
+ * multiple of 32, padding zero, 16-byte aligned) and for each block of 32 rows x 32 columns the byte
+ * e + 127 (ceil(rows / 32) x ceil(cols / 32)): e the least exponent with which the block's largest
+ * finite magnitude is at most 448 2^e, clamped to [-117, 119]. Values round to nearest even; past
+ * 448 2^119 they are held as that, infinities and NaN as NaN. Reading back is exact in bf16 and fp32.
+ *   tm_quantize_e4m3    from bf16 or (src_f32) fp32 rows lds apart. d_copy, when given: the values as bf16
+ *                       too, rows ldc apart (cols' next multiple of 8; padding zero, 16-byte aligned).
+ *   tm_dequantize_e4m3  to bf16 or fp32 rows ldd apart.
+ */
+int tm_quantize_e4m3(uint8_t* d_values, uint8_t* d_exponents, int64_t ldv, const void* d_src, int src_f32, int64_t lds,
+                     int64_t rows, int64_t cols, uint16_t* d_copy, int64_t ldc, void* stream);
+int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_values, const uint8_t* d_exponents,
+                       int64_t ldv, int64_t rows, int64_t cols, void* stream);
+
+/*
+ * The way back through an activation: d_dz (bf16, rows lddz apart, a multiple of 8 of at least cols, zeros
+ * past cols, 16-byte aligned; or NULL) = dy act'(z), dy bf16 or (dy_f32) fp32 rows ldy apart, z as held
+ * by tm_lin (rows ldz apart, exponents with TM_HELD_E4M3; not read when act is TM_ACT_NONE, which makes
+ * this a cast into padded rows). d_bias (bf16 or, bias_f32, fp32; or NULL) = the sums of the unrounded
+ * dz over the rows, by fp32 partial sums over 128 rows each in d_ws, tm_act_grad_workspace_bytes bytes,
+ * added in order.
+ */
+size_t tm_act_grad_workspace_bytes(int64_t rows, int64_t cols);
+int tm_act_grad(uint16_t* d_dz, int64_t lddz, void* d_bias, int bias_f32, const void* d_dy, int dy_f32, int64_t ldy,
+                const void* d_z, const uint8_t* d_exponents, int64_t ldz, int held, int act, int64_t rows, int64_t cols,
+                void* d_ws, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

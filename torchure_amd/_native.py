@@ -32,6 +32,10 @@ TM_CHUNK_ALIGN = 2048
 TM_NORM_PARTIALS = 2048
 TM_NOALLOC_MAX_TENSORS = 16384
 
+TM_LIN_FORWARD, TM_LIN_GATE, TM_LIN_GRAD_X, TM_LIN_GATE_GRAD, TM_LIN_GRAD_W = range(5)
+TM_ACTS = ("none", "relu", "silu", "gelu", "gelu_tanh")  # TM_ACT_*, in order
+TM_HELD_NOT, TM_HELD_BF16, TM_HELD_E4M3 = range(3)
+
 # tm_tensor_t (include/torchure_amd.h), 64 bytes.
 TENSOR_DTYPE = np.dtype(
     [
@@ -65,6 +69,21 @@ class TmHyper(ctypes.Structure):
         ("weight_decay", ctypes.c_double),
         ("eps", ctypes.c_double),
     ]
+
+
+class TmLin(ctypes.Structure):
+    """tm_lin_t."""
+
+    _fields_ = ([(n, ctypes.c_int64) for n in ("rows", "inp", "out")]
+                + [(n, ctypes.c_void_p) for n in ("a", "b0", "b1")]
+                + [(n, ctypes.c_int64) for n in ("lda", "ldb")]
+                + [(n, ctypes.c_void_p) for n in ("o0", "o1")]
+                + [(n, ctypes.c_int64) for n in ("ldo", "ldo1")]
+                + [(n, ctypes.c_void_p) for n in ("bias", "res")]
+                + [("ldr", ctypes.c_int64)]
+                + [(n, ctypes.c_void_p) for n in ("z0", "z1", "s0", "s1")]
+                + [("ldz", ctypes.c_int64)]
+                + [(n, ctypes.c_int32) for n in ("op", "act", "held", "out_f32", "bias_f32", "res_f32")])
 
 
 # Every symbol include/torchure_amd.h declares, with its ctypes signature.
@@ -119,6 +138,16 @@ _SIGNATURES = {
     "tm_ce_grad_h_ld_bf16": (ctypes.c_int, [_vp, _vp, _i64, _vp, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
     "tm_ce_grad_w_ld_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
     "tm_ce_grad_w_ld_bf16": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
+    "tm_lin_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _i64, _i64, _i64, ctypes.c_int]),
+    "tm_lin": (ctypes.c_int, [ctypes.POINTER(TmLin), _vp, ctypes.c_size_t, _vp]),
+    "tm_quantize_e4m3": (ctypes.c_int, [_vp, _vp, _i64, _vp, ctypes.c_int, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "tm_dequantize_e4m3": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "tm_act_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "tm_act_grad": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, ctypes.c_int, _vp, ctypes.c_int, _i64, _vp, _vp, _i64, ctypes.c_int, ctypes.c_int, _i64, _i64,
+         _vp, ctypes.c_size_t, _vp],
+    ),
 }
 
 EXPORTED = tuple(_SIGNATURES)

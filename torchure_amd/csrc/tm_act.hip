@@ -1,0 +1,346 @@
+// tm_act.hip -- gfx950 element-wise kernels around the linear layers' products (tm_linear.hip):
+//   quantize_kernel, dequantize_kernel   activations into 8 bits and back (the format: tm_act.h)
+//   act_grad_kernel                      dz = dy act'(z) from z as held, with the column sums of dz, and
+//   col_sum_kernel                       the bias gradient from those sums
+// All are bound by memory: every element is read and written once, 16 bytes a lane.
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "torchure_amd.h"
+#include "tm_act.h"
+#include "tm_internal.h"
+
+namespace {
+
+using tm_act::f32x4;
+using tm_act::pack_bf16;
+using tm_act::u32x2;
+using tm_act::u32x4;
+
+template <typename... A>
+int act_fail(int code, const char* fmt, A... args) {
+  return tm_internal_fail(code, fmt, args...);
+}
+
+// Eight bf16 or fp32 values of a row; `left` of them exist (zeros after), vec: 16-byte pieces.
+template <bool kF32>
+__device__ __forceinline__ void get8(float (&x)[8], const void* base, int64_t at, int left, bool vec) {
+  if (vec && left >= 8) {
+    if constexpr (kF32) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + at);
+      const f32x4 a = p[0], b = p[1];
+      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+      const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + at);
+      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = tm_act::bf16_lo(w[e]);
+        x[2 * e + 1] = tm_act::bf16_hi(w[e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = 0.0f;
+      if (e < left)
+        x[e] = kF32 ? static_cast<const float*>(base)[at + e]
+                    : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(base)[at + e]) << 16);
+    }
+  }
+}
+
+template <bool kF32>
+__device__ __forceinline__ void put8(void* base, int64_t at, const float (&x)[8], int left, bool vec) {
+  if constexpr (kF32) {
+    float* p = static_cast<float*>(base) + at;
+    if (vec && left >= 8) {
+      reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
+      reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) p[e] = x[e];
+    }
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(base) + at;
+    const uint32_t w[4] = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
+    if (vec && left >= 8) {
+      *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < left) p[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
+    }
+  }
+}
+
+// A wave takes 32 rows x 64 columns, two blocks side by side: lane l the columns 8 (l % 8) .. + 7 of rows
+// l / 8, + 8, + 16, + 24.
+template <bool kF32>
+__global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
+                                                       int64_t ldv, const void* __restrict__ src, int64_t lds,
+                                                       int64_t rows, int cols, int vec, int wide,
+                                                       uint16_t* __restrict__ copy, int64_t ldc) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t band = blockIdx.x / wide;
+  const int n0 = (static_cast<int>(blockIdx.x % wide) * 4 + wave) * 64, n = n0 + 8 * (lane & 7);
+  if (n0 >= cols) return;
+  const int64_t m = band * 32 + (lane >> 3);
+  float x[4][8];
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool in = m + 8 * i < rows;
+    get8<kF32>(x[i], src, in ? (m + 8 * i) * lds + n : 0, in ? cols - n : 0, vec != 0);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) most = max(most, tm_act::finite_bits(x[i][e]));
+#pragma unroll
+  for (int d : {1, 2, 8, 16, 32}) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
+  const int e2 = tm_act::block_exponent(most);
+  const float inv = tm_act::two_to(-e2);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (m + 8 * i >= rows) continue;
+    if (n < ldv) {
+      const u32x2 w = {tm_act::encode4(x[i][0], x[i][1], x[i][2], x[i][3], inv),
+                       tm_act::encode4(x[i][4], x[i][5], x[i][6], x[i][7], inv)};
+      *reinterpret_cast<u32x2*>(values + (m + 8 * i) * ldv + n) = w;
+    }
+    if (copy && n < ldc) put8<false>(copy, (m + 8 * i) * ldc + n, x[i], 8, true);
+  }
+  const int block = (n0 >> 5) + ((lane >> 2) & 1);
+  if ((lane & ~4) == 0 && block * 32 < cols)
+    exps[band * ((cols + 31) / 32) + block] = static_cast<uint8_t>(e2 + 127);
+}
+
+template <bool kF32>
+__global__ __launch_bounds__(256) void dequantize_kernel(void* __restrict__ dst, int64_t ldd,
+                                                         const uint8_t* __restrict__ values,
+                                                         const uint8_t* __restrict__ exps, int64_t ldv, int64_t rows,
+                                                         int cols, int vec, int wide) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t band = blockIdx.x / wide;
+  const int n0 = (static_cast<int>(blockIdx.x % wide) * 4 + wave) * 64, n = n0 + 8 * (lane & 7);
+  if (n >= cols) return;
+  const int64_t m = band * 32 + (lane >> 3);
+  const float scale = tm_act::two_to(static_cast<int>(exps[band * ((cols + 31) / 32) + (n >> 5)]) - 127);
+  u32x2 w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (m + 8 * i < rows) w[i] = *reinterpret_cast<const u32x2*>(values + (m + 8 * i) * ldv + n);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (m + 8 * i >= rows) continue;
+    const f32x4 a = tm_act::decode4(w[i].x, scale), b = tm_act::decode4(w[i].y, scale);
+    const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    put8<kF32>(dst, (m + 8 * i) * ldd + n, x, cols - n, vec != 0);
+  }
+}
+
+constexpr int kBandRows = 128;  // rows of one partial column sum
+
+// A workgroup takes kBandRows rows x 256 columns: thread t the columns 8 (t % 32) .. + 7 of rows t / 32, + 8, ...
+template <bool kF32>
+__global__ __launch_bounds__(256) void act_grad_kernel(uint16_t* __restrict__ dz, int64_t lddz,
+                                                       float* __restrict__ sums, const void* __restrict__ dy,
+                                                       int64_t ldy, int vec, const uint8_t* __restrict__ z,
+                                                       const uint8_t* __restrict__ exps, int64_t ldz, int held, int act,
+                                                       int64_t rows, int cols, int wide) {
+  const int t = threadIdx.x;
+  const int64_t band = blockIdx.x / wide;
+  const int n = static_cast<int>(blockIdx.x % wide) * 256 + 8 * (t & 31);
+  const int64_t m_end = min(rows, (band + 1) * kBandRows);
+  const int blocks = (cols + 31) / 32;
+  float total[8] = {};
+  if (n < cols) {
+#pragma unroll 4
+    for (int64_t m = band * kBandRows + (t >> 5); m < m_end; m += 8) {
+      float d[8];
+      get8<kF32>(d, dy, m * ldy + n, cols - n, vec != 0);
+      if (act != TM_ACT_NONE) {
+        float x[8];
+        if (held == TM_HELD_BF16) {
+          get8<false>(x, z, m * ldz + n, 8, true);
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(z + m * ldz + n);
+          const float scale = tm_act::two_to(static_cast<int>(exps[(m >> 5) * blocks + (n >> 5)]) - 127);
+          const f32x4 a = tm_act::decode4(w.x, scale), b = tm_act::decode4(w.y, scale);
+          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+          x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+        }
+        auto each = [&](auto f) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] *= f(x[e]);
+        };
+        if (act == tm_act::kRelu) each([](float v) { return tm_act::act1_grad(tm_act::kRelu, v); });
+        else if (act == tm_act::kSilu) each([](float v) { return tm_act::act1_grad(tm_act::kSilu, v); });
+        else if (act == tm_act::kGelu) each([](float v) { return tm_act::act1_grad(tm_act::kGelu, v); });
+        else each([](float v) { return tm_act::act1_grad(tm_act::kGeluTanh, v); });
+        if (cols - n < 8)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e >= cols) d[e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) total[e] += d[e];
+      if (dz) put8<false>(dz, m * lddz + n, d, 8, true);
+    }
+  } else if (dz && n < lddz) {  // whole groups of padding
+    const float none[8] = {};
+    for (int64_t m = band * kBandRows + (t >> 5); m < m_end; m += 8) put8<false>(dz, m * lddz + n, none, 8, true);
+  }
+  if (!sums) return;
+  __shared__ float part[8][256];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[t >> 5][8 * (t & 31) + e] = total[e];
+  __syncthreads();
+  const int c = static_cast<int>(blockIdx.x % wide) * 256 + t;
+  if (c >= cols) return;
+  float sum = part[0][t];
+#pragma unroll
+  for (int r = 1; r < 8; ++r) sum += part[r][t];
+  sums[band * cols + c] = sum;
+}
+
+// A column's partial sums, a quarter of the bands by each of a workgroup's waves, then the quarters, in order.
+__global__ __launch_bounds__(256) void col_sum_kernel(void* __restrict__ out, int f32, const float* __restrict__ sums,
+                                                      int64_t bands, int cols) {
+  __shared__ float part[4][64];
+  const int c = static_cast<int>(blockIdx.x) * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const int64_t per = (bands + 3) / 4, from = w * per, to = min(bands, from + per);
+  float sum = 0.0f;
+  if (c < cols)
+#pragma unroll 8
+    for (int64_t b = from; b < to; ++b) sum += sums[b * cols + c];
+  part[w][threadIdx.x & 63] = sum;
+  __syncthreads();
+  if (w || c >= cols) return;
+  sum = ((part[0][threadIdx.x] + part[1][threadIdx.x]) + part[2][threadIdx.x]) + part[3][threadIdx.x];
+  if (f32) static_cast<float*>(out)[c] = sum;
+  else static_cast<uint16_t*>(out)[c] = static_cast<uint16_t>(pack_bf16(sum, sum));
+}
+
+bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxCols = int64_t(1) << 30, kMaxGroups = int64_t(1) << 30;
+
+int check_shape(const char* who, int64_t rows, int64_t cols, int64_t groups) {
+  if (rows < 0 || cols < 0 || rows > kMaxRows || cols > kMaxCols || groups > kMaxGroups)
+    return act_fail(TM_EINVAL, "%s: %lld rows of %lld are negative or too large", who, (long long)rows, (long long)cols);
+  return TM_OK;
+}
+
+int launched(const char* who) {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? TM_OK : act_fail(TM_ELAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
+}
+
+}  // namespace
+
+extern "C" {
+
+int tm_quantize_e4m3(uint8_t* d_values, uint8_t* d_exponents, int64_t ldv, const void* d_src, int src_f32, int64_t lds,
+                     int64_t rows, int64_t cols, uint16_t* d_copy, int64_t ldc, void* stream) {
+  const char* who = "tm_quantize_e4m3";
+  const int64_t wide = ceil_div(cols, 256), groups = rows > 0 && cols > 0 ? ceil_div(rows, 32) * wide : 0;
+  if (const int rc = check_shape(who, rows, cols, groups)) return rc;
+  if (groups == 0) return TM_OK;
+  if (!d_values || !d_exponents || !d_src) return act_fail(TM_EINVAL, "%s: null pointer", who);
+  if (ldv != ceil_div(cols, 32) * 32 || !aligned(d_values, 16) || lds < cols || !aligned(d_src, src_f32 ? 4 : 2))
+    return act_fail(TM_EINVAL, "%s: values (rows %lld apart) need rows of the next multiple of 32 to %lld, 16-byte "
+                    "aligned; source rows are %lld apart", who, (long long)ldv, (long long)cols, (long long)lds);
+  if (d_copy && (ldc != ceil_div(cols, 8) * 8 || !aligned(d_copy, 16)))
+    return act_fail(TM_EINVAL, "%s: copy rows %lld apart for %lld columns: the next multiple of 8, 16-byte aligned", who,
+                    (long long)ldc, (long long)cols);
+  const int vec = lds % (src_f32 ? 4 : 8) == 0 && aligned(d_src, 16);
+  const dim3 grid(static_cast<uint32_t>(groups));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (src_f32)
+    hipLaunchKernelGGL(quantize_kernel<true>, grid, dim3(256), 0, s, d_values, d_exponents, ldv, d_src, lds, rows,
+                       static_cast<int>(cols), vec, static_cast<int>(wide), d_copy, ldc);
+  else
+    hipLaunchKernelGGL(quantize_kernel<false>, grid, dim3(256), 0, s, d_values, d_exponents, ldv, d_src, lds, rows,
+                       static_cast<int>(cols), vec, static_cast<int>(wide), d_copy, ldc);
+  return launched(who);
+}
+
+int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_values, const uint8_t* d_exponents,
+                       int64_t ldv, int64_t rows, int64_t cols, void* stream) {
+  const char* who = "tm_dequantize_e4m3";
+  const int64_t wide = ceil_div(cols, 256), groups = rows > 0 && cols > 0 ? ceil_div(rows, 32) * wide : 0;
+  if (const int rc = check_shape(who, rows, cols, groups)) return rc;
+  if (groups == 0) return TM_OK;
+  if (!d_values || !d_exponents || !d_dst) return act_fail(TM_EINVAL, "%s: null pointer", who);
+  if (ldv != ceil_div(cols, 32) * 32 || !aligned(d_values, 16) || ldd < cols || !aligned(d_dst, dst_f32 ? 4 : 2))
+    return act_fail(TM_EINVAL, "%s: values (rows %lld apart) need rows of the next multiple of 32 to %lld, 16-byte "
+                    "aligned; output rows are %lld apart", who, (long long)ldv, (long long)cols, (long long)ldd);
+  const int vec = ldd % (dst_f32 ? 4 : 8) == 0 && aligned(d_dst, 16);
+  const dim3 grid(static_cast<uint32_t>(groups));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dst_f32)
+    hipLaunchKernelGGL(dequantize_kernel<true>, grid, dim3(256), 0, s, d_dst, ldd, d_values, d_exponents, ldv, rows,
+                       static_cast<int>(cols), vec, static_cast<int>(wide));
+  else
+    hipLaunchKernelGGL(dequantize_kernel<false>, grid, dim3(256), 0, s, d_dst, ldd, d_values, d_exponents, ldv, rows,
+                       static_cast<int>(cols), vec, static_cast<int>(wide));
+  return launched(who);
+}
+
+size_t tm_act_grad_workspace_bytes(int64_t rows, int64_t cols) {
+  if (rows <= 0 || cols <= 0) return 0;
+  return static_cast<size_t>(ceil_div(rows, kBandRows)) * cols * sizeof(float);
+}
+
+int tm_act_grad(uint16_t* d_dz, int64_t lddz, void* d_bias, int bias_f32, const void* d_dy, int dy_f32, int64_t ldy,
+                const void* d_z, const uint8_t* d_exponents, int64_t ldz, int held, int act, int64_t rows, int64_t cols,
+                void* d_ws, size_t ws_bytes, void* stream) {
+  const char* who = "tm_act_grad";
+  const int64_t wide = ceil_div(d_dz && lddz > cols ? lddz : cols, 256);
+  const int64_t bands = rows > 0 ? ceil_div(rows, kBandRows) : 0;
+  if (const int rc = check_shape(who, rows, cols, bands * wide)) return rc;
+  if (rows == 0 || cols == 0) return act_fail(TM_EINVAL, "%s: no elements", who);
+  if (!d_dy || (!d_dz && !d_bias)) return act_fail(TM_EINVAL, "%s: null pointer", who);
+  if (act < 0 || act > TM_ACT_GELU_TANH) return act_fail(TM_EINVAL, "%s: unknown activation %d", who, act);
+  if (ldy < cols || !aligned(d_dy, dy_f32 ? 4 : 2))
+    return act_fail(TM_EINVAL, "%s: dy rows %lld apart for %lld columns", who, (long long)ldy, (long long)cols);
+  if (d_dz && (lddz % 8 || lddz < cols || lddz - cols >= 256 || !aligned(d_dz, 16)))
+    return act_fail(TM_EINVAL, "%s: dz rows %lld apart for %lld columns, 16-byte aligned", who, (long long)lddz,
+                    (long long)cols);
+  if (act != TM_ACT_NONE) {
+    if (!d_z || !aligned(d_z, 16) || (held == TM_HELD_E4M3 && !d_exponents))
+      return act_fail(TM_EINVAL, "%s: z must be 16-byte aligned, not null", who);
+    if (held == TM_HELD_BF16 ? ldz % 8 || ldz < cols : held != TM_HELD_E4M3 || ldz != ceil_div(cols, 32) * 32)
+      return act_fail(TM_EINVAL, "%s: z held as %d in rows %lld apart for %lld columns", who, held, (long long)ldz,
+                      (long long)cols);
+  }
+  const size_t need = d_bias ? tm_act_grad_workspace_bytes(rows, cols) : 0;
+  if (need && (!d_ws || ws_bytes < need || !aligned(d_ws, 4)))
+    return act_fail(TM_EINVAL, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, need);
+  const int vec = ldy % (dy_f32 ? 4 : 8) == 0 && aligned(d_dy, 16);
+  float* sums = d_bias ? static_cast<float*>(d_ws) : nullptr;
+  const dim3 grid(static_cast<uint32_t>(bands * wide));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (dy_f32)
+    hipLaunchKernelGGL(act_grad_kernel<true>, grid, dim3(256), 0, s, d_dz, lddz, sums, d_dy, ldy, vec,
+                       static_cast<const uint8_t*>(d_z), d_exponents, ldz, held, act, rows, static_cast<int>(cols),
+                       static_cast<int>(wide));
+  else
+    hipLaunchKernelGGL(act_grad_kernel<false>, grid, dim3(256), 0, s, d_dz, lddz, sums, d_dy, ldy, vec,
+                       static_cast<const uint8_t*>(d_z), d_exponents, ldz, held, act, rows, static_cast<int>(cols),
+                       static_cast<int>(wide));
+  if (const int rc = launched(who)) return rc;
+  if (!d_bias) return TM_OK;
+  hipLaunchKernelGGL(col_sum_kernel, dim3(static_cast<uint32_t>(ceil_div(cols, 64))), dim3(256), 0, s, d_bias, bias_f32,
+                     sums, bands, static_cast<int>(cols));
+  return launched(who);
+}
+
+}  // extern "C"
