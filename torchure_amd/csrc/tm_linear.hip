@@ -9,17 +9,21 @@
 //   gate_grad   dh  = dy Wd, then d_gate = dh u silu'(g), d_up = dh silu(g), silu(g) u
 //   grad_w      dW  = dz^T x                 both K-major
 //
-// One kernel template (lin_kernel) with fp32 accumulation on v_mfma_f32_32x32x16_bf16: 8 wave64, two a
+// One kernel template (lin_kernel) with fp32 accumulation on v_mfma_f32_16x16x32_bf16 (the chip's power
+// bounds long runs of products, and this shape takes less of it than 32x32x16): 8 wave64, two a
 // SIMD, wave (wm, wn) = (w / 4, w % 4) computing 32 kMB x 32 kNB of a 64 kMB x 128 kNB tile. Operands
-// stream global -> LDS (global_load_lds, 16 bytes a lane) into two stages of 64-deep K slices. A
-// K-contiguous operand lies there in 128-byte rows, chunk c of row r at slot c ^ ((r >> 1) & 7); a
-// K-major one in whole rows of the tile's columns, chunk c of row k at slot c ^ (4 (k & 3)), and is
-// read transposed (ds_read_b64_tr_b16): in both, the 16 lanes of a read hit 16 bank groups.
+// stream global -> LDS (global_load_lds, 16 bytes a lane) through five units, each one operand's slice of
+// 64 K (32 KB for 256 rows: all of a CU's 160 KB): two hold the current slice, three what comes next, so
+// that B's loads have one slice's products to come in and A's two. A K-contiguous operand is loaded in
+// whole 128-byte lines (64-byte pieces come in at little more than half the rate: 34 against 56 bytes a
+// clock and CU) and lies in 128-byte rows, chunk c of row r at slot c ^ ((r >> 1) & 7); a K-major one in
+// whole rows of the tile's columns, chunks swizzled by k_swizzle, and is read transposed
+// (ds_read_b64_tr_b16): in both, what a read's lanes get at a time lies on 16 bank groups.
 //
-// Workgroups are persistent. A workgroup's tiles form one stream of K slices: the loads run two
-// slices ahead of the products, across tiles, so that a tile starts on operands that came in during
-// the one before it; its results leave through a strip of LDS of their own while the next tile's
-// loads are in flight. Workgroup w runs on XCD w % 8; each XCD takes a contiguous range of tile
+// Workgroups are persistent. A workgroup's tiles form one stream of K slices: the loads run ahead of the
+// products across tiles, so that a tile starts on operands that came in during the one before it;
+// its results leave through the unit used up last, while loads into the others are in flight.
+// Workgroup w runs on XCD w % 8; each XCD takes a contiguous range of tile
 // positions, in groups of gm x gn tiles whose operand panels share its L2.
 //
 // Edges: rows and columns past an operand's last are loaded again (their results are not stored); K
@@ -46,20 +50,21 @@ using tm_act::u32x4;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 template <typename... A>
 int lin_fail(int code, const char* fmt, A... args) {
   return tm_internal_fail(code, fmt, args...);
 }
 
-constexpr int kSliceK = 64;  // K depth of one LDS stage
+constexpr int kSliceK = 64;  // K depth of one slice
+constexpr int kUnits = 5;    // LDS units, each one operand's slice
 
 constexpr int waitcnt_vm(int n) { return (n & 15) | ((n >> 4) << 14) | (7 << 4) | (15 << 8); }
 
 __device__ const u32x4 g_zeros = {0, 0, 0, 0};  // what K past an operand's end reads
 
-enum Mode { kLinear, kPlain, kGate, kGateGrad };
+// What follows a product: all of the forward's; only a residual, or nothing; the gate; its gradient.
+enum Mode { kLinear, kResidual, kPlain, kGate, kGateGrad };
 
 struct Args {
   const char* a;
@@ -92,21 +97,13 @@ struct Args {
   float* partial;
 };
 
-// Tile of position p: n-blocks of gn tile columns; inside each, m-blocks of gm tile rows, a
-// block's gm x gn tiles consecutive in p.
-__device__ __forceinline__ void tile_of(int p, int tiles_m, int tiles_n, int gm, int gn, int& tm, int& tn) {
-  const int per_nb = tiles_m * gn;
-  const int nb = p / per_nb, rem = p - nb * per_nb;
-  const int gn_eff = min(gn, tiles_n - nb * gn);
-  const int mb = rem / (gm * gn_eff), rem2 = rem - mb * gm * gn_eff;
-  tm = mb * gm + rem2 / gn_eff;
-  tn = nb * gn + rem2 % gn_eff;
-}
+// A K-major row's chunk c lies at slot c ^ k_swizzle(row).
+__device__ __forceinline__ int k_swizzle(int row) { return 2 * ((row & 3) | ((row >> 3 & 1) << 2)); }
 
 // ------------------------------------------------------------------------------ a tile's results
 //
-// A wave's accumulators come out in blocks of 32 x 32: register 4 q + e of lane l holds row l % 32, column
-// 8 q + 4 (l / 32) + e. Each block goes through this wave's strip of LDS (fp32, 128-byte rows, chunk c of
+// A wave's accumulators come out in blocks of 32 x 32, each 2 x 2 of the products' 16 x 16: there lane l
+// holds row l % 16, columns 4 (l / 16) .. + 3. Each block goes through this wave's strip of LDS (fp32, 128-byte rows, chunk c of
 // row r at slot c ^ ((r >> 1) & 7): a wave's LDS accesses are served in order, so no barrier and no wait
 // is needed between its writes and its reads) and is read back in the order of the output's rows: lane l
 // has columns 8 (l % 4) .. + 7 of rows l / 4 and 16 + l / 4. From there on every access to memory is 16
@@ -114,97 +111,218 @@ __device__ __forceinline__ void tile_of(int p, int tiles_m, int tiles_n, int gm,
 
 typedef const __attribute__((address_space(4))) Args* ArgsPtr;  // the kernel's arguments, where they are
 
+// What a tile's end needs of them, in scalar registers: read once for each tile and before its first block (one
+// after the other as a block needs them, the reads' latencies were 10 us of a tile; kept through
+// the products, they spill).
+struct End {
+  int m;
+  int n;
+  char* o0;
+  char* o1;
+  int64_t ldo;
+  int64_t ldo1;
+  int out_f32;
+  int out_vec;
+  int act;
+  int n_store;
+  const char* bias;
+  const char* res;
+  int64_t ldr;
+  int bias_f32;
+  int bias_vec;
+  int res_f32;
+  int res_vec;
+  char* z0;
+  char* z1;
+  uint8_t* s0;
+  uint8_t* s1;
+  int64_t ldz;
+  int held;
+  int blocks;
+};
+
+template <int kMode>
+__device__ __forceinline__ End end_of() {
+  ArgsPtr g = (ArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(g));
+  End e = {};
+#define TM_TAKE(field) e.field = g->field
+  if constexpr (kMode == kLinear) {
+    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(ldo); TM_TAKE(out_f32); TM_TAKE(out_vec); TM_TAKE(act);
+    TM_TAKE(bias); TM_TAKE(res); TM_TAKE(ldr); TM_TAKE(bias_f32); TM_TAKE(bias_vec); TM_TAKE(res_f32);
+    TM_TAKE(res_vec); TM_TAKE(z0); TM_TAKE(s0); TM_TAKE(ldz); TM_TAKE(held); TM_TAKE(blocks);
+  }
+  if constexpr (kMode == kResidual) {
+    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(ldo); TM_TAKE(out_f32); TM_TAKE(out_vec); TM_TAKE(res);
+    TM_TAKE(ldr); TM_TAKE(res_f32); TM_TAKE(res_vec);
+  }
+  if constexpr (kMode == kPlain) {
+    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(o1); TM_TAKE(ldo); TM_TAKE(out_f32); TM_TAKE(out_vec);
+  }
+  if constexpr (kMode == kGate) {
+    TM_TAKE(m); TM_TAKE(n); TM_TAKE(n_store); TM_TAKE(o0); TM_TAKE(ldo); TM_TAKE(z0); TM_TAKE(z1);
+    TM_TAKE(s0); TM_TAKE(s1); TM_TAKE(ldz); TM_TAKE(held); TM_TAKE(blocks);
+  }
+  if constexpr (kMode == kGateGrad) {
+    TM_TAKE(m); TM_TAKE(n); TM_TAKE(n_store); TM_TAKE(o0); TM_TAKE(o1); TM_TAKE(ldo); TM_TAKE(ldo1);
+    TM_TAKE(z0); TM_TAKE(z1); TM_TAKE(s0); TM_TAKE(s1); TM_TAKE(ldz); TM_TAKE(held); TM_TAKE(blocks);
+  }
+#undef TM_TAKE
+#define TM_KEEP(field) asm volatile("" : "+s"(e.field))
+  if constexpr (kMode == kLinear) {
+    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(ldo); TM_KEEP(out_f32); TM_KEEP(out_vec); TM_KEEP(act);
+    TM_KEEP(bias); TM_KEEP(res); TM_KEEP(ldr); TM_KEEP(bias_f32); TM_KEEP(bias_vec); TM_KEEP(res_f32);
+    TM_KEEP(res_vec); TM_KEEP(z0); TM_KEEP(s0); TM_KEEP(ldz); TM_KEEP(held); TM_KEEP(blocks);
+  }
+  if constexpr (kMode == kResidual) {
+    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(ldo); TM_KEEP(out_f32); TM_KEEP(out_vec); TM_KEEP(res);
+    TM_KEEP(ldr); TM_KEEP(res_f32); TM_KEEP(res_vec);
+  }
+  if constexpr (kMode == kPlain) {
+    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(o1); TM_KEEP(ldo); TM_KEEP(out_f32); TM_KEEP(out_vec);
+  }
+  if constexpr (kMode == kGate) {
+    TM_KEEP(m); TM_KEEP(n); TM_KEEP(n_store); TM_KEEP(o0); TM_KEEP(ldo); TM_KEEP(z0); TM_KEEP(z1);
+    TM_KEEP(s0); TM_KEEP(s1); TM_KEEP(ldz); TM_KEEP(held); TM_KEEP(blocks);
+  }
+  if constexpr (kMode == kGateGrad) {
+    TM_KEEP(m); TM_KEEP(n); TM_KEEP(n_store); TM_KEEP(o0); TM_KEEP(o1); TM_KEEP(ldo); TM_KEEP(ldo1);
+    TM_KEEP(z0); TM_KEEP(z1); TM_KEEP(s0); TM_KEEP(s1); TM_KEEP(ldz); TM_KEEP(held); TM_KEEP(blocks);
+  }
+#undef TM_KEEP
+  return e;
+}
+
+template <bool kV>
+struct Bool {
+  static constexpr bool value = kV;
+};
+
 struct Block {
   float v[16];  // [row half][column]
 };
 
-// kHalves: a strip of 2 KB, 16 rows at a time (else 4 KB).
+// A lane's places: where it writes and reads a block in the strip, and its bytes past a block's first element
+// in each matrix (rows 16 on: 16 rows more).
+struct Lane {
+  uint32_t w[2], r[2];
+  uint32_t out, out1, res, z;
+};
+
+template <int kMode>
+__device__ __forceinline__ Lane lane_of(const End& g, uint32_t stg, int lane) {
+  Lane l;
+  const uint32_t row = lane & 15, r = lane >> 2, sr = (r >> 1) & 7, c = 2 * (lane & 3), col = 8 * (lane & 3);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    l.w[i] = stg + row * 128 + (((4 * i + (lane >> 4)) ^ (row >> 1)) << 4);
+    l.r[i] = stg + r * 128 + (((c + i) ^ sr) << 4);
+  }
+  l.out = (r * static_cast<uint32_t>(g.ldo) + col) * (kMode <= kPlain && g.out_f32 ? 4 : 2);
+  if constexpr (kMode <= kResidual) l.res = (r * static_cast<uint32_t>(g.ldr) + col) * (g.res_f32 ? 4 : 2);
+  if constexpr (kMode == kGateGrad) l.out1 = (r * static_cast<uint32_t>(g.ldo1) + col) * 2;
+  if constexpr (kMode == kLinear || kMode >= kGate) l.z = (r * static_cast<uint32_t>(g.ldz) + col) * (g.held == TM_HELD_BF16 ? 2 : 1);
+  return l;
+}
+
+// kHalves: a strip of 2 KB, 16 rows at a time (else 4 KB). acc[row half][column half].
 template <bool kHalves>
-__device__ __forceinline__ void to_rows(Block& b, const f32x16& acc, uint32_t stg, int lane) {
-  const int row = lane & 31, sw = (row >> 1) & 7;
+__device__ __forceinline__ void to_rows(Block& b, const f32x4 (&acc)[2][2], const Lane& l) {
+  auto write = [&](int h, int at) {  // 16 rows on: the same slots
 #pragma unroll
-  for (int h = 0; h < (kHalves ? 2 : 1); ++h) {
-    if (!kHalves || (row >> 4) == h) {
+    for (int i = 0; i < 2; ++i)
+      asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(l.w[i]), "v"(acc[h][i]), "i"(at) : "memory");
+  };
+  auto keep = [&](int at, const f32x4& t) {
+    b.v[at] = t.x;
+    b.v[at + 1] = t.y;
+    b.v[at + 2] = t.z;
+    b.v[at + 3] = t.w;
+  };
+  f32x4 t[4];
+  if constexpr (kHalves) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t at = stg + (kHalves ? row & 15 : row) * 128 + (((2 * q + (lane >> 5)) ^ sw) << 4);
-        const f32x4 o = {acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]};
-        asm volatile("ds_write_b128 %0, %1" ::"v"(at), "v"(o) : "memory");
-      }
-    }
-    f32x4 t[4];
-    if constexpr (kHalves) {
-      const int r = lane >> 2, s = (r >> 1) & 7, c = 2 * (lane & 3);
+    for (int h = 0; h < 2; ++h) {
+      write(h, 0);
       asm volatile("ds_read_b128 %0, %2\n\tds_read_b128 %1, %3\n\ts_waitcnt lgkmcnt(0)"
                    : "=&v"(t[0]), "=&v"(t[1])
-                   : "v"(stg + r * 128 + ((c ^ s) << 4)), "v"(stg + r * 128 + (((c + 1) ^ s) << 4))
+                   : "v"(l.r[0]), "v"(l.r[1])
                    : "memory");
-    } else {
-      const int r = lane >> 2, s = (r >> 1) & 7, c = 2 * (lane & 3);
-      const uint32_t a0 = stg + r * 128 + ((c ^ s) << 4), a1 = stg + r * 128 + (((c + 1) ^ s) << 4);
-      // 16 rows on: the same slots
-      asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:2048\n\t"
-                   "ds_read_b128 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
-                   : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
-                   : "v"(a0), "v"(a1)
-                   : "memory");
+      keep(8 * h, t[0]);
+      keep(8 * h + 4, t[1]);
     }
+  } else {
+    write(0, 0);
+    write(1, 2048);
+    asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b128 %2, %4 offset:2048\n\t"
+                 "ds_read_b128 %3, %5 offset:2048\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3])
+                 : "v"(l.r[0]), "v"(l.r[1])
+                 : "memory");
 #pragma unroll
-    for (int i = 0; i < (kHalves ? 2 : 4); ++i) {
-      const int at = (kHalves ? 8 * h : 0) + 4 * i;
-      b.v[at] = t[i].x;
-      b.v[at + 1] = t[i].y;
-      b.v[at + 2] = t[i].z;
-      b.v[at + 3] = t[i].w;
+    for (int i = 0; i < 4; ++i) keep(4 * i, t[i]);
+  }
+}
+
+// Eight bf16 or fp32 values as they lie in memory.
+struct Raw8 {
+  u32x4 w[2];
+};
+
+__device__ __forceinline__ Raw8 raw8(const char* p, bool f32) {  // 16-byte aligned
+  Raw8 r;
+  r.w[0] = *reinterpret_cast<const u32x4*>(p);
+  r.w[1] = u32x4{0, 0, 0, 0};
+  if (f32) r.w[1] = *reinterpret_cast<const u32x4*>(p + 16);
+  return r;
+}
+
+__device__ __forceinline__ Raw8 raw8(const char* p, bool f32, int left, bool vec) {  // `left` of them exist
+  if (vec && left >= 8) return raw8(p, f32);
+  uint32_t w[8] = {};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < left) {
+      if (f32) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
+      else w[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
+    }
+  return {{u32x4{w[0], w[1], w[2], w[3]}, u32x4{w[4], w[5], w[6], w[7]}}};
+}
+
+__device__ __forceinline__ void values8(float* x, const Raw8& r, bool f32) {
+  const uint32_t a[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w}, b[4] = {r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (f32) {
+      x[e] = __uint_as_float(a[e]);
+      x[4 + e] = __uint_as_float(b[e]);
+    } else {
+      x[2 * e] = tm_act::bf16_lo(a[e]);
+      x[2 * e + 1] = tm_act::bf16_hi(a[e]);
     }
   }
 }
 
-// Eight bf16 or fp32 values of a row; `left` of them exist, vec: 16-byte pieces.
-__device__ __forceinline__ void get8(float (&x)[8], const char* p, bool f32, int left, bool vec) {
-  if (vec && left >= 8) {
-    if (f32) {
-      const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(p);
-      x[0] = tm_act::bf16_lo(a.x); x[1] = tm_act::bf16_hi(a.x);
-      x[2] = tm_act::bf16_lo(a.y); x[3] = tm_act::bf16_hi(a.y);
-      x[4] = tm_act::bf16_lo(a.z); x[5] = tm_act::bf16_hi(a.z);
-      x[6] = tm_act::bf16_lo(a.w); x[7] = tm_act::bf16_hi(a.w);
-    }
+__device__ __forceinline__ void put8(char* p, const float* x, bool f32) {  // 16-byte aligned
+  if (f32) {
+    reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
+    reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = 0.0f;
-      if (e < left)
-        x[e] = f32 ? reinterpret_cast<const float*>(p)[e]
-                   : __uint_as_float(static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << 16);
-    }
+    *reinterpret_cast<u32x4*>(p) =
+        u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
   }
 }
 
 __device__ __forceinline__ void put8(char* p, const float* x, bool f32, int left, bool vec) {
-  if (f32) {
-    if (vec && left >= 8) {
-      reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-      reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) reinterpret_cast<float*>(p)[e] = x[e];
-    }
+  if (vec && left >= 8) {
+    put8(p, x, f32);
   } else {
-    const u32x4 w = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
-    if (vec && left >= 8) {
-      *reinterpret_cast<u32x4*>(p) = w;
-    } else {
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < left) reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(u[e / 2] >> (16 * (e & 1)));
-    }
+    for (int e = 0; e < 8; ++e)
+      if (e < left) {
+        if (f32) reinterpret_cast<float*>(p)[e] = x[e];
+        else reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(pack_bf16(x[e], 0.0f));
+      }
   }
 }
 
@@ -215,21 +333,21 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
   return v;
 }
 
-// Where a lane's values of a block are, and which of them exist.
+// Where a block is, and which of a lane's values exist (kWhole: all).
 struct Spot {
-  int64_t m;        // first row; the second is 16 on
-  int n, cols;      // first column; columns left from it
+  int m0, n0;
+  int cols;     // columns left from the lane's first
   bool row[2];
 };
 
-__device__ __forceinline__ Spot spot_of(ArgsPtr g, int m0, int n0, int lane) {
-  Spot s;
-  s.m = m0 + (lane >> 2);
-  s.n = n0 + 8 * (lane & 3);
-  s.cols = g->n - s.n;
-  s.row[0] = s.m < g->m;
-  s.row[1] = s.m + 16 < g->m;
-  return s;
+__device__ __forceinline__ Spot spot_of(const End& g, int m0, int n0, int lane) {
+  const int m = m0 + (lane >> 2);
+  return {m0, n0, g.n - n0 - 8 * (lane & 3), {m < g.m, m + 16 < g.m}};
+}
+
+// A block's first element, row half i, of a matrix with rows ld elements of `size` bytes apart.
+__device__ __forceinline__ char* at_block(const char* p, int64_t ld, int size, const Spot& s, int i) {
+  return const_cast<char*>(p) + ((static_cast<int64_t>(s.m0) + 16 * i) * ld + s.n0) * size;
 }
 
 __device__ __forceinline__ void mask(Block& b, const Spot& s) {
@@ -238,14 +356,20 @@ __device__ __forceinline__ void mask(Block& b, const Spot& s) {
     if (!s.row[i / 8] || i % 8 >= s.cols) b.v[i] = 0.0f;
 }
 
-// A block as the backward pass reads it (its values outside the matrix zero): z's padding columns are
-// written too.
-__device__ __forceinline__ void hold(ArgsPtr g, const Block& b, const Spot& s, int m0, int n0, char* z, uint8_t* exps,
+__device__ __forceinline__ int64_t exponent_at(const End& g, const Spot& s) {
+  return static_cast<int64_t>(s.m0 >> 5) * g.blocks + (s.n0 >> 5);
+}
+
+// A block as the backward pass reads it (its values outside the matrix zero): the padding columns are written
+// too.
+template <bool kWhole>
+__device__ __forceinline__ void hold(const End& g, const Lane& l, const Block& b, const Spot& s, char* z, uint8_t* exps,
                                      int lane) {
-  if (g->held == TM_HELD_BF16) {
+  if (g.held == TM_HELD_BF16) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (s.row[i] && s.n < g->ldz) put8(z + ((s.m + 16 * i) * g->ldz + s.n) * 2, b.v + 8 * i, false, 8, true);
+      if (kWhole || (s.row[i] && s.n0 + 8 * (lane & 3) < g.ldz))
+        put8(at_block(z, g.ldz, 2, s, i) + l.z, b.v + 8 * i, false);
   } else {
     uint32_t most = 0;
 #pragma unroll
@@ -256,53 +380,84 @@ __device__ __forceinline__ void hold(ArgsPtr g, const Block& b, const Spot& s, i
     for (int i = 0; i < 2; ++i) {
       const float* x = b.v + 8 * i;
       const u32x2 w = {tm_act::encode4(x[0], x[1], x[2], x[3], inv), tm_act::encode4(x[4], x[5], x[6], x[7], inv)};
-      if (s.row[i]) *reinterpret_cast<u32x2*>(z + (s.m + 16 * i) * g->ldz + s.n) = w;
+      if (kWhole || s.row[i]) *reinterpret_cast<u32x2*>(at_block(z, g.ldz, 1, s, i) + l.z) = w;
     }
-    if (lane == 0) exps[static_cast<int64_t>(m0 >> 5) * g->blocks + (n0 >> 5)] = static_cast<uint8_t>(e + 127);
+    if (lane == 0) exps[exponent_at(g, s)] = static_cast<uint8_t>(e + 127);
   }
 }
 
-__device__ __forceinline__ void held_block(ArgsPtr g, Block& b, const Spot& s, int m0, int n0, const char* z,
-                                           const uint8_t* exps) {
-  if (g->held == TM_HELD_BF16) {
+// What a block's end reads from memory: the residual, or the gate's and up's products. (Whole tiles' is read
+// while the block before it is worked on.)
+struct Early {
+  Raw8 a[2], b[2];  // [row half]
+  uint32_t exps[2];
+};
+
+template <int kMode, bool kWhole>
+__device__ __forceinline__ Early early_of(const End& g, const Lane& l, int m0, int n0, int lane) {
+  Early r = {};
+  if (!kWhole && (m0 >= g.m || n0 >= g.n)) return r;
+  const Spot s = spot_of(g, m0, n0, lane);
+  if constexpr (kMode <= kResidual) {
+    if (kMode == kLinear && !g.res) return r;
+    const int size = g.res_f32 ? 4 : 2;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float x[8] = {};
-      if (s.row[i] && s.n < g->ldz) get8(x, z + ((s.m + 16 * i) * g->ldz + s.n) * 2, false, 8, true);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b.v[8 * i + e] = x[e];
+      const char* p = at_block(g.res, g.ldr, size, s, i);
+      if (kWhole) r.a[i] = raw8(p + l.res, g.res_f32);
+      else if (s.row[i] && s.cols > 0)
+        r.a[i] = raw8(p + (static_cast<int64_t>(lane >> 2) * g.ldr + 8 * (lane & 3)) * size, g.res_f32, s.cols, g.res_vec);
     }
-  } else {
-    const float scale =
-        tm_act::two_to(static_cast<int>(exps[static_cast<int64_t>(m0 >> 5) * g->blocks + (n0 >> 5)]) - 127);
+  }
+  if constexpr (kMode == kGateGrad) {
+    const bool bf16 = g.held == TM_HELD_BF16;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      u32x2 w = {0, 0};
-      if (s.row[i]) w = *reinterpret_cast<const u32x2*>(z + (s.m + 16 * i) * g->ldz + s.n);
-      const f32x4 lo = tm_act::decode4(w.x, scale), hi = tm_act::decode4(w.y, scale);
-      float* x = b.v + 8 * i;
-      x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
-      x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+      if (!kWhole && !(s.row[i] && (!bf16 || s.n0 + 8 * (lane & 3) < g.ldz))) continue;
+      const char *pg = at_block(g.z0, g.ldz, bf16 ? 2 : 1, s, i), *pu = at_block(g.z1, g.ldz, bf16 ? 2 : 1, s, i);
+      if (bf16) {
+        r.a[i].w[0] = *reinterpret_cast<const u32x4*>(pg + l.z);
+        r.b[i].w[0] = *reinterpret_cast<const u32x4*>(pu + l.z);
+      } else {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(pg + l.z), y = *reinterpret_cast<const u32x2*>(pu + l.z);
+        r.a[i].w[0] = u32x4{x.x, x.y, 0, 0};
+        r.b[i].w[0] = u32x4{y.x, y.y, 0, 0};
+      }
     }
+    if (!bf16) {
+      r.exps[0] = g.s0[exponent_at(g, s)];
+      r.exps[1] = g.s1[exponent_at(g, s)];
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ void add_residual(const End& g, Block& b, const Early& early) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float x[8];
+    values8(x, early.a[i], g.res_f32);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b.v[8 * i + e] += x[e];
   }
 }
 
 // y = act(z + b) + r, and z as it is kept. The products' fp32 sums are rounded once, in y's type; z
 // is rounded to what the backward pass reads.
-__device__ __forceinline__ void end_linear(ArgsPtr g, Block& b, int m0, int n0, int lane) {
-  if (m0 >= g->m || n0 >= g->n) return;
-  const Spot s = spot_of(g, m0, n0, lane);
-  if (g->bias) {
+template <bool kWhole>
+__device__ __forceinline__ void end_linear(const End& g, const Lane& l, Block& b, const Spot& s, const Raw8& bias,
+                                           const Early& early, int lane) {
+  if (g.bias) {
     float x[8];
-    get8(x, g->bias + static_cast<int64_t>(s.n) * (g->bias_f32 ? 4 : 2), g->bias_f32, s.cols, g->bias_vec);
+    values8(x, bias, g.bias_f32);
 #pragma unroll
     for (int i = 0; i < 16; ++i) b.v[i] += x[i % 8];
   }
-  if (g->held) {
-    if (m0 + 32 > g->m || n0 + 32 > g->n) mask(b, s);
-    hold(g, b, s, m0, n0, g->z0, g->s0, lane);
+  if (g.held) {
+    if (!kWhole) mask(b, s);
+    hold<kWhole>(g, l, b, s, g.z0, g.s0, lane);
   }
-  const int act = g->act;
+  const int act = g.act;
   auto each = [&](auto f) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) b.v[i] = f(b.v[i]);
@@ -311,99 +466,152 @@ __device__ __forceinline__ void end_linear(ArgsPtr g, Block& b, int m0, int n0, 
   else if (act == tm_act::kSilu) each([](float z) { return tm_act::act1(tm_act::kSilu, z); });
   else if (act == tm_act::kGelu) each([](float z) { return tm_act::act1(tm_act::kGelu, z); });
   else if (act == tm_act::kGeluTanh) each([](float z) { return tm_act::act1(tm_act::kGeluTanh, z); });
-  const int size_r = g->res_f32 ? 4 : 2, size_o = g->out_f32 ? 4 : 2;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    if (!s.row[i] || s.cols <= 0) continue;
-    if (g->res) {
-      float x[8];
-      get8(x, g->res + ((s.m + 16 * i) * g->ldr + s.n) * size_r, g->res_f32, s.cols, g->res_vec);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) b.v[8 * i + e] += x[e];
-    }
-    put8(g->o0 + ((s.m + 16 * i) * g->ldo + s.n) * size_o, b.v + 8 * i, g->out_f32, s.cols, g->out_vec);
-  }
+  if (g.res) add_residual(g, b, early);
 }
 
-__device__ __forceinline__ void end_plain(ArgsPtr g, int batch, Block& b, int m0, int n0, int lane) {
-  if (m0 >= g->m || n0 >= g->n) return;
-  const Spot s = spot_of(g, m0, n0, lane);
-  const int size_o = g->out_f32 ? 4 : 2;
-  char* out = batch ? g->o1 : g->o0;
+// A block of y, of a gradient: kWhole, in 16-byte pieces.
+template <bool kWhole>
+__device__ __forceinline__ void store_block(const End& g, const Lane& l, char* out, const Block& b, const Spot& s, int lane) {
+  const int size = g.out_f32 ? 4 : 2;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if (s.row[i] && s.cols > 0)
-      put8(out + ((s.m + 16 * i) * g->ldo + s.n) * size_o, b.v + 8 * i, g->out_f32, s.cols, g->out_vec);
+  for (int i = 0; i < 2; ++i) {
+    char* p = at_block(out, g.ldo, size, s, i);
+    if (kWhole) put8(p + l.out, b.v + 8 * i, g.out_f32);
+    else if (s.row[i] && s.cols > 0)
+      put8(p + (static_cast<int64_t>(lane >> 2) * g.ldo + 8 * (lane & 3)) * size, b.v + 8 * i, g.out_f32, s.cols,
+           g.out_vec);
+  }
 }
 
 // h = silu(g) u of 32 features, g and u kept on the way. Columns of padding are zeros.
-__device__ __forceinline__ void end_gate(ArgsPtr g, Block& gate, Block& up, int m0, int n0, int lane) {
-  if (m0 >= g->m || n0 >= g->n_store) return;
-  const Spot s = spot_of(g, m0, n0, lane);
-  if (m0 + 32 > g->m || n0 + 32 > g->n) {
+template <bool kWhole>
+__device__ __forceinline__ void end_gate(const End& g, const Lane& l, Block& gate, Block& up, const Spot& s, int lane) {
+  if (!kWhole) {
     mask(gate, s);
     mask(up, s);
   }
-  if (g->held && n0 < g->n) {
-    hold(g, gate, s, m0, n0, g->z0, g->s0, lane);
-    hold(g, up, s, m0, n0, g->z1, g->s1, lane);
+  if (g.held && s.n0 < g.n) {
+    hold<kWhole>(g, l, gate, s, g.z0, g.s0, lane);
+    hold<kWhole>(g, l, up, s, g.z1, g.s1, lane);
   }
 #pragma unroll
   for (int i = 0; i < 16; ++i) gate.v[i] = gate.v[i] * tm_act::sigmoid(gate.v[i]) * up.v[i];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (s.row[i] && s.n < g->n_store)
-      put8(g->o0 + ((s.m + 16 * i) * g->ldo + s.n) * 2, gate.v + 8 * i, false, 8, true);
+    if (kWhole || (s.row[i] && s.n0 + 8 * (lane & 3) < g.n_store))
+      put8(at_block(g.o0, g.ldo, 2, s, i) + l.out, gate.v + 8 * i, false);
 }
 
 // From dh: d_gate and d_up (columns 0.. and n_store.. of o0's rows) and silu(g) u (o1), g and u as held.
-__device__ __forceinline__ void end_gate_grad(ArgsPtr g, Block& d, int m0, int n0, int lane) {
-  if (m0 >= g->m || n0 >= g->n_store) return;
-  const Spot s = spot_of(g, m0, n0, lane);
-  Block gate = {}, up = {};
-  if (n0 < g->n) {
-    held_block(g, gate, s, m0, n0, g->z0, g->s0);
-    held_block(g, up, s, m0, n0, g->z1, g->s1);
-  }
-  if (n0 + 32 > g->n) mask(d, s);  // g and u are zero there
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float z = gate.v[i], q = tm_act::sigmoid(z), a = z * q;
-    gate.v[i] = d.v[i] * up.v[i] * tm_act::silu_grad(z, q);
-    d.v[i] *= a;
-    up.v[i] *= a;
+template <bool kWhole>
+__device__ __forceinline__ void end_gate_grad(const End& g, const Lane& l, Block& d, const Spot& s, const Early& early,
+                                              int lane) {
+  if (!kWhole && s.n0 + 32 > g.n) mask(d, s);  // g and u are zero there
+  const bool bf16 = g.held == TM_HELD_BF16;
+  float sg = 1.0f, su = 1.0f;
+  if (!bf16 && s.n0 < g.n) {
+    sg = tm_act::two_to(static_cast<int>(early.exps[0]) - 127);
+    su = tm_act::two_to(static_cast<int>(early.exps[1]) - 127);
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    if (!s.row[i] || s.n >= g->n_store) continue;
-    char* o = g->o0 + ((s.m + 16 * i) * g->ldo + s.n) * 2;
-    put8(o, gate.v + 8 * i, false, 8, true);
-    put8(o + static_cast<int64_t>(g->n_store) * 2, d.v + 8 * i, false, 8, true);
-    if (g->o1) put8(g->o1 + ((s.m + 16 * i) * g->ldo1 + s.n) * 2, up.v + 8 * i, false, 8, true);
+    float z[8], u[8];
+    if (bf16) {
+      values8(z, early.a[i], false);
+      values8(u, early.b[i], false);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const f32x4 x = tm_act::decode4(e ? early.a[i].w[0].y : early.a[i].w[0].x, sg);
+        const f32x4 y = tm_act::decode4(e ? early.b[i].w[0].y : early.b[i].w[0].x, su);
+        z[4 * e] = x.x; z[4 * e + 1] = x.y; z[4 * e + 2] = x.z; z[4 * e + 3] = x.w;
+        u[4 * e] = y.x; u[4 * e + 1] = y.y; u[4 * e + 2] = y.z; u[4 * e + 3] = y.w;
+      }
+    }
+    float* dh = d.v + 8 * i;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float q = tm_act::sigmoid(z[e]), a = z[e] * q;
+      z[e] = dh[e] * u[e] * tm_act::silu_grad(z[e], q);
+      dh[e] *= a;
+      u[e] *= a;
+    }
+    if (kWhole || (s.row[i] && s.n0 + 8 * (lane & 3) < g.n_store)) {
+      char* o = at_block(g.o0, g.ldo, 2, s, i);
+      put8(o + l.out, z, false);
+      put8(o + static_cast<int64_t>(g.n_store) * 2 + l.out, dh, false);
+      if (g.o1) put8(at_block(g.o1, g.ldo1, 2, s, i) + l.out1, u, false);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // one half's values at a time
   }
 }
 
-// The blocks acc(0) .. acc(kBlocks - 1) of a wave, block b at row m(b), column n(b). One copy of the ends: a
-// loop over the blocks whose first step picks the block's registers.
-template <int kMode, bool kHalves, int kNB, int kMBs>
-__device__ __forceinline__ void finish(f32x16 (&acc)[kMBs][kNB], int batch, int m0, int n0, int lane, uint32_t stg) {
-  ArgsPtr g = (ArgsPtr)__builtin_amdgcn_kernarg_segment_ptr();
-  asm volatile("" : "+s"(g));  // read again for each tile: held in registers through the product they spill
-  constexpr int kPer = kMode == kGate ? 2 : 1;
+template <int kMode, bool kWhole>
+__device__ __forceinline__ void end_block(const End& g, const Lane& l, int batch, Block& x, Block& y, int m, int n,
+                                          const Raw8& bias, const Early& early, int lane) {
+  const Spot s = spot_of(g, m, n, lane);
+  if constexpr (kMode == kLinear) end_linear<kWhole>(g, l, x, s, bias, early, lane);
+  if constexpr (kMode == kResidual) add_residual(g, x, early);
+  if constexpr (kMode <= kPlain) store_block<kWhole>(g, l, kMode == kPlain && batch ? g.o1 : g.o0, x, s, lane);
+  else if constexpr (kMode == kGate) end_gate<kWhole>(g, l, x, y, s, lane);
+  else end_gate_grad<kWhole>(g, l, x, s, early, lane);
+}
+
+// A wave's blocks, of which the first is at row m0, column n0, down each column of blocks. Of tiles inside the
+// matrix, one after the other in straight code (but for kLinear, whose code is long); else in a loop whose
+// first step picks the block's registers. No register may spill here: a spill's reload waits for all
+// stores before it.
+template <int kMode, bool kHalves, int kRowBlocks, int kColBlocks>
+__device__ __forceinline__ void finish(f32x4 (&acc)[2 * kRowBlocks][2 * kColBlocks], int batch, int m0, int n0, int lane,
+                                       uint32_t stg) {
+  const End g = end_of<kMode>();
+  asm volatile("" : "+v"(lane));  // what derives from it is made again for each tile: kept, it spills
+  const Lane l = lane_of<kMode>(g, stg, lane);
+  constexpr int kPer = kMode == kGate ? 2 : 1, kCols = kColBlocks / kPer, kBlocks = kRowBlocks * kCols;
+  constexpr bool kReads = kMode == kResidual || kMode == kGateGrad;
+  bool whole = m0 + 32 * kRowBlocks <= g.m && n0 + 32 * kCols <= g.n;
+  if (kMode <= kPlain) whole = whole && g.out_vec;
+  if (kMode == kResidual) whole = whole && g.res_vec;
+  auto pick = [&](Block& x, Block& y, int c) {
+    const int jj = 2 * (c % kRowBlocks), ii = 2 * kPer * (c / kRowBlocks);
+    const f32x4 t[2][2] = {{acc[jj][ii], acc[jj][ii + 1]}, {acc[jj + 1][ii], acc[jj + 1][ii + 1]}};
+    to_rows<kHalves>(x, t, l);
+    if constexpr (kMode == kGate) {
+      const f32x4 u[2][2] = {{acc[jj][ii + 2], acc[jj][ii + 3]}, {acc[jj + 1][ii + 2], acc[jj + 1][ii + 3]}};
+      to_rows<kHalves>(y, u, l);
+    }
+  };
+  if (kMode != kLinear && whole) {
+    Early early;
+    if constexpr (kReads) early = early_of<kMode, true>(g, l, m0, n0, lane);
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+      Block x, y;
+      pick(x, y, b);
+      const Early now = early;
+      if (kReads && b + 1 < kBlocks)
+        early = early_of<kMode, true>(g, l, m0 + (b + 1) % kRowBlocks * 32, n0 + (b + 1) / kRowBlocks * 32, lane);
+      end_block<kMode, true>(g, l, batch, x, y, m0 + b % kRowBlocks * 32, n0 + b / kRowBlocks * 32, Raw8{}, now, lane);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    return;
+  }
+  Raw8 bias = {};
 #pragma unroll 1
-  for (int b = 0; b < kMBs * kNB / kPer; ++b) {
+  for (int b = 0; b < kBlocks; ++b) {
+    const int m = m0 + b % kRowBlocks * 32, n = n0 + b / kRowBlocks * 32;
+    if constexpr (kMode == kLinear)
+      if (g.bias && b % kRowBlocks == 0)
+        bias = raw8(g.bias + (static_cast<int64_t>(n) + 8 * (lane & 3)) * (g.bias_f32 ? 4 : 2), g.bias_f32,
+                    g.n - n - 8 * (lane & 3), g.bias_vec);
+    const Early early = early_of<kMode, false>(g, l, m, n, lane);
     Block x, y;
 #pragma unroll
-    for (int c = 0; c < kMBs * kNB / kPer; ++c)
-      if (b == c) {
-        to_rows<kHalves>(x, acc[c * kPer / kNB][c * kPer % kNB], stg, lane);
-        if constexpr (kMode == kGate) to_rows<kHalves>(y, acc[c * kPer / kNB][c * kPer % kNB + 1], stg, lane);
-      }
-    const int m = m0 + b * kPer / kNB * 32, n = n0 + (kMode == kGate ? 0 : b % kNB * 32);
-    if constexpr (kMode == kLinear) end_linear(g, x, m, n, lane);
-    else if constexpr (kMode == kPlain) end_plain(g, batch, x, m, n, lane);
-    else if constexpr (kMode == kGate) end_gate(g, x, y, m, n, lane);
-    else end_gate_grad(g, x, m, n, lane);
+    for (int c = 0; c < kBlocks; ++c)
+      if (b == c) pick(x, y, c);
+    if (m >= g.m || n >= (kMode >= kGate ? g.n_store : g.n)) continue;
+    if (kMode == kLinear && whole) end_block<kMode, kMode == kLinear>(g, l, batch, x, y, m, n, bias, early, lane);
+    else end_block<kMode, false>(g, l, batch, x, y, m, n, bias, early, lane);
   }
 }
 
@@ -411,31 +619,164 @@ __device__ __forceinline__ void finish(f32x16 (&acc)[kMBs][kNB], int batch, int 
 
 template <int kMB, int kNB>
 struct Tile {
-  static constexpr int kTM = 64 * kMB, kTN = 128 * kNB, kStage = (kTM + kTN) * 128;
-  static constexpr bool kHalves = kMB * kNB == 2;         // 80 KB: two workgroups a CU
-  static constexpr int kStrip = kHalves ? 2048 : 4096;  // one wave's
-  static constexpr int kLds = 2 * kStage + 8 * kStrip;
+  static constexpr int kTM = 64 * kMB, kTN = 128 * kNB;
+  static constexpr int kUnit = (kTM > kTN ? kTM : kTN) * kSliceK * 2;  // LDS for one operand's slice
+  static constexpr int kStrip = kUnit / 8 < 4096 ? 2048 : 4096;        // one wave's, in a unit just used up
+  static constexpr bool kHalves = kStrip == 2048;
+  static constexpr int kLds = kUnits * kUnit;  // 80 KB (two workgroups a CU) or 160 KB
 };
 
-// Position -> split, batch and the tile's first row and column (gate: feature).
+// a / d and the remainder, for 0 <= a < 2^22: the estimate is off by at most one.
+__device__ __forceinline__ int divide(int a, int d, int& rem) {
+  int q = static_cast<int>(static_cast<float>(a) * __builtin_amdgcn_rcpf(static_cast<float>(d)));
+  rem = a - q * d;
+  if (rem < 0) {
+    --q;
+    rem += d;
+  } else if (rem >= d) {
+    ++q;
+    rem -= d;
+  }
+  return q;
+}
+
+// Position -> split, batch and the tile's first row and column (gate: feature): n-blocks of gn tile
+// columns; inside each, m-blocks of gm tile rows, a block's gm x gn tiles consecutive.
 template <int kTM, int kTN, bool kHalf>
 __device__ __forceinline__ void place(const Args& g, int p, int& split, int& batch, int& m0, int& n0) {
-  const int tb = g.tiles_m * g.tiles_n, t_all = tb * g.batch;
-  split = p / t_all;
-  const int t = p - split * t_all;
-  batch = t / tb;
-  int tm, tn;
-  tile_of(t - batch * tb, g.tiles_m, g.tiles_n, g.gm, g.gn, tm, tn);
+  split = batch = 0;
+  const int tb = g.tiles_m * g.tiles_n;
+  if (g.splits > 1) split = divide(p, tb * g.batch, p);
+  if (g.batch > 1) batch = divide(p, tb, p);
+  int rem, tn;
+  const int nb = divide(p, g.tiles_m * g.gn, rem);
+  const int gn = min(g.gn, g.tiles_n - nb * g.gn);
+  const int mb = divide(rem, g.gm * gn, rem);
+  const int tm = mb * g.gm + divide(rem, gn, tn);
   m0 = tm * kTM;
-  n0 = tn * (kHalf ? kTN / 2 : kTN);
+  n0 = (nb * g.gn + tn) * (kHalf ? kTN / 2 : kTN);
 }
+
+// One operand's loads: a stream of units (the tile's kT rows or columns of 64 K) over the workgroup's
+// positions. Load j of wave w fills KB 8 j + w: K-contiguous, 8 rows of 128 bytes; K-major, whole K rows of
+// the tile's columns.
+template <int kT, bool kContig, bool kIsA, bool kPairs, int kTM, int kTN>
+struct Feed {
+  static constexpr int kLoads = kT / 64;
+  int lp, lit, lend;      // position; slice of the next one that is not plain; the position's last, + 1
+  int plain;              // slices before that: one after another, whole
+  const char* at;         // the operand at the next slice
+  int64_t step, col;
+  uint32_t off[kLoads];   // this lane's bytes past `at`
+
+  // the operand's row (or K row) and 16-byte chunk that a lane loads in KB q
+  static __device__ __forceinline__ void spot(int lane, int q, int& r, int& c) {
+    if constexpr (kContig) {
+      r = q * 8 + lane / 8;
+      c = (lane % 8) ^ ((r >> 1) & 7);
+    } else {
+      r = q * (512 / kT) + lane / (kT / 8);
+      c = (lane % (kT / 8)) ^ k_swizzle(r);
+    }
+  }
+  __device__ __forceinline__ int left(const Args& g) const {  // K that the operand holds from slice lit on
+    if constexpr (kIsA) return g.ka - lit * kSliceK;
+    else return g.kb - (!kContig && lit >= g.seg ? lit - g.seg : lit) * kSliceK;
+  }
+  __device__ __forceinline__ void count(const Args& g) {
+    int n = min(lend - 1 - lit, left(g) / kSliceK);
+    if (!kIsA && !kContig && lit < g.seg) n = min(n, g.seg - 1 - lit);
+    plain = max(n, 0);
+    lit += plain;
+  }
+  __device__ __forceinline__ void seek(const Args& g, int pos, int lane, int wave) {
+    asm volatile("" : "+v"(lane));  // derived again for each tile, not kept through the products
+    int split, batch, m0, n0;
+    place<kTM, kTN, kPairs>(g, pos, split, batch, m0, n0);
+    lp = pos;
+    lit = split * g.per;
+    lend = min(lit + g.per, g.slices);
+    const int64_t ld = kIsA ? g.a_ld : g.b_ld;
+    step = kContig ? kSliceK * 2 : kSliceK * ld;
+    if constexpr (kIsA) {
+      at = kContig ? g.a + m0 * ld + lit * step : g.a + batch * g.a_batch + static_cast<int64_t>(m0) * 2 + lit * step;
+    } else if constexpr (kContig) {
+      at = (kPairs && (wave & 4) ? g.b1 : g.b0) + n0 * ld + lit * step;  // KB 8 j + 4 .. 7: the up weight's rows
+    } else {
+      col = static_cast<int64_t>(n0) * 2;
+      at = lit >= g.seg ? g.b1 + col + (lit - g.seg) * step : g.b0 + col + lit * step;
+    }
+    const int most = kIsA ? g.a_rows - m0 : g.b_rows - n0;
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      int r, c;
+      spot(lane, 8 * j + wave, r, c);
+      if constexpr (kContig) {
+        const int row = kPairs && !kIsA ? (r >> 6) * 32 + (r & 31) : r;
+        off[j] = static_cast<uint32_t>(min(row, most - 1)) * static_cast<uint32_t>(ld) + c * 16;
+      } else {
+        off[j] = static_cast<uint32_t>(r) * static_cast<uint32_t>(ld) + min(8 * c, most - 8) * 2;
+      }
+    }
+  }
+  static __device__ __forceinline__ void to_lds(const char* from, uint8_t* unit, int j) {
+    __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)from,
+                                     (void __attribute__((address_space(3)))*)(unit + j * 8192), 16, 0, 0);
+  }
+  // `unit` is where this wave's first KB goes
+  __device__ __forceinline__ void load(uint8_t* unit, int j) const { to_lds(at + off[j], unit, j); }
+  __device__ __forceinline__ void next() {
+    at += step;
+    --plain;
+  }
+  // The slice that is not plain: the position's last, or one that reaches past the operand's K (zeros) or
+  // up to its other segment.
+  __device__ __forceinline__ void load_event(const Args& g, uint8_t* unit, int pend, int lane, int wave) {
+    const int k = left(g);
+    if (k >= kSliceK) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) load(unit, j);
+    } else {
+      int ln = lane;
+      asm volatile("" : "+v"(ln));
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) {
+        int r, c;
+        spot(ln, 8 * j + wave, r, c);
+        to_lds((kContig ? c * 8 : r) < k ? at + off[j] : reinterpret_cast<const char*>(&g_zeros), unit, j);
+      }
+    }
+    if (lit + 1 < lend) {
+      ++lit;
+      at += step;
+      if (!kIsA && !kContig && lit == g.seg) at = g.b1 + col;
+    } else if (lp + g.wpx < pend) {
+      seek(g, lp + g.wpx, lane, wave);
+    }  // else: the last slice again, which nothing reads
+    count(g);
+  }
+  __device__ __forceinline__ void load_all(const Args& g, uint8_t* unit, int pend, int lane, int wave) {
+    if (plain > 0) {
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) load(unit, j);
+      next();
+    } else {
+      load_event(g, unit, pend, lane, wave);
+    }
+  }
+};
+
+template <int kQ>
+struct Quarter {
+  static constexpr int q = kQ;
+};
 
 template <int kMB, int kNB, bool kAK, bool kBK, int kMode>
 __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const Args g) {
   using C = Tile<kMB, kNB>;
-  constexpr int kTM = C::kTM, kTN = C::kTN, kStage = C::kStage;
-  constexpr int kLoads = (kTM + kTN) / 64, kInA = kTM / 8, kInB = kTN / 8;
-  constexpr int kRdA = kAK ? kMB : 2 * kMB, kRdB = kBK ? kNB : 2 * kNB, kRd = kRdA + kRdB, kMf = kMB * kNB;
+  constexpr int kTM = C::kTM, kTN = C::kTN, kUnit = C::kUnit;
+  constexpr int kFB = 2 * kNB;  // B fragments, 16 columns each; A: two halves of kMB, 16 rows each
+  constexpr int kRdA = kAK ? kMB : 2 * kMB, kRdB = kBK ? kFB : 2 * kFB;
   constexpr bool kPairs = kMode == kGate;
   static_assert(!kPairs || (kNB == 2 && kBK), "gate and up columns alternate by 32 within a wave");
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
@@ -448,256 +789,174 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave >> 2, wn = wave & 3;
 
-  // ---- the loader's place: position lp, slice lit of lend, operand pointers at that slice
-  int lp = p, lit = 0, lend = 0;
-  const char *la = nullptr, *lb = nullptr, *lb2 = nullptr;
-  uint32_t off[kLoads];  // this lane's bytes past the operand's pointer, load j
-  const int64_t step_a = kAK ? kSliceK * 2 : kSliceK * g.a_ld, step_b = kBK ? kSliceK * 2 : kSliceK * g.b_ld;
-  int64_t col_b = 0;
-  // Load q = kLoads wave + j: 1 KB of A's stage (q < kInA), then of B's. K-contiguous: 8 rows;
-  // K-major: whole K rows of the tile's columns.
-  auto k_contig = [&](int qq, int& r, int& c) {
-    r = qq * 8 + lane / 8;
-    c = (lane % 8) ^ ((r >> 1) & 7);
-  };
-  auto k_major = [&](int qq, int cpr, int& kr, int& c) {
-    kr = qq * (64 / cpr) + lane / cpr;
-    c = (lane % cpr) ^ (4 * (kr & 3));
-  };
-  auto seek = [&](int pos) {
-    int split, batch, m0, n0;
-    place<kTM, kTN, kPairs>(g, pos, split, batch, m0, n0);
-    lit = split * g.per;
-    lend = min(lit + g.per, g.slices);
-    if constexpr (kAK) la = g.a + m0 * g.a_ld + static_cast<int64_t>(lit) * (kSliceK * 2);
-    else la = g.a + batch * g.a_batch + static_cast<int64_t>(m0) * 2 + lit * step_a;
-    if constexpr (kBK) {
-      const int64_t at = n0 * g.b_ld + static_cast<int64_t>(lit) * (kSliceK * 2);
-      lb = g.b0 + at;
-      if constexpr (kPairs) lb2 = g.b1 + at;
-    } else {
-      col_b = static_cast<int64_t>(n0) * 2;
-      lb = lit >= g.seg ? g.b1 + col_b + (lit - g.seg) * step_b : g.b0 + col_b + lit * step_b;
-    }
-    const int left_a = g.a_rows - m0, left_b = g.b_rows - n0;
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int q = wave * kLoads + j;
-      int r, c;
-      if (q < kInA) {
-        if constexpr (kAK) {
-          k_contig(q, r, c);
-          off[j] = static_cast<uint32_t>(min(r, left_a - 1)) * static_cast<uint32_t>(g.a_ld) + c * 16;
-        } else {
-          k_major(q, kTM / 8, r, c);
-          off[j] = static_cast<uint32_t>(r) * static_cast<uint32_t>(g.a_ld) + min(8 * c, left_a - 8) * 2;
-        }
-      } else {
-        if constexpr (kBK) {
-          k_contig(q - kInA, r, c);
-          const int row = kPairs ? (r >> 6) * 32 + (r & 31) : r;
-          off[j] = static_cast<uint32_t>(min(row, left_b - 1)) * static_cast<uint32_t>(g.b_ld) + c * 16;
-        } else {
-          k_major(q - kInA, kTN / 8, r, c);
-          off[j] = static_cast<uint32_t>(r) * static_cast<uint32_t>(g.b_ld) + min(8 * c, left_b - 8) * 2;
-        }
-      }
-    }
-  };
-  auto advance = [&]() {
-    if (lit + 1 < lend) {
-      ++lit;
-      la += step_a;
-      if (!kBK && lit == g.seg) lb = g.b1 + col_b;
-      else lb += step_b;
-      if (kPairs) lb2 += step_b;
-    } else if (lp + g.wpx < pend) {
-      lp += g.wpx;
-      seek(lp);
-    }  // else: the last slice again, which nothing reads
-  };
-  auto to_lds = [&](const char* from, int stage, int q) {
-    __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)from,
-                                     (void __attribute__((address_space(3)))*)(smem + stage * kStage + q * 1024), 16, 0, 0);
-  };
-  auto source = [&](int j) {
-    const int q = wave * kLoads + j;
-    if (q < kInA) return la + off[j];
-    if (kPairs && (((q - kInA) >> 2) & 1)) return lb2 + off[j];
-    return lb + off[j];
-  };
-  auto load = [&](int stage, int j) { to_lds(source(j), stage, wave * kLoads + j); };
-  // whether the loader's slice reaches past an operand's K; its loads then
-  auto ragged = [&]() {
-    const int kb0 = !kBK && lit >= g.seg ? lit - g.seg : lit;
-    return (lit + 1) * kSliceK > g.ka || (kb0 + 1) * kSliceK > g.kb;
-  };
-  auto load_ragged = [&](int stage) {
-    const int kb0 = !kBK && lit >= g.seg ? lit - g.seg : lit;
-#pragma unroll
-    for (int j = 0; j < kLoads; ++j) {
-      const int q = wave * kLoads + j;
-      int r, c;
-      bool in;
-      if (q < kInA) {
-        if constexpr (kAK) {
-          k_contig(q, r, c);
-          in = lit * kSliceK + c * 8 < g.ka;
-        } else {
-          k_major(q, kTM / 8, r, c);
-          in = lit * kSliceK + r < g.ka;
-        }
-      } else {
-        if constexpr (kBK) {
-          k_contig(q - kInA, r, c);
-          in = lit * kSliceK + c * 8 < g.kb;
-        } else {
-          k_major(q - kInA, kTN / 8, r, c);
-          in = kb0 * kSliceK + r < g.kb;
-        }
-      }
-      to_lds(in ? source(j) : reinterpret_cast<const char*>(&g_zeros), stage, q);
-    }
-  };
-
-  // ---- fragments: K-contiguous, row lane % 32 of a block, chunk 2 kk + lane / 32; K-major, two
-  // transposing reads (K rows +0 and +4) of 8-byte pieces
+  // ---- fragments of v_mfma_f32_16x16x32_bf16: lane l has row (column) l % 16, K 8 (l / 16) .. + 7.
+  // K-contiguous: chunk 4 t + l / 16 of its row, t the K32 step. K-major: two transposing reads (K rows +0
+  // and +4), lane l addressing the 8-byte piece l % 4 of K row 32 t + 8 (l / 16) + l / 4 % 4; the swizzle
+  // puts the 8 K rows and 2 chunks that 32 lanes read on 16 bank groups.
   const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem));
-  const int tx = (lane >> 5) ^ ((lane >> 1) & 7);
-  uint32_t vk[4];
-#pragma unroll
-  for (int kk = 0; kk < 4; ++kk) vk[kk] = lds0 + (lane & 31) * 128 + (((2 * kk) ^ tx) * 16);
-  const int s16 = lane & 15, s4 = s16 >> 2;
-  const int lcf = ((lane >> 4) & 1) * 2 + ((s16 & 3) >> 1);
-  uint32_t ba[kMB], bb[kNB];
-#pragma unroll
-  for (int i = 0; i < kMB; ++i)
-    ba[i] = lds0 + (8 * (lane >> 5) + s4) * (kTM * 2) + (s16 & 1) * 8 + (4 * ((wm * kMB + i) ^ s4) + lcf) * 16;
-#pragma unroll
-  for (int i = 0; i < kNB; ++i)
-    bb[i] = lds0 + kInA * 1024 + (8 * (lane >> 5) + s4) * (kTN * 2) + (s16 & 1) * 8 +
-            (4 * ((wn * kNB + i) ^ s4) + lcf) * 16;
-  const uint32_t off_a = wm * kMB * 32 * 128, off_b = kInA * 1024 + wn * kNB * 32 * 128;
+  const int kr = 8 * (lane >> 4) + ((lane >> 2) & 3);
+  const uint32_t vc = (lane & 15) * 128 + (((lane >> 4) ^ ((lane >> 1) & 7)) << 4);  // step 1: chunk ^ 4
+  const uint32_t base_a = lds0 + (kAK ? vc + wm * kMB * 32 * 128 : kr * (kTM * 2) + (lane & 1) * 8);
+  const uint32_t base_b = lds0 + (kBK ? vc + wn * kNB * 32 * 128 : kr * (kTN * 2) + (lane & 1) * 8);
+  const int ksw = k_swizzle(kr), kc = (lane >> 1) & 1;
 #define TM_RD(dst, base, imm) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(dst) : "v"(base), "i"(imm))
 #define TM_TR(dst, base, imm) asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(dst) : "v"(base), "i"(imm))
-  bf16x8 a8[2][kAK ? kMB : 1], b8[2][kBK ? kNB : 1];
-  bf16x4 a4[2][kAK ? 1 : 2 * kMB], b4[2][kBK ? 1 : 2 * kNB];
-  auto rd = [&](int z, uint32_t so, int kk, int i) {
-    if (i < kRdA) {
-      if constexpr (kAK) TM_RD(a8[z][i], vk[kk] + so + off_a, i * 32 * 128);
-      else TM_TR(a4[z][i], ba[i >> 1] + so, kk * 16 * kTM * 2 + (i & 1) * 4 * kTM * 2);
-    } else {
-      const int h = i - kRdA;
-      if constexpr (kBK) TM_RD(b8[z][h], vk[kk] + so + off_b, h * 32 * 128);
-      else TM_TR(b4[z][h], bb[h >> 1] + so, kk * 16 * kTN * 2 + (h & 1) * 4 * kTN * 2);
-    }
+  bf16x8 a8[2][kAK ? kMB : 1], b8[2][kBK ? kFB : 1];
+  bf16x4 a4[2][kAK ? 1 : 2 * kMB], b4[2][kBK ? 1 : 2 * kFB];
+  auto rd_a = [&](int t, int h, uint32_t ua, int i) {  // read i of step t, half h, from the unit at ua
+    if constexpr (kAK) TM_RD(a8[h][i], (base_a ^ (t * 64)) + ua, (h * kMB + i) * 16 * 128);
+    else
+      TM_TR(a4[h][i], base_a + ua + ((2 * (wm * 2 * kMB + h * kMB + (i >> 1)) + kc) ^ ksw) * 16,
+            t * 64 * kTM + (i & 1) * 4 * kTM * 2);
   };
-  // waits for set z's reads; naming every fragment keeps the MFMAs that use them behind the wait
-  auto wait = [&](int z) {
+  auto rd_b = [&](int t, uint32_t ub, int i) {
+    if constexpr (kBK) TM_RD(b8[t][i], (base_b ^ (t * 64)) + ub, i * 16 * 128);
+    else
+      TM_TR(b4[t][i], base_b + ub + ((2 * (wn * kFB + (i >> 1)) + kc) ^ ksw) * 16,
+            t * 64 * kTN + (i & 1) * 4 * kTN * 2);
+  };
+  // waits for the reads of A's half h and (t >= 0) of B's step t; naming every fragment keeps the MFMAs that
+  // use them behind the wait
+  auto wait = [&](int h, int t) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
     for (int i = 0; i < kRdA; ++i) {
-      if constexpr (kAK) asm volatile("" : "+v"(a8[z][i]));
-      else asm volatile("" : "+v"(a4[z][i]));
+      if constexpr (kAK) asm volatile("" : "+v"(a8[h][i]));
+      else asm volatile("" : "+v"(a4[h][i]));
     }
+    if (t >= 0)
 #pragma unroll
-    for (int i = 0; i < kRdB; ++i) {
-      if constexpr (kBK) asm volatile("" : "+v"(b8[z][i]));
-      else asm volatile("" : "+v"(b4[z][i]));
-    }
+      for (int i = 0; i < kRdB; ++i) {
+        if constexpr (kBK) asm volatile("" : "+v"(b8[t][i]));
+        else asm volatile("" : "+v"(b4[t][i]));
+      }
   };
-  auto afrag = [&](int z, int i) {
-    if constexpr (kAK) return a8[z][i];
-    else return __builtin_shufflevector(a4[z][2 * i], a4[z][2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+  auto afrag = [&](int h, int i) {
+    if constexpr (kAK) return a8[h][i];
+    else return __builtin_shufflevector(a4[h][2 * i], a4[h][2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  auto bfrag = [&](int z, int i) {
-    if constexpr (kBK) return b8[z][i];
-    else return __builtin_shufflevector(b4[z][2 * i], b4[z][2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-  auto load_slice = [&](int stage) {
-    if (ragged()) {
-      load_ragged(stage);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kLoads; ++j) load(stage, j);
-    }
-    advance();
+  auto bfrag = [&](int t, int i) {
+    if constexpr (kBK) return b8[t][i];
+    else return __builtin_shufflevector(b4[t][2 * i], b4[t][2 * i + 1], 0, 1, 2, 3, 4, 5, 6, 7);
   };
 
-  seek(p);
-  load_slice(0);
-  load_slice(1);
-  __builtin_amdgcn_s_waitcnt(waitcnt_vm(kLoads));
+  // ---- five units of LDS in a ring: A 0, B 0, A 1, B 1, A 2, ...
+  auto after = [&](uint32_t u, int n) {  // the unit n on
+    u += n * kUnit;
+    return u >= static_cast<uint32_t>(C::kLds) ? u - C::kLds : u;
+  };
+  uint8_t* const mine = smem + wave * 1024;
+  Feed<kTM, kAK, true, kPairs, kTM, kTN> fa;
+  Feed<kTN, kBK, false, kPairs, kTM, kTN> fb;
+  fa.seek(g, p, lane, wave);
+  fb.seek(g, p, lane, wave);
+  fa.count(g);
+  fb.count(g);
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    fa.load_all(g, mine + 2 * i * kUnit, pend, lane, wave);
+    fb.load_all(g, mine + (2 * i + 1) * kUnit, pend, lane, wave);
+  }
+  __builtin_amdgcn_s_waitcnt(waitcnt_vm(fa.kLoads + fb.kLoads));
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
+  uint32_t ua = 0, free_b = 4 * kUnit;  // the slice's A (its B is in the next unit); the unit of the last slice's B
 #pragma unroll
-  for (int i = 0; i < kRd; ++i) rd(0, 0, 0, i);
-  wait(0);
+  for (int i = 0; i < kRdA; ++i) rd_a(0, 0, 0, i);
+#pragma unroll
+  for (int i = 0; i < kRdB; ++i) rd_b(0, kUnit, i);
+  wait(0, 0);
   __builtin_amdgcn_sched_barrier(0);
 
-  uint32_t so = 0;  // the stage that holds the current slice
   for (;;) {
     int split, batch, m0, n0;
     place<kTM, kTN, kPairs>(g, p, split, batch, m0, n0);
     const int n_it = min(g.per, g.slices - split * g.per);
-    f32x16 acc[kMB][kNB];
+    f32x4 acc[2 * kMB][kFB];
 #pragma unroll
-    for (int i = 0; i < kMB; ++i)
+    for (int i = 0; i < 2 * kMB; ++i)
 #pragma unroll
-      for (int j = 0; j < kNB; ++j) acc[i][j] = f32x16{};
+      for (int j = 0; j < kFB; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // A slice is four quarters (K32 step t = q / 2, A's half h = q % 2); in each the operands of the next are
+    // read, early, so that the products that follow cover them. In the first, A two slices on is loaded
+    // into the unit that the last slice's B has left. Before the fourth the workgroup meets: every
+    // wave's loads of the next slice have come in, and nobody reads this slice's units any more, so
+    // that B two slices on may be loaded into A's.
     for (int it = 0; it < n_it; ++it) {
-      const uint32_t no = kStage - so;
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const int z = kk & 1;
-        bool late = false;  // loads already issued, before the products
-        if (kk == 3) {
-          __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));  // this wave's loads of the next slice are in LDS
-          __builtin_amdgcn_s_barrier();               // every wave's, and this slice's reads are done
-          __builtin_amdgcn_sched_barrier(0);
-          late = ragged();
-          if (late) load_ragged(so ? 1 : 0);
+      const uint32_t ub = after(ua, 1), na = after(ua, 2), nb = after(ua, 3);
+      auto quarter = [&](auto which) {
+        constexpr int q = decltype(which)::q, t = q / 2, h = q % 2;
+        constexpr int kMf = kMB * kFB, kReads = h == 0 ? kRdA : kRdA + kRdB;
+        constexpr int kPer = (4 * kReads + 3 * kMf - 1) / (3 * kMf);
+        constexpr int kLoads = q == 0 ? fa.kLoads : (q == 3 ? fb.kLoads : 0);
+        bool loads = false;
+        if (q == 0) {
+          loads = fa.plain > 0;
+          if (!loads) fa.load_event(g, mine + free_b, pend, lane, wave);
+        }
+        if (q == 3) {
+          loads = fb.plain > 0;
+          if (!loads) fb.load_event(g, mine + ua, pend, lane, wave);
         }
 #pragma unroll
-        for (int f = 0; f < kMf; ++f) {  // one MFMA, its share of the next step's reads and of the loads
+        for (int f = 0; f < kMf; ++f) {  // one MFMA, its share of the reads and of the loads
 #pragma unroll
-          for (int i = f * kRd / kMf; i < (f + 1) * kRd / kMf; ++i) {
-            if (kk < 3) rd(z ^ 1, so, kk + 1, i);
-            else rd(z ^ 1, no, 0, i);
+          for (int i = f * kPer; i < (f + 1) * kPer && i < kReads; ++i) {
+            if (h == 0) rd_a(t, 1, ua, i);
+            else if (i < kRdA) rd_a(t ^ 1, 0, q == 1 ? ua : na, i);
+            else rd_b(t ^ 1, q == 1 ? ub : nb, i - kRdA);
           }
-          if (kk == 3 && !late) {
+          if (kLoads && loads)
 #pragma unroll
-            for (int j = f * kLoads / kMf; j < (f + 1) * kLoads / kMf; ++j) load(so ? 1 : 0, j);
-          }
-          const int jj = f / kNB, ii = f % kNB;
-          acc[jj][ii] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bfrag(z, ii), afrag(z, jj), acc[jj][ii], 0, 0, 0);
+            for (int j = f * kLoads / kMf; j < (f + 1) * kLoads / kMf; ++j) {
+              if (q == 0) fa.load(mine + free_b, j);
+              else fb.load(mine + ua, j);
+            }
+          const int jj = f / kFB, ii = f % kFB;
+          acc[h * kMB + jj][ii] =
+              __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfrag(t, ii), afrag(h, jj), acc[h * kMB + jj][ii], 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
-        wait(z ^ 1);
+        if (loads) {
+          if (q == 0) fa.next();
+          else fb.next();
+        }
+        wait(h ^ 1, h == 1 ? t ^ 1 : -1);
         __builtin_amdgcn_sched_barrier(0);
-      }
-      advance();
-      so = no;
+      };
+      quarter(Quarter<0>{});
+      quarter(Quarter<1>{});
+      quarter(Quarter<2>{});
+      __builtin_amdgcn_s_waitcnt(waitcnt_vm(fa.kLoads));
+      __builtin_amdgcn_s_barrier();
+      __builtin_amdgcn_sched_barrier(0);
+      quarter(Quarter<3>{});
+      free_b = ub;
+      ua = na;
     }
     if (g.partial) {
       f32x4* dst = reinterpret_cast<f32x4*>(g.partial) +
                    (static_cast<int64_t>(p) * 8 + wave) * (kMB * kNB * 4 * 64) + lane;
 #pragma unroll
-      for (int jj = 0; jj < kMB; ++jj)
+      for (int jj = 0; jj < 2 * kMB; ++jj)
 #pragma unroll
-        for (int ii = 0; ii < kNB; ++ii)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            dst[((jj * kNB + ii) * 4 + q) * 64] = f32x4{acc[jj][ii][4 * q], acc[jj][ii][4 * q + 1],
-                                                        acc[jj][ii][4 * q + 2], acc[jj][ii][4 * q + 3]};
-    } else {
-      finish<kMode, C::kHalves>(acc, batch, m0 + wm * kMB * 32, n0 + wn * (kPairs ? 32 : 32 * kNB), lane,
-                                lds0 + 2 * kStage + wave * C::kStrip);
+        for (int ii = 0; ii < kFB; ++ii) dst[(jj * kFB + ii) * 64] = acc[jj][ii];
+    } else {  // through the unit that B has left
+      finish<kMode, C::kHalves, kMB, kNB>(acc, batch, m0 + wm * kMB * 32, n0 + wn * (kPairs ? 32 : 32 * kNB), lane,
+                                          lds0 + free_b + wave * C::kStrip);
+      __builtin_amdgcn_s_barrier();  // every wave is done with its strip: A's loads follow there
     }
     p += g.wpx;
     if (p >= pend) break;
+    // the next tile's first operands again: their registers were the end's
+#pragma unroll
+    for (int i = 0; i < kRdA; ++i) rd_a(0, 0, ua, i);
+#pragma unroll
+    for (int i = 0; i < kRdB; ++i) rd_b(0, after(ua, 1), i);
+    wait(0, 0);
+    __builtin_amdgcn_sched_barrier(0);
   }
-  __builtin_amdgcn_s_waitcnt(0);  // the reload of the last slice
+  __builtin_amdgcn_s_waitcnt(0);  // the reloads of the last slices
 #undef TM_RD
 #undef TM_TR
 }
@@ -737,23 +996,17 @@ __global__ __launch_bounds__(256) void lin_finish_kernel(const Args g) {
       sum[i].w += v[i].w;
     }
   }
-  f32x16 v[1][kNB];
+  f32x4 v[2][2 * kNB];
 #pragma unroll
-  for (int ii = 0; ii < kNB; ++ii)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      v[0][ii][4 * q] = sum[ii * 4 + q].x;
-      v[0][ii][4 * q + 1] = sum[ii * 4 + q].y;
-      v[0][ii][4 * q + 2] = sum[ii * 4 + q].z;
-      v[0][ii][4 * q + 3] = sum[ii * 4 + q].w;
-    }
+  for (int i = 0; i < kVec; ++i) v[i / (2 * kNB)][i % (2 * kNB)] = sum[i];
   const int wm = wave >> 2, wn = wave & 3;
-  finish<kMode, C::kHalves>(v, batch, m0 + (wm * kMB + jj) * 32, n0 + wn * (kMode == kGate ? 32 : 32 * kNB), lane,
+  finish<kMode, C::kHalves, 1, kNB>(v, batch, m0 + (wm * kMB + jj) * 32, n0 + wn * (kMode == kGate ? 32 : 32 * kNB), lane,
                             static_cast<uint32_t>(reinterpret_cast<uintptr_t>(strips)) + w4 * C::kStrip);
 }
 
 // ------------------------------------------------------------------------------ the host's side
 
+constexpr int64_t kPad = 64;  // [d0 | d1]: each half is padded to a multiple of this
 constexpr int64_t kMaxPartialBytes = int64_t(2) << 30;
 // Measured on MI355X: microseconds of a 64-deep K slice of a 256 x 256 tile; of a 128 x 128 tile alone on
 // its CU and of two of them on one; what a tile's end costs beyond its products.
@@ -814,13 +1067,13 @@ Product product_of(int op, int64_t rows, int64_t inp, int64_t out, bool two) {
   switch (op) {
     case TM_LIN_FORWARD: return {rows, out, ceil_div(inp, kSliceK), 1, false};
     case TM_LIN_GATE: return {rows, out, ceil_div(inp, kSliceK), 1, true};
-    case TM_LIN_GRAD_X: return {rows, inp, ceil_div(out, kSliceK) * (two ? 2 : 1), 1, false};
+    case TM_LIN_GRAD_X: return {rows, inp, two ? 2 * ceil_div(out, kPad) * (kPad / kSliceK) : ceil_div(out, kSliceK), 1, false};
     case TM_LIN_GATE_GRAD: return {rows, inp, ceil_div(out, kSliceK), 1, false};
     default: return {out, inp, ceil_div(rows, kSliceK), two ? 2 : 1, false};
   }
 }
 
-constexpr int kMaxDevices = 64, kKernels = 10;
+constexpr int kMaxDevices = 64, kKernels = 14;
 std::mutex g_mu;
 bool g_lds_set[kKernels][kMaxDevices] = {};
 int g_cus[kMaxDevices] = {};
@@ -907,8 +1160,8 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
   auto up8 = [](int64_t v) { return (v + 7) / 8 * 8; };
   // the stored widths of the operands, and what of K each holds
   const int64_t wide_a = op == TM_LIN_FORWARD || op == TM_LIN_GATE ? up8(d->inp)
-                         : op == TM_LIN_GRAD_X && two              ? 2 * ceil_div(d->out, kSliceK) * kSliceK
-                         : op == TM_LIN_GRAD_W && two_out          ? ceil_div(d->out, kSliceK) * kSliceK + up8(d->out)
+                         : op == TM_LIN_GRAD_X && two              ? 2 * ceil_div(d->out, kPad) * kPad
+                         : op == TM_LIN_GRAD_W && two_out          ? ceil_div(d->out, kPad) * kPad + up8(d->out)
                                                                    : up8(d->out);
   if (d->lda < wide_a || d->ldb < up8(d->inp) || d->lda >= (1 << 23) || d->ldb >= (1 << 23))
     return lin_fail(TM_EINVAL, "tm_lin: operand rows %lld and %lld elements apart, at least %lld and %lld (whole groups "
@@ -943,12 +1196,12 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
       g.a_rows = static_cast<int>(up8(d->out));
       g.b_rows = static_cast<int>(up8(d->inp));
       g.ka = g.kb = static_cast<int>(d->rows);
-      g.a_batch = ceil_div(d->out, kSliceK) * kSliceK * 2;
+      g.a_batch = ceil_div(d->out, kPad) * kPad * 2;
   }
   g.splits = static_cast<int>(p.splits);
   g.per = static_cast<int>(ceil_div(q.slices, p.splits));
   const int64_t tiles_m = ceil_div(q.m, 64 * p.mb), tiles_n = ceil_div(q.n, 128 * p.nb / (q.gate ? 2 : 1));
-  if (tiles_m * tiles_n * q.batch * p.splits > (int64_t(1) << 27))
+  if (tiles_m * tiles_n * q.batch * p.splits > (int64_t(1) << 22))
     return lin_fail(TM_EINVAL, "tm_lin: %lld x %lld x %lld is too large", (long long)d->rows, (long long)d->inp,
                     (long long)d->out);
   g.tiles_m = static_cast<int>(tiles_m);
@@ -988,7 +1241,7 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
                       "or of 32, with exponents (e4m3)", (long long)d->ldz, (long long)cols);
   }
   if (pairs) {  // rows of whole vectors that the next product reads
-    const int64_t pad = op == TM_LIN_GATE ? up8(cols) : ceil_div(cols, kSliceK) * kSliceK;
+    const int64_t pad = op == TM_LIN_GATE ? up8(cols) : ceil_div(cols, kPad) * kPad;
     g.n_store = static_cast<int>(pad);
     if (g.out_f32 || d->ldo % 8 || d->ldo < (op == TM_LIN_GATE ? pad : 2 * pad) || !aligned(d->o0, 16) ||
         (op == TM_LIN_GATE_GRAD && d->o1 && (d->ldo1 % 8 || d->ldo1 < pad || !aligned(d->o1, 16))))
@@ -999,19 +1252,24 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
     return lin_fail(TM_EINVAL, "tm_lin: output rows %lld elements apart for %lld columns", (long long)d->ldo,
                     (long long)cols);
   }
-  g.out_vec = d->ldo % (g.out_f32 ? 4 : 8) == 0 && aligned(d->o0, 16) && aligned(d->o1, 16);
+  const int64_t kNear = 1 << 24;  // rows this near keep a lane's offsets in 32 bits
+  g.out_vec = d->ldo < kNear && d->ldo % (g.out_f32 ? 4 : 8) == 0 && aligned(d->o0, 16) && aligned(d->o1, 16);
   g.bias = static_cast<const char*>(d->bias);
   g.bias_f32 = d->bias_f32 != 0;
   g.bias_vec = aligned(d->bias, g.bias_f32 ? 16 : 8);
   g.res = static_cast<const char*>(d->res);
   g.res_f32 = d->res_f32 != 0;
   g.ldr = d->ldr;
-  g.res_vec = d->ldr % (g.res_f32 ? 4 : 8) == 0 && aligned(d->res, 16);
+  g.res_vec = d->ldr < kNear && d->ldr % (g.res_f32 ? 4 : 8) == 0 && aligned(d->res, 16);
 
   hipStream_t s = static_cast<hipStream_t>(stream);
   const bool big = p.mb == 4;
   switch (op) {
     case TM_LIN_FORWARD:
+      if (!g.bias && !g.act && !g.held) {
+        if (!g.res) return big ? launch<4, 2, true, true, kPlain>(10, g, s) : launch<2, 1, true, true, kPlain>(11, g, s);
+        return big ? launch<4, 2, true, true, kResidual>(12, g, s) : launch<2, 1, true, true, kResidual>(13, g, s);
+      }
       return big ? launch<4, 2, true, true, kLinear>(0, g, s) : launch<2, 1, true, true, kLinear>(1, g, s);
     case TM_LIN_GATE:
       return big ? launch<4, 2, true, true, kGate>(2, g, s) : launch<2, 2, true, true, kGate>(3, g, s);
