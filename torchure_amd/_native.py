@@ -212,6 +212,20 @@ def ce_host():
     return _CE_HOST
 
 
+_LIN_HOST = None
+
+
+def lin_host():
+    """``host()`` with the linear layers' C entry points bound."""
+    global _LIN_HOST
+    if _LIN_HOST is None:
+        handle = lib()
+        h = host()
+        h.lin_bind({n: ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _SIGNATURES}, NativeError)
+        _LIN_HOST = h
+    return _LIN_HOST
+
+
 def check(rc: int, what: str) -> None:
     if rc != TM_OK:
         msg = lib().tm_last_error().decode(errors="replace")

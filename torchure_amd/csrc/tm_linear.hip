@@ -97,8 +97,14 @@ struct Args {
   float* partial;
 };
 
-// A K-major row's chunk c lies at slot c ^ k_swizzle(row).
-__device__ __forceinline__ int k_swizzle(int row) { return 2 * ((row & 3) | ((row >> 3 & 1) << 2)); }
+// Chunk c of K row `row` of a K-major operand lies at slot c ^ k_swizzle(row): what 32 lanes read at a time,
+// 2 chunks of 8 K rows (4 in a row, and 4 that are 8 on), then falls on 16 different bank groups. Rows
+// of 192 columns are 384 bytes, so that odd ones are half the banks on already, and have 3 times 8 chunks.
+template <int kT>
+__device__ __forceinline__ int k_swizzle(int row) {
+  if constexpr (kT == 192) return (row & 2) | (row >> 3 & 1) << 2;
+  else return 2 * ((row & 3) | (row >> 3 & 1) << 2);
+}
 
 // ------------------------------------------------------------------------------ a tile's results
 //
@@ -660,7 +666,7 @@ __device__ __forceinline__ void place(const Args& g, int p, int& split, int& bat
 // One operand's loads: a stream of units (the tile's kT rows or columns of 64 K) over the workgroup's
 // positions. Load j of wave w fills KB 8 j + w: K-contiguous, 8 rows of 128 bytes; K-major, whole K rows of
 // the tile's columns.
-template <int kT, bool kContig, bool kIsA, bool kPairs, int kTM, int kTN>
+template <int kT, bool kContig, bool kIsA, bool kPairs, bool kRagged, int kTM, int kTN>
 struct Feed {
   static constexpr int kLoads = kT / 64;
   int lp, lit, lend;      // position; slice of the next one that is not plain; the position's last, + 1
@@ -675,8 +681,9 @@ struct Feed {
       r = q * 8 + lane / 8;
       c = (lane % 8) ^ ((r >> 1) & 7);
     } else {
-      r = q * (512 / kT) + lane / (kT / 8);
-      c = (lane % (kT / 8)) ^ k_swizzle(r);
+      const int id = q * 64 + lane;
+      r = id / (kT / 8);
+      c = id % (kT / 8) ^ k_swizzle<kT>(r);
     }
   }
   __device__ __forceinline__ int left(const Args& g) const {  // K that the operand holds from slice lit on
@@ -684,7 +691,8 @@ struct Feed {
     else return g.kb - (!kContig && lit >= g.seg ? lit - g.seg : lit) * kSliceK;
   }
   __device__ __forceinline__ void count(const Args& g) {
-    int n = min(lend - 1 - lit, left(g) / kSliceK);
+    int n = lend - 1 - lit;
+    if (kRagged) n = min(n, left(g) / kSliceK);
     if (!kIsA && !kContig && lit < g.seg) n = min(n, g.seg - 1 - lit);
     plain = max(n, 0);
     lit += plain;
@@ -732,7 +740,7 @@ struct Feed {
   // The slice that is not plain: the position's last, or one that reaches past the operand's K (zeros) or
   // up to its other segment.
   __device__ __forceinline__ void load_event(const Args& g, uint8_t* unit, int pend, int lane, int wave) {
-    const int k = left(g);
+    const int k = kRagged ? left(g) : kSliceK;
     if (k >= kSliceK) {
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) load(unit, j);
@@ -746,6 +754,10 @@ struct Feed {
         to_lds((kContig ? c * 8 : r) < k ? at + off[j] : reinterpret_cast<const char*>(&g_zeros), unit, j);
       }
     }
+    past_event(g, pend, lane, wave);
+  }
+  // On from the slice that is not plain.
+  __device__ __forceinline__ void past_event(const Args& g, int pend, int lane, int wave) {
     if (lit + 1 < lend) {
       ++lit;
       at += step;
@@ -771,7 +783,7 @@ struct Quarter {
   static constexpr int q = kQ;
 };
 
-template <int kMB, int kNB, bool kAK, bool kBK, int kMode>
+template <int kMB, int kNB, bool kAK, bool kBK, bool kRagged, int kMode>
 __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const Args g) {
   using C = Tile<kMB, kNB>;
   constexpr int kTM = C::kTM, kTN = C::kTN, kUnit = C::kUnit;
@@ -798,7 +810,7 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
   const uint32_t vc = (lane & 15) * 128 + (((lane >> 4) ^ ((lane >> 1) & 7)) << 4);  // step 1: chunk ^ 4
   const uint32_t base_a = lds0 + (kAK ? vc + wm * kMB * 32 * 128 : kr * (kTM * 2) + (lane & 1) * 8);
   const uint32_t base_b = lds0 + (kBK ? vc + wn * kNB * 32 * 128 : kr * (kTN * 2) + (lane & 1) * 8);
-  const int ksw = k_swizzle(kr), kc = (lane >> 1) & 1;
+  const int ksa = k_swizzle<kTM>(kr), ksb = k_swizzle<kTN>(kr), kc = (lane >> 1) & 1;
 #define TM_RD(dst, base, imm) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(dst) : "v"(base), "i"(imm))
 #define TM_TR(dst, base, imm) asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(dst) : "v"(base), "i"(imm))
   bf16x8 a8[2][kAK ? kMB : 1], b8[2][kBK ? kFB : 1];
@@ -806,13 +818,13 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
   auto rd_a = [&](int t, int h, uint32_t ua, int i) {  // read i of step t, half h, from the unit at ua
     if constexpr (kAK) TM_RD(a8[h][i], (base_a ^ (t * 64)) + ua, (h * kMB + i) * 16 * 128);
     else
-      TM_TR(a4[h][i], base_a + ua + ((2 * (wm * 2 * kMB + h * kMB + (i >> 1)) + kc) ^ ksw) * 16,
+      TM_TR(a4[h][i], base_a + ua + ((2 * (wm * 2 * kMB + h * kMB + (i >> 1)) + kc) ^ ksa) * 16,
             t * 64 * kTM + (i & 1) * 4 * kTM * 2);
   };
   auto rd_b = [&](int t, uint32_t ub, int i) {
     if constexpr (kBK) TM_RD(b8[t][i], (base_b ^ (t * 64)) + ub, i * 16 * 128);
     else
-      TM_TR(b4[t][i], base_b + ub + ((2 * (wn * kFB + (i >> 1)) + kc) ^ ksw) * 16,
+      TM_TR(b4[t][i], base_b + ub + ((2 * (wn * kFB + (i >> 1)) + kc) ^ ksb) * 16,
             t * 64 * kTN + (i & 1) * 4 * kTN * 2);
   };
   // waits for the reads of A's half h and (t >= 0) of B's step t; naming every fragment keeps the MFMAs that
@@ -846,8 +858,8 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
     return u >= static_cast<uint32_t>(C::kLds) ? u - C::kLds : u;
   };
   uint8_t* const mine = smem + wave * 1024;
-  Feed<kTM, kAK, true, kPairs, kTM, kTN> fa;
-  Feed<kTN, kBK, false, kPairs, kTM, kTN> fb;
+  Feed<kTM, kAK, true, kPairs, kRagged, kTM, kTN> fa;
+  Feed<kTN, kBK, false, kPairs, kRagged, kTM, kTN> fb;
   fa.seek(g, p, lane, wave);
   fb.seek(g, p, lane, wave);
   fa.count(g);
@@ -888,13 +900,15 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
         constexpr int q = decltype(which)::q, t = q / 2, h = q % 2;
         constexpr int kMf = kMB * kFB, kReads = h == 0 ? kRdA : kRdA + kRdB;
         constexpr int kPer = (4 * kReads + 3 * kMf - 1) / (3 * kMf);
-        constexpr int kLoads = q == 0 ? fa.kLoads : (q == 3 ? fb.kLoads : 0);
-        bool loads = false;
-        if (q == 0) {
+        // loads of this quarter, [from, to): A's in three (kRagged: the first), B's in the fourth
+        constexpr int from = kRagged || q == 3 ? 0 : fa.kLoads * q / 3;
+        constexpr int to = q == 3 ? fb.kLoads : (kRagged ? (q == 0 ? fa.kLoads : 0) : fa.kLoads * (q + 1) / 3);
+        bool loads = true;
+        if (kRagged && q == 0) {
           loads = fa.plain > 0;
           if (!loads) fa.load_event(g, mine + free_b, pend, lane, wave);
         }
-        if (q == 3) {
+        if (kRagged && q == 3) {
           loads = fb.plain > 0;
           if (!loads) fb.load_event(g, mine + ua, pend, lane, wave);
         }
@@ -906,10 +920,10 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
             else if (i < kRdA) rd_a(t ^ 1, 0, q == 1 ? ua : na, i);
             else rd_b(t ^ 1, q == 1 ? ub : nb, i - kRdA);
           }
-          if (kLoads && loads)
+          if (to > from && loads)
 #pragma unroll
-            for (int j = f * kLoads / kMf; j < (f + 1) * kLoads / kMf; ++j) {
-              if (q == 0) fa.load(mine + free_b, j);
+            for (int j = from + f * (to - from) / kMf; j < from + (f + 1) * (to - from) / kMf; ++j) {
+              if (q != 3) fa.load(mine + free_b, j);
               else fb.load(mine + ua, j);
             }
           const int jj = f / kFB, ii = f % kFB;
@@ -917,9 +931,13 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
               __builtin_amdgcn_mfma_f32_16x16x32_bf16(bfrag(t, ii), afrag(h, jj), acc[h * kMB + jj][ii], 0, 0, 0);
           __builtin_amdgcn_sched_barrier(0);
         }
-        if (loads) {
-          if (q == 0) fa.next();
-          else fb.next();
+        if (kRagged ? q == 0 && loads : q == 2) {
+          if (kRagged || fa.plain > 0) fa.next();
+          else fa.past_event(g, pend, lane, wave);
+        }
+        if (q == 3 && loads) {
+          if (kRagged || fb.plain > 0) fb.next();
+          else fb.past_event(g, pend, lane, wave);
         }
         wait(h ^ 1, h == 1 ? t ^ 1 : -1);
         __builtin_amdgcn_sched_barrier(0);
@@ -1004,14 +1022,110 @@ __global__ __launch_bounds__(256) void lin_finish_kernel(const Args g) {
                             static_cast<uint32_t>(reinterpret_cast<uintptr_t>(strips)) + w4 * C::kStrip);
 }
 
+// ------------------------------------------------------------------------------ few rows
+//
+// The forward products of up to 16 kMT rows (a token, a short sequence's end): bound by the weight's bytes, or,
+// where those are few, by the latency of one launch. A workgroup takes 32 output columns (with a gate 32 of
+// each weight); its waves take 64 K each in turn and keep the whole result, which they add up in LDS
+// in order. An operand's 64 K of a row are 128 bytes of four lanes, 32 each: the two MFMAs of a step take
+// the lanes' first and second 16 bytes, the same K of both operands. Nothing is loaded twice, so nothing
+// goes through LDS on the way in. The end is the tiles'.
+template <int kMT, int kMode>
+struct Few {
+  static constexpr int kWaves = kMT == 4 || kMode == kLinear ? 8 : 16;  // kLinear's end takes over 128 registers
+  static constexpr int lds(int nt) { return kWaves * kMT * nt * 1024 + 8192; }
+};
+
+template <int kMT, int kMode>
+__global__ __launch_bounds__((Few<kMT, kMode>::kWaves * 64)) void lin_rows_kernel(const Args g) {
+  constexpr bool kPairs = kMode == kGate;
+  constexpr int kNT = kPairs ? 4 : 2, kWaves = Few<kMT, kMode>::kWaves, kSums = (kMT + 1) / 2;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n0 = static_cast<int>(blockIdx.x) * 32, r = lane & 15, c = lane >> 4;
+  const char *pw[kNT], *px[kMT];
+#pragma unroll
+  for (int t = 0; t < kNT; ++t)
+    pw[t] = (t >= 2 ? g.b1 : g.b0) + min(n0 + 16 * (t & 1) + r, g.n - 1) * g.b_ld + c * 32;
+#pragma unroll
+  for (int t = 0; t < kMT; ++t) px[t] = g.a + min(16 * t + r, g.m - 1) * g.a_ld + c * 32;
+  f32x4 acc[kMT][kNT];
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  // several steps' loads at a time in flight
+  constexpr int kBatch = kMT == 4 ? 1 : (kMT == 2 ? 2 : 4) / (kPairs ? 2 : 1), kStep = kWaves * kSliceK;
+  for (int k0 = wave * kSliceK; k0 < g.ka; k0 += kBatch * kStep) {
+    bf16x8 w[kBatch][kNT][2], x[kBatch][kMT][2];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int k = k0 + b * kStep;
+      if (k >= g.ka) break;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool in = k + c * 16 + u * 8 < g.ka;
+#pragma unroll
+        for (int t = 0; t < kNT; ++t) {
+          w[b][t][u] = bf16x8{};
+          if (in) w[b][t][u] = *reinterpret_cast<const bf16x8*>(pw[t] + static_cast<int64_t>(k) * 2 + u * 16);
+        }
+#pragma unroll
+        for (int t = 0; t < kMT; ++t) {
+          x[b][t][u] = bf16x8{};
+          if (in) x[b][t][u] = *reinterpret_cast<const bf16x8*>(px[t] + static_cast<int64_t>(k) * 2 + u * 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (k0 + b * kStep >= g.ka) break;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < kMT; ++i)
+#pragma unroll
+          for (int j = 0; j < kNT; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[b][j][u], x[b][i][u], acc[i][j], 0, 0, 0);
+    }
+  }
+  f32x4* part = reinterpret_cast<f32x4*>(smem);
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) part[((wave * kMT + i) * kNT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  if (wave >= kSums) return;
+  f32x4 sum[2][kNT];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) {
+      sum[h][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (2 * wave + h >= kMT) continue;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) sum[h][j] += part[((w * kMT + 2 * wave + h) * kNT + j) * 64 + lane];
+    }
+  finish<kMode, false, 1, kNT / 2>(sum, 0, wave * 32, n0, lane,
+                                   static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) +
+                                       kWaves * kMT * kNT * 1024 + wave * 4096);
+}
+
 // ------------------------------------------------------------------------------ the host's side
 
 constexpr int64_t kPad = 64;  // [d0 | d1]: each half is padded to a multiple of this
 constexpr int64_t kMaxPartialBytes = int64_t(2) << 30;
-// Measured on MI355X: microseconds of a 64-deep K slice of a 256 x 256 tile; of a 128 x 128 tile alone on
-// its CU and of two of them on one; what a tile's end costs beyond its products.
-constexpr double kUsSlice256 = 1.42, kUsSlice128 = 0.62, kUsSlice128Pair = 0.95;
-constexpr double kUsLaunch = 3.0, kUsEnd = 2.0, kUsReduce = 3.0, kBytesPerUs = 4.5e6;
+// Measured on MI355X (sweeps of tiles and splits over the block's products at 8192 rows): microseconds of a
+// slice and of a tile's end, by tile. The ends of a round of tiles come together and are bound by memory;
+// the gate's, by what they read and write more. Up to 128 workgroups run at a higher clock.
+struct Cost {
+  int mb, nb;
+  double slice, end;
+};
+constexpr Cost kCosts[] = {{4, 2, 1.37, 6.0}, {3, 2, 1.24, 5.0}, {2, 2, 0.95, 4.0}, {2, 1, 0.95, 5.0}};
+constexpr double kUsSliceAlone = 0.62, kUsEndAlone = 3.0;  // 128 x 128 tiles, one workgroup on a CU instead of two
+constexpr double kUsLaunch = 3.0, kUsReduce = 5.0, kBytesPerUs = 4.5e6, kFewer = 0.9;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -1019,7 +1133,8 @@ bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(
 // What a call computes, in the kernel's terms.
 struct Product {
   int64_t m, n, slices, batch;
-  bool gate;  // n counts features, a tile has half as many as columns
+  bool gate;    // n counts features, a tile has half as many as columns
+  double ends;  // what a tile's end moves, to a plain one's
 };
 
 struct Plan {
@@ -1028,29 +1143,28 @@ struct Plan {
   double us;
 };
 
-Plan plan_of(const Product& q, int mb, int nb, int64_t splits) {
-  const int64_t tm = 64 * mb, tn = 128 * nb / (q.gate ? 2 : 1);
+Plan plan_of(const Product& q, const Cost& c, int64_t splits) {
+  const int64_t tm = 64 * c.mb, tn = 128 * c.nb / (q.gate ? 2 : 1);
   const int64_t tiles = ceil_div(q.m, tm) * ceil_div(q.n, tn) * q.batch, wgs = tiles * splits;
   const int64_t per = ceil_div(q.slices, splits);
   double us = kUsLaunch;
-  if (mb == 4) us += ceil_div(wgs, 256) * (per * kUsSlice256 + kUsEnd);
-  else if (nb == 2) us += ceil_div(wgs, 256) * (per * 0.5 * (kUsSlice256 + kUsSlice128) + kUsEnd);
-  else if (wgs <= 256) us += per * kUsSlice128 + kUsEnd;
-  else us += ceil_div(wgs, 512) * (per * kUsSlice128Pair + kUsEnd);
-  if (splits > 1) us += kUsReduce + static_cast<double>(wgs) * (tm * 128 * nb) * 8.0 / kBytesPerUs;
-  return {mb, nb, splits, us};
+  if (c.nb == 2) us += ceil_div(wgs, 256) * (per * c.slice * (wgs <= 128 ? kFewer : 1.0) + c.end * q.ends);
+  else if (wgs <= 256) us += per * kUsSliceAlone + kUsEndAlone * q.ends;
+  else us += ceil_div(wgs, 512) * (per * c.slice + c.end * q.ends);
+  if (splits > 1) us += kUsReduce + static_cast<double>(wgs) * (tm * 128 * c.nb) * 8.0 / kBytesPerUs;
+  return {c.mb, c.nb, splits, us};
 }
 
 // The tile and the number of splits with the least estimated time.
 Plan best_plan(const Product& q) {
   Plan best = {0, 0, 0, 0.0};
-  const int shapes[2][2] = {{4, 2}, {2, q.gate ? 2 : 1}};
-  for (const auto& sh : shapes) {
-    const int64_t tiles = ceil_div(q.m, 64 * sh[0]) * ceil_div(q.n, 128 * sh[1] / (q.gate ? 2 : 1)) * q.batch;
+  for (const Cost& c : kCosts) {
+    if (c.mb == 2 && (c.nb == 2) != q.gate) continue;
+    const int64_t tiles = ceil_div(q.m, 64 * c.mb) * ceil_div(q.n, 128 * c.nb / (q.gate ? 2 : 1)) * q.batch;
     for (int64_t s = 1; s <= 64 && s <= q.slices; ++s) {
       if (ceil_div(q.slices, ceil_div(q.slices, s)) != s) continue;  // some split would be empty
-      if (s > 1 && tiles * s * (64 * sh[0]) * (128 * sh[1]) * 4 > kMaxPartialBytes) break;
-      const Plan p = plan_of(q, sh[0], sh[1], s);
+      if (s > 1 && tiles * s * (64 * c.mb) * (128 * c.nb) * 4 > kMaxPartialBytes) break;
+      const Plan p = plan_of(q, c, s);
       if (best.splits == 0 || p.us < best.us) best = p;
     }
   }
@@ -1065,15 +1179,24 @@ size_t partial_bytes(const Product& q, const Plan& p) {
 
 Product product_of(int op, int64_t rows, int64_t inp, int64_t out, bool two) {
   switch (op) {
-    case TM_LIN_FORWARD: return {rows, out, ceil_div(inp, kSliceK), 1, false};
-    case TM_LIN_GATE: return {rows, out, ceil_div(inp, kSliceK), 1, true};
-    case TM_LIN_GRAD_X: return {rows, inp, two ? 2 * ceil_div(out, kPad) * (kPad / kSliceK) : ceil_div(out, kSliceK), 1, false};
-    case TM_LIN_GATE_GRAD: return {rows, inp, ceil_div(out, kSliceK), 1, false};
-    default: return {out, inp, ceil_div(rows, kSliceK), two ? 2 : 1, false};
+    case TM_LIN_FORWARD: return {rows, out, ceil_div(inp, kSliceK), 1, false, 1.0};
+    case TM_LIN_GATE: return {rows, out, ceil_div(inp, kSliceK), 1, true, 1.5};
+    case TM_LIN_GRAD_X: return {rows, inp,
+                               two ? 2 * ceil_div(out, kPad) * (kPad / kSliceK) : ceil_div(out, kSliceK), 1,
+                               false, 1.0};
+    case TM_LIN_GATE_GRAD: return {rows, inp, ceil_div(out, kSliceK), 1, false, 5.0};
+    default: return {out, inp, ceil_div(rows, kSliceK), two ? 2 : 1, false, 1.0};
   }
 }
 
-constexpr int kMaxDevices = 64, kKernels = 14;
+// What lin_rows_kernel takes: up to 16 rows, and up to 64 of short K. (Microseconds against 128 x 128 tiles:
+// 1 x 1024 -> 2816 5.1 / 12.6, 1 x 2816 -> 1024 8.7 / 14.7, 64 x 1024 -> 2816 9.0 / 12.7, but 64 x 2816 -> 1024
+// 18.3 / 14.7 and 64 x 9728 -> 2560 53 / 22.)
+bool few_rows(int op, int64_t rows, int64_t inp) {
+  return op <= TM_LIN_GATE && (rows <= 16 || (rows <= 64 && inp <= 1536));
+}
+
+constexpr int kMaxDevices = 64, kKernels = 54;
 std::mutex g_mu;
 bool g_lds_set[kKernels][kMaxDevices] = {};
 int g_cus[kMaxDevices] = {};
@@ -1104,17 +1227,17 @@ hipError_t allow_lds(hipStream_t stream, int which, const void* fn, int bytes, i
   return hipSuccess;
 }
 
-template <int kMB, int kNB, bool kAK, bool kBK, int kMode>
-int launch(int which, Args& g, hipStream_t s) {
+template <int kMB, int kNB, bool kAK, bool kBK, bool kRagged, int kMode>
+int launch_one(int which, Args& g, hipStream_t s) {
   using C = Tile<kMB, kNB>;
   int cus = 0;
-  const void* fn = reinterpret_cast<const void*>(lin_kernel<kMB, kNB, kAK, kBK, kMode>);
+  const void* fn = reinterpret_cast<const void*>(lin_kernel<kMB, kNB, kAK, kBK, kRagged, kMode>);
   hipError_t e = allow_lds(s, which, fn, C::kLds, &cus);
   if (e != hipSuccess) return lin_fail(TM_ELAUNCH, "tm_lin: LDS attribute: %s", hipGetErrorString(e));
   const int64_t positions = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.batch * g.splits;
   const int64_t per_xcd = ceil_div(positions, 8), room = (cus >= 16 ? cus / 8 : 1) * (2 * C::kLds <= 163840 ? 2 : 1);
   g.wpx = static_cast<int>(per_xcd < room ? per_xcd : room);
-  hipLaunchKernelGGL((lin_kernel<kMB, kNB, kAK, kBK, kMode>), dim3(static_cast<uint32_t>(8 * g.wpx)), dim3(512), C::kLds,
+  hipLaunchKernelGGL((lin_kernel<kMB, kNB, kAK, kBK, kRagged, kMode>), dim3(static_cast<uint32_t>(8 * g.wpx)), dim3(512), C::kLds,
                      s, g);
   e = hipGetLastError();
   if (e != hipSuccess) return lin_fail(TM_ELAUNCH, "lin_kernel: launch failed: %s", hipGetErrorString(e));
@@ -1128,12 +1251,49 @@ int launch(int which, Args& g, hipStream_t s) {
   return TM_OK;
 }
 
+// kRagged: some slice reaches past an operand's K.
+template <int kMB, int kNB, bool kAK, bool kBK, int kMode>
+int launch(int which, Args& g, hipStream_t s) {
+  const int seg = g.slices / g.seg;
+  if (g.ka == g.slices * kSliceK && g.kb == g.seg * kSliceK && seg * g.seg == g.slices)
+    return launch_one<kMB, kNB, kAK, kBK, false, kMode>(2 * which, g, s);
+  return launch_one<kMB, kNB, kAK, kBK, true, kMode>(2 * which + 1, g, s);
+}
+
+template <int kMT, int kMode>
+int launch_rows(int which, Args& g, hipStream_t s) {
+  constexpr int kLds = Few<kMT, kMode>::lds(kMode == kGate ? 4 : 2);
+  int cus = 0;
+  hipError_t e = allow_lds(s, which, reinterpret_cast<const void*>(lin_rows_kernel<kMT, kMode>), kLds, &cus);
+  if (e != hipSuccess) return lin_fail(TM_ELAUNCH, "tm_lin: LDS attribute: %s", hipGetErrorString(e));
+  const int cols = kMode == kGate ? g.n_store : g.n;
+  hipLaunchKernelGGL((lin_rows_kernel<kMT, kMode>), dim3(static_cast<uint32_t>(ceil_div(cols, 32))),
+                     dim3(Few<kMT, kMode>::kWaves * 64), kLds, s, g);
+  e = hipGetLastError();
+  return e == hipSuccess ? TM_OK : lin_fail(TM_ELAUNCH, "lin_rows_kernel: launch failed: %s", hipGetErrorString(e));
+}
+
+template <int kMode>
+int launch_few(int which, Args& g, hipStream_t s) {
+  if (g.m <= 16) return launch_rows<1, kMode>(which, g, s);
+  if (g.m <= 32) return launch_rows<2, kMode>(which + 1, g, s);
+  return launch_rows<4, kMode>(which + 2, g, s);
+}
+
+template <bool kAK, bool kBK, int kMode>
+int launch_tile(const Plan& p, int which, Args& g, hipStream_t s) {
+  if (p.mb == 4) return launch<4, 2, kAK, kBK, kMode>(3 * which, g, s);
+  if (p.mb == 3) return launch<3, 2, kAK, kBK, kMode>(3 * which + 1, g, s);
+  return launch<2, kMode == kGate ? 2 : 1, kAK, kBK, kMode>(3 * which + 2, g, s);
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t tm_lin_workspace_bytes(int op, int64_t rows, int64_t inp, int64_t out, int two) {
   if (op < TM_LIN_FORWARD || op > TM_LIN_GRAD_W || rows <= 0 || inp <= 0 || out <= 0) return 0;
+  if (few_rows(op, rows, inp)) return 0;
   const Product q = product_of(op, rows, inp, out, two != 0);
   return partial_bytes(q, best_plan(q));
 }
@@ -1154,7 +1314,7 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
                     "(%lld, %lld)", (long long)d->lda, (long long)d->ldb);
   const Product q = product_of(op, d->rows, d->inp, d->out, two || two_out);
   const Plan p = best_plan(q);
-  const size_t need = partial_bytes(q, p);
+  const size_t need = few_rows(op, d->rows, d->inp) ? 0 : partial_bytes(q, p);
   if (need && (!d_ws || ws_bytes < need || !aligned(d_ws, 16)))
     return lin_fail(TM_EINVAL, "tm_lin: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, need);
   auto up8 = [](int64_t v) { return (v + 7) / 8 * 8; };
@@ -1263,22 +1423,19 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
   g.res_vec = d->ldr < kNear && d->ldr % (g.res_f32 ? 4 : 8) == 0 && aligned(d->res, 16);
 
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool big = p.mb == 4;
+  if (few_rows(op, d->rows, d->inp)) {
+    if (op == TM_LIN_GATE) return launch_few<kGate>(kKernels - 12, g, s);
+    if (g.bias || g.act || g.held) return launch_few<kLinear>(kKernels - 9, g, s);
+    return g.res ? launch_few<kResidual>(kKernels - 6, g, s) : launch_few<kPlain>(kKernels - 3, g, s);
+  }
   switch (op) {
     case TM_LIN_FORWARD:
-      if (!g.bias && !g.act && !g.held) {
-        if (!g.res) return big ? launch<4, 2, true, true, kPlain>(10, g, s) : launch<2, 1, true, true, kPlain>(11, g, s);
-        return big ? launch<4, 2, true, true, kResidual>(12, g, s) : launch<2, 1, true, true, kResidual>(13, g, s);
-      }
-      return big ? launch<4, 2, true, true, kLinear>(0, g, s) : launch<2, 1, true, true, kLinear>(1, g, s);
-    case TM_LIN_GATE:
-      return big ? launch<4, 2, true, true, kGate>(2, g, s) : launch<2, 2, true, true, kGate>(3, g, s);
-    case TM_LIN_GRAD_X:
-      return big ? launch<4, 2, true, false, kPlain>(4, g, s) : launch<2, 1, true, false, kPlain>(5, g, s);
-    case TM_LIN_GATE_GRAD:
-      return big ? launch<4, 2, true, false, kGateGrad>(6, g, s) : launch<2, 1, true, false, kGateGrad>(7, g, s);
-    default:
-      return big ? launch<4, 2, false, false, kPlain>(8, g, s) : launch<2, 1, false, false, kPlain>(9, g, s);
+      if (g.bias || g.act || g.held) return launch_tile<true, true, kLinear>(p, 0, g, s);
+      return g.res ? launch_tile<true, true, kResidual>(p, 1, g, s) : launch_tile<true, true, kPlain>(p, 2, g, s);
+    case TM_LIN_GATE: return launch_tile<true, true, kGate>(p, 3, g, s);
+    case TM_LIN_GRAD_X: return launch_tile<true, false, kPlain>(p, 4, g, s);
+    case TM_LIN_GATE_GRAD: return launch_tile<true, false, kGateGrad>(p, 5, g, s);
+    default: return launch_tile<false, false, kPlain>(p, 6, g, s);
   }
 }
 
