@@ -530,7 +530,7 @@ int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_v
  * past cols, 16-byte aligned; or NULL) = dy act'(z), dy bf16 or (dy_f32) fp32 rows ldy apart, z as held
  * by tm_lin (rows ldz apart, exponents with TM_HELD_E4M3; not read when act is TM_ACT_NONE, which makes
  * this a cast into padded rows). d_bias (bf16 or, bias_f32, fp32; or NULL) = the sums of the unrounded
- * dz over the rows, by fp32 partial sums over 128 rows each in d_ws, tm_act_grad_workspace_bytes bytes,
+ * dz over the rows, by fp32 partial sums over 64 rows each in d_ws, tm_act_grad_workspace_bytes bytes,
  * added in order.
  */
 size_t tm_act_grad_workspace_bytes(int64_t rows, int64_t cols);

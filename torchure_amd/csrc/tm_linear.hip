@@ -28,8 +28,9 @@
 //
 // Edges: rows and columns past an operand's last are loaded again (their results are not stored); K
 // past the operand's end is loaded from 16 bytes of zeros, on both sides, so that no garbage meets
-// a zero. Products with few tiles are split over K: fp32 partial tiles in the workspace, added in
-// split order by lin_finish_kernel, which then does what the unsplit kernel's end does.
+// a zero. Where whole rounds of tiles over the CUs leave some over, or there are few tiles at all, those are
+// split over K: fp32 partial tiles in the workspace, added in order by lin_finish_kernel, which then does what
+// the unsplit tiles' end does.
 
 #include <hip/hip_runtime.h>
 
@@ -76,7 +77,7 @@ struct Args {
   int a_rows, b_rows;       // K-contiguous: rows stored; K-major: columns stored, whole groups of 8
   int ka, kb;               // K that A holds, and that B holds (of one segment)
   int slices, seg;          // K slices, and of them those before b1's (grad_x of two weights)
-  int per, splits;          // K slices a position covers
+  int whole, splits, per;   // an XCD's tiles before its split ones; parts of those, of `per` slices each
   int tiles_m, tiles_n, batch, gm, gn, wpx;
   // what follows the product
   char* o0;
@@ -646,21 +647,52 @@ __device__ __forceinline__ int divide(int a, int d, int& rem) {
   return q;
 }
 
-// Position -> split, batch and the tile's first row and column (gate: feature): n-blocks of gn tile
-// columns; inside each, m-blocks of gm tile rows, a block's gm x gn tiles consecutive.
+// An XCD's share of the tiles: `whole` of them in one position each, then the others in g.splits positions each,
+// all first parts before all second ones.
+struct Share {
+  int first, whole, others;
+  __device__ __forceinline__ int positions(const Args& g) const { return whole + others * g.splits; }
+};
+
+__device__ __forceinline__ Share share_of(const Args& g, int xcd) {
+  const int T = g.tiles_m * g.tiles_n * g.batch, t8 = (T + 7) / 8, first = xcd * t8;
+  const int n = max(0, min(t8, T - first)), whole = min(g.whole, n);
+  return {first, whole, n - whole};
+}
+
+// Tile -> batch and the tile's first row and column (gate: feature): n-blocks of gn tile columns; inside each,
+// m-blocks of gm tile rows, a block's gm x gn tiles consecutive.
 template <int kTM, int kTN, bool kHalf>
-__device__ __forceinline__ void place(const Args& g, int p, int& split, int& batch, int& m0, int& n0) {
-  split = batch = 0;
-  const int tb = g.tiles_m * g.tiles_n;
-  if (g.splits > 1) split = divide(p, tb * g.batch, p);
-  if (g.batch > 1) batch = divide(p, tb, p);
+__device__ __forceinline__ void place(const Args& g, int tile, int& batch, int& m0, int& n0) {
+  batch = 0;
+  if (g.batch > 1) batch = divide(tile, g.tiles_m * g.tiles_n, tile);
   int rem, tn;
-  const int nb = divide(p, g.tiles_m * g.gn, rem);
+  const int nb = divide(tile, g.tiles_m * g.gn, rem);
   const int gn = min(g.gn, g.tiles_n - nb * g.gn);
   const int mb = divide(rem, g.gm * gn, rem);
   const int tm = mb * g.gm + divide(rem, gn, tn);
   m0 = tm * kTM;
   n0 = (nb * g.gn + tn) * (kHalf ? kTN / 2 : kTN);
+}
+
+// An XCD's position -> tile, and its slices [lit, lend); the part of a split tile, else -1.
+__device__ __forceinline__ int part_of(const Args& g, const Share& s, int p, int& tile, int& lit, int& lend) {
+  lit = 0;
+  lend = g.slices;
+  tile = s.first + p;
+  if (p < s.whole) return -1;
+  int rem;
+  const int part = divide(p - s.whole, s.others, rem);
+  tile = s.first + s.whole + rem;
+  lit = part * g.per;
+  lend = min(lit + g.per, g.slices);
+  return part;
+}
+
+// Where part `part` of an XCD's split tile `tile` lies in the workspace, in tiles.
+__device__ __forceinline__ int64_t partial_at(const Args& g, int tile, int part) {
+  const int T = g.tiles_m * g.tiles_n * g.batch, t8 = (T + 7) / 8, xcd = tile / t8;
+  return static_cast<int64_t>(xcd * (t8 - g.whole) + tile - xcd * t8 - g.whole) * g.splits + part;
 }
 
 // One operand's loads: a stream of units (the tile's kT rows or columns of 64 K) over the workgroup's
@@ -697,13 +729,12 @@ struct Feed {
     plain = max(n, 0);
     lit += plain;
   }
-  __device__ __forceinline__ void seek(const Args& g, int pos, int lane, int wave) {
+  __device__ __forceinline__ void seek(const Args& g, const Share& sh, int pos, int lane, int wave) {
     asm volatile("" : "+v"(lane));  // derived again for each tile, not kept through the products
-    int split, batch, m0, n0;
-    place<kTM, kTN, kPairs>(g, pos, split, batch, m0, n0);
+    int tile, batch, m0, n0;
     lp = pos;
-    lit = split * g.per;
-    lend = min(lit + g.per, g.slices);
+    part_of(g, sh, pos, tile, lit, lend);
+    place<kTM, kTN, kPairs>(g, tile, batch, m0, n0);
     const int64_t ld = kIsA ? g.a_ld : g.b_ld;
     step = kContig ? kSliceK * 2 : kSliceK * ld;
     if constexpr (kIsA) {
@@ -739,7 +770,7 @@ struct Feed {
   }
   // The slice that is not plain: the position's last, or one that reaches past the operand's K (zeros) or
   // up to its other segment.
-  __device__ __forceinline__ void load_event(const Args& g, uint8_t* unit, int pend, int lane, int wave) {
+  __device__ __forceinline__ void load_event(const Args& g, const Share& sh, uint8_t* unit, int lane, int wave) {
     const int k = kRagged ? left(g) : kSliceK;
     if (k >= kSliceK) {
 #pragma unroll
@@ -754,26 +785,26 @@ struct Feed {
         to_lds((kContig ? c * 8 : r) < k ? at + off[j] : reinterpret_cast<const char*>(&g_zeros), unit, j);
       }
     }
-    past_event(g, pend, lane, wave);
+    past_event(g, sh, lane, wave);
   }
   // On from the slice that is not plain.
-  __device__ __forceinline__ void past_event(const Args& g, int pend, int lane, int wave) {
+  __device__ __forceinline__ void past_event(const Args& g, const Share& sh, int lane, int wave) {
     if (lit + 1 < lend) {
       ++lit;
       at += step;
       if (!kIsA && !kContig && lit == g.seg) at = g.b1 + col;
-    } else if (lp + g.wpx < pend) {
-      seek(g, lp + g.wpx, lane, wave);
+    } else if (lp + g.wpx < sh.positions(g)) {
+      seek(g, sh, lp + g.wpx, lane, wave);
     }  // else: the last slice again, which nothing reads
     count(g);
   }
-  __device__ __forceinline__ void load_all(const Args& g, uint8_t* unit, int pend, int lane, int wave) {
+  __device__ __forceinline__ void load_all(const Args& g, const Share& sh, uint8_t* unit, int lane, int wave) {
     if (plain > 0) {
 #pragma unroll
       for (int j = 0; j < kLoads; ++j) load(unit, j);
       next();
     } else {
-      load_event(g, unit, pend, lane, wave);
+      load_event(g, sh, unit, lane, wave);
     }
   }
 };
@@ -792,10 +823,9 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
   constexpr bool kPairs = kMode == kGate;
   static_assert(!kPairs || (kNB == 2 && kBK), "gate and up columns alternate by 32 within a wave");
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-  const int P = g.tiles_m * g.tiles_n * g.batch * g.splits;
-  const int p8 = (P + 7) / 8;
-  const int pend = min((static_cast<int>(blockIdx.x % 8) + 1) * p8, P);
-  int p = static_cast<int>(blockIdx.x % 8) * p8 + static_cast<int>(blockIdx.x / 8);
+  const Share sh = share_of(g, static_cast<int>(blockIdx.x % 8));
+  const int pend = sh.positions(g);
+  int p = static_cast<int>(blockIdx.x / 8);
   if (p >= pend) return;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -860,14 +890,14 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
   uint8_t* const mine = smem + wave * 1024;
   Feed<kTM, kAK, true, kPairs, kRagged, kTM, kTN> fa;
   Feed<kTN, kBK, false, kPairs, kRagged, kTM, kTN> fb;
-  fa.seek(g, p, lane, wave);
-  fb.seek(g, p, lane, wave);
+  fa.seek(g, sh, p, lane, wave);
+  fb.seek(g, sh, p, lane, wave);
   fa.count(g);
   fb.count(g);
 #pragma unroll 1
   for (int i = 0; i < 2; ++i) {
-    fa.load_all(g, mine + 2 * i * kUnit, pend, lane, wave);
-    fb.load_all(g, mine + (2 * i + 1) * kUnit, pend, lane, wave);
+    fa.load_all(g, sh, mine + 2 * i * kUnit, lane, wave);
+    fb.load_all(g, sh, mine + (2 * i + 1) * kUnit, lane, wave);
   }
   __builtin_amdgcn_s_waitcnt(waitcnt_vm(fa.kLoads + fb.kLoads));
   __builtin_amdgcn_s_barrier();
@@ -881,9 +911,10 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
   __builtin_amdgcn_sched_barrier(0);
 
   for (;;) {
-    int split, batch, m0, n0;
-    place<kTM, kTN, kPairs>(g, p, split, batch, m0, n0);
-    const int n_it = min(g.per, g.slices - split * g.per);
+    int tile, batch, m0, n0, n_it, it0;
+    const int part = part_of(g, sh, p, tile, it0, n_it);
+    place<kTM, kTN, kPairs>(g, tile, batch, m0, n0);
+    n_it -= it0;
     f32x4 acc[2 * kMB][kFB];
 #pragma unroll
     for (int i = 0; i < 2 * kMB; ++i)
@@ -906,11 +937,11 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
         bool loads = true;
         if (kRagged && q == 0) {
           loads = fa.plain > 0;
-          if (!loads) fa.load_event(g, mine + free_b, pend, lane, wave);
+          if (!loads) fa.load_event(g, sh, mine + free_b, lane, wave);
         }
         if (kRagged && q == 3) {
           loads = fb.plain > 0;
-          if (!loads) fb.load_event(g, mine + ua, pend, lane, wave);
+          if (!loads) fb.load_event(g, sh, mine + ua, lane, wave);
         }
 #pragma unroll
         for (int f = 0; f < kMf; ++f) {  // one MFMA, its share of the reads and of the loads
@@ -933,11 +964,11 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
         }
         if (kRagged ? q == 0 && loads : q == 2) {
           if (kRagged || fa.plain > 0) fa.next();
-          else fa.past_event(g, pend, lane, wave);
+          else fa.past_event(g, sh, lane, wave);
         }
         if (q == 3 && loads) {
           if (kRagged || fb.plain > 0) fb.next();
-          else fb.past_event(g, pend, lane, wave);
+          else fb.past_event(g, sh, lane, wave);
         }
         wait(h ^ 1, h == 1 ? t ^ 1 : -1);
         __builtin_amdgcn_sched_barrier(0);
@@ -952,9 +983,9 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
       free_b = ub;
       ua = na;
     }
-    if (g.partial) {
+    if (part >= 0 && g.splits > 1) {
       f32x4* dst = reinterpret_cast<f32x4*>(g.partial) +
-                   (static_cast<int64_t>(p) * 8 + wave) * (kMB * kNB * 4 * 64) + lane;
+                   (partial_at(g, tile, part) * 8 + wave) * (kMB * kNB * 4 * 64) + lane;
 #pragma unroll
       for (int jj = 0; jj < 2 * kMB; ++jj)
 #pragma unroll
@@ -979,25 +1010,25 @@ __global__ __launch_bounds__(512, kMB * kNB == 2 ? 4 : 2) void lin_kernel(const 
 #undef TM_TR
 }
 
-// The partial tiles of split s of tile t are at position s T + t, in the order of the accumulators
-// (a wave's 64 lanes of one register group consecutive): summed split 0 first, then the strip's end.
+// A split tile's parts lie one after the other, each in the order of the accumulators (a wave's 64 lanes of one
+// register group consecutive): summed in order, then the end of the tile's.
 template <int kMB, int kNB, int kMode>
 __global__ __launch_bounds__(256) void lin_finish_kernel(const Args g) {
   using C = Tile<kMB, kNB>;
   __shared__ __attribute__((aligned(1024))) uint8_t strips[4 * C::kStrip];
   const int lane = threadIdx.x & 63;
   const int w4 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int T = g.tiles_m * g.tiles_n * g.batch;
-  const int id = static_cast<int>(blockIdx.x) * 4 + w4;  // (tile, wave, jj)
-  const int t = id / (8 * kMB);
-  if (t >= T) return;
+  const int T = g.tiles_m * g.tiles_n * g.batch, t8 = (T + 7) / 8;
+  const int id = static_cast<int>(blockIdx.x) * 4 + w4;  // (split tile, wave, jj)
+  const int xcd = id / (8 * kMB) / (t8 - g.whole), t = xcd * t8 + g.whole + id / (8 * kMB) % (t8 - g.whole);
+  if (xcd >= 8 || t >= T) return;
   const int wave = (id / kMB) % 8, jj = id % kMB;
-  int split, batch, m0, n0;
-  place<C::kTM, C::kTN, kMode == kGate>(g, t, split, batch, m0, n0);
+  int batch, m0, n0;
+  place<C::kTM, C::kTN, kMode == kGate>(g, t, batch, m0, n0);
   constexpr int kVec = kNB * 4;
   const f32x4* src = reinterpret_cast<const f32x4*>(g.partial) +
-                     (static_cast<int64_t>(t) * 8 + wave) * (kMB * kNB * 4 * 64) + jj * kVec * 64 + lane;
-  const int64_t step = static_cast<int64_t>(T) * 8 * (kMB * kNB * 4 * 64);
+                     (partial_at(g, t, 0) * 8 + wave) * (kMB * kNB * 4 * 64) + jj * kVec * 64 + lane;
+  const int64_t step = 8 * (kMB * kNB * 4 * 64);
   f32x4 sum[kVec];
 #pragma unroll
   for (int i = 0; i < kVec; ++i) sum[i] = src[i * 64];
@@ -1116,16 +1147,19 @@ __global__ __launch_bounds__((Few<kMT, kMode>::kWaves * 64)) void lin_rows_kerne
 
 constexpr int64_t kPad = 64;  // [d0 | d1]: each half is padded to a multiple of this
 constexpr int64_t kMaxPartialBytes = int64_t(2) << 30;
-// Measured on MI355X (sweeps of tiles and splits over the block's products at 8192 rows): microseconds of a
-// slice and of a tile's end, by tile. The ends of a round of tiles come together and are bound by memory;
-// the gate's, by what they read and write more. Up to 128 workgroups run at a higher clock.
+// Measured on MI355X: microseconds of a slice and of a tile's end, by tile, fitted to a sweep of 15 tilings and
+// splits of 22 products (the block's forward, gradient and weight-gradient products at 8192 rows and some of
+// 1999 rows; 8192 x 9728 -> 2560, 320 tiles of 256 x 256: 357 us with 256 of them whole and the others in
+// four parts, 418 unsplit, 386 in tiles of 192 x 256). With them the choice took at most 5% more time than
+// the best of the 15. The ends of a round of tiles come together and are bound by memory: the gate's, by
+// what they read and write more.
 struct Cost {
   int mb, nb;
   double slice, end;
 };
-constexpr Cost kCosts[] = {{4, 2, 1.37, 6.0}, {3, 2, 1.24, 5.0}, {2, 2, 0.95, 4.0}, {2, 1, 0.95, 5.0}};
-constexpr double kUsSliceAlone = 0.62, kUsEndAlone = 3.0;  // 128 x 128 tiles, one workgroup on a CU instead of two
-constexpr double kUsLaunch = 3.0, kUsReduce = 5.0, kBytesPerUs = 4.5e6, kFewer = 0.9;
+constexpr Cost kCosts[] = {{4, 2, 1.25, 7.0}, {3, 2, 1.24, 3.8}, {2, 2, 0.95, 4.0}, {2, 1, 1.0, 2.9}};
+constexpr double kUsSliceAlone = 0.62, kUsEndAlone = 3.3;  // 128 x 128 tiles, one workgroup on a CU instead of two
+constexpr double kUsLaunch = 3.0, kUsReduce = 3.8, kBytesPerUs = 5.7e6;
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -1139,52 +1173,70 @@ struct Product {
 
 struct Plan {
   int mb, nb;      // tile of 64 mb x 128 nb
-  int64_t splits;
+  int64_t whole;   // an XCD's tiles before its split ones
+  int64_t splits;  // of those
   double us;
 };
 
-Plan plan_of(const Product& q, const Cost& c, int64_t splits) {
-  const int64_t tm = 64 * c.mb, tn = 128 * c.nb / (q.gate ? 2 : 1);
-  const int64_t tiles = ceil_div(q.m, tm) * ceil_div(q.n, tn) * q.batch, wgs = tiles * splits;
-  const int64_t per = ceil_div(q.slices, splits);
-  double us = kUsLaunch;
-  if (c.nb == 2) us += ceil_div(wgs, 256) * (per * c.slice * (wgs <= 128 ? kFewer : 1.0) + c.end * q.ends);
-  else if (wgs <= 256) us += per * kUsSliceAlone + kUsEndAlone * q.ends;
-  else us += ceil_div(wgs, 512) * (per * c.slice + c.end * q.ends);
-  if (splits > 1) us += kUsReduce + static_cast<double>(wgs) * (tm * 128 * c.nb) * 8.0 / kBytesPerUs;
-  return {c.mb, c.nb, splits, us};
+int64_t tiles_of(const Product& q, int mb, int nb) {
+  return ceil_div(q.m, 64 * mb) * ceil_div(q.n, 128 * nb / (q.gate ? 2 : 1)) * q.batch;
 }
 
-// The tile and the number of splits with the least estimated time.
+// Split tiles' parts in the workspace.
+int64_t parts_of(const Product& q, int mb, int nb, int64_t whole, int64_t splits) {
+  return splits > 1 ? 8 * (ceil_div(tiles_of(q, mb, nb), 8) - whole) * splits : 0;
+}
+
+Plan plan_of(const Product& q, const Cost& c, int64_t whole, int64_t splits) {
+  const int64_t per_xcd = ceil_div(tiles_of(q, c.mb, c.nb), 8), rest = (per_xcd - whole) * splits;
+  const int64_t per = ceil_div(q.slices, splits), parts = parts_of(q, c.mb, c.nb, whole, splits);
+  const bool pair = c.mb * c.nb == 2;
+  double us = kUsLaunch;
+  auto rounds = [&](int64_t n, int64_t slices, bool ends) {
+    const double end = ends ? c.end * q.ends : c.end;
+    if (!pair) return ceil_div(n, 32) * (slices * c.slice + end);
+    if (whole == 0 && n <= 32) return slices * kUsSliceAlone + kUsEndAlone * (ends ? q.ends : 1.0);
+    return ceil_div(n, 64) * (slices * c.slice + end);
+  };
+  us += rounds(whole, q.slices, true) * (whole > 0) + rounds(rest, per, splits == 1) * (rest > 0);
+  if (parts) us += kUsReduce + static_cast<double>(parts) * (64 * c.mb * 128 * c.nb) * 8.0 / kBytesPerUs;
+  return {c.mb, c.nb, whole, splits, us};
+}
+
+// The tile, which of the tiles are split, and in how many parts, with the least estimated time: none, all, or
+// those that whole rounds over the CUs leave over.
 Plan best_plan(const Product& q) {
-  Plan best = {0, 0, 0, 0.0};
+  Plan best = {0, 0, 0, 0, 0.0};
   for (const Cost& c : kCosts) {
     if (c.mb == 2 && (c.nb == 2) != q.gate) continue;
-    const int64_t tiles = ceil_div(q.m, 64 * c.mb) * ceil_div(q.n, 128 * c.nb / (q.gate ? 2 : 1)) * q.batch;
+    const int64_t per_xcd = ceil_div(tiles_of(q, c.mb, c.nb), 8), room = c.mb * c.nb == 2 ? 64 : 32;
+    const int64_t full = per_xcd / room * room;
     for (int64_t s = 1; s <= 64 && s <= q.slices; ++s) {
-      if (ceil_div(q.slices, ceil_div(q.slices, s)) != s) continue;  // some split would be empty
-      if (s > 1 && tiles * s * (64 * c.mb) * (128 * c.nb) * 4 > kMaxPartialBytes) break;
-      const Plan p = plan_of(q, c, s);
-      if (best.splits == 0 || p.us < best.us) best = p;
+      if (ceil_div(q.slices, ceil_div(q.slices, s)) != s) continue;  // some part would be empty
+      for (int64_t whole : {int64_t(0), full}) {
+        if ((s == 1 && whole) || whole == per_xcd) continue;
+        if (parts_of(q, c.mb, c.nb, whole, s) * (64 * c.mb) * (128 * c.nb) * 4 > kMaxPartialBytes) continue;
+        const Plan p = plan_of(q, c, whole, s);
+        if (best.splits == 0 || p.us < best.us) best = p;
+        if (full == 0) break;
+      }
     }
   }
   return best;
 }
 
 size_t partial_bytes(const Product& q, const Plan& p) {
-  if (p.splits <= 1) return 0;
-  const int64_t tiles = ceil_div(q.m, 64 * p.mb) * ceil_div(q.n, 128 * p.nb / (q.gate ? 2 : 1)) * q.batch;
-  return static_cast<size_t>(tiles * p.splits) * (64 * p.mb) * (128 * p.nb) * sizeof(float);
+  return static_cast<size_t>(parts_of(q, p.mb, p.nb, p.whole, p.splits)) * (64 * p.mb) * (128 * p.nb) * sizeof(float);
 }
 
 Product product_of(int op, int64_t rows, int64_t inp, int64_t out, bool two) {
   switch (op) {
     case TM_LIN_FORWARD: return {rows, out, ceil_div(inp, kSliceK), 1, false, 1.0};
-    case TM_LIN_GATE: return {rows, out, ceil_div(inp, kSliceK), 1, true, 1.5};
+    case TM_LIN_GATE: return {rows, out, ceil_div(inp, kSliceK), 1, true, 1.85};
     case TM_LIN_GRAD_X: return {rows, inp,
                                two ? 2 * ceil_div(out, kPad) * (kPad / kSliceK) : ceil_div(out, kSliceK), 1,
                                false, 1.0};
-    case TM_LIN_GATE_GRAD: return {rows, inp, ceil_div(out, kSliceK), 1, false, 5.0};
+    case TM_LIN_GATE_GRAD: return {rows, inp, ceil_div(out, kSliceK), 1, false, 7.5};
     default: return {out, inp, ceil_div(rows, kSliceK), two ? 2 : 1, false, 1.0};
   }
 }
@@ -1234,15 +1286,15 @@ int launch_one(int which, Args& g, hipStream_t s) {
   const void* fn = reinterpret_cast<const void*>(lin_kernel<kMB, kNB, kAK, kBK, kRagged, kMode>);
   hipError_t e = allow_lds(s, which, fn, C::kLds, &cus);
   if (e != hipSuccess) return lin_fail(TM_ELAUNCH, "tm_lin: LDS attribute: %s", hipGetErrorString(e));
-  const int64_t positions = static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.batch * g.splits;
-  const int64_t per_xcd = ceil_div(positions, 8), room = (cus >= 16 ? cus / 8 : 1) * (2 * C::kLds <= 163840 ? 2 : 1);
+  const int64_t t8 = ceil_div(static_cast<int64_t>(g.tiles_m) * g.tiles_n * g.batch, 8);
+  const int64_t per_xcd = g.whole + (t8 - g.whole) * g.splits, room = (cus >= 16 ? cus / 8 : 1) * (2 * C::kLds <= 163840 ? 2 : 1);
   g.wpx = static_cast<int>(per_xcd < room ? per_xcd : room);
   hipLaunchKernelGGL((lin_kernel<kMB, kNB, kAK, kBK, kRagged, kMode>), dim3(static_cast<uint32_t>(8 * g.wpx)), dim3(512), C::kLds,
                      s, g);
   e = hipGetLastError();
   if (e != hipSuccess) return lin_fail(TM_ELAUNCH, "lin_kernel: launch failed: %s", hipGetErrorString(e));
   if (g.splits > 1) {
-    const int64_t waves = positions / g.splits * 8 * kMB;
+    const int64_t waves = 8 * (t8 - g.whole) * 8 * kMB;
     hipLaunchKernelGGL((lin_finish_kernel<kMB, kNB, kMode>), dim3(static_cast<uint32_t>(ceil_div(waves, 4))), dim3(256),
                        0, s, g);
     e = hipGetLastError();
@@ -1358,6 +1410,7 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
       g.ka = g.kb = static_cast<int>(d->rows);
       g.a_batch = ceil_div(d->out, kPad) * kPad * 2;
   }
+  g.whole = static_cast<int>(p.whole);
   g.splits = static_cast<int>(p.splits);
   g.per = static_cast<int>(ceil_div(q.slices, p.splits));
   const int64_t tiles_m = ceil_div(q.m, 64 * p.mb), tiles_n = ceil_div(q.n, 128 * p.nb / (q.gate ? 2 : 1));
