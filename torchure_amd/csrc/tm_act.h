@@ -100,18 +100,61 @@ __device__ __forceinline__ int block_exponent(uint32_t most) {
 }
 __device__ __forceinline__ float two_to(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
-// Four values times `inv` (2^-e) -> four e4m3 bytes, round to nearest even.
+// Four values times `inv` (2^-e) -> four e4m3 bytes, round to nearest even. kAny: any values; else none past the
+// range (NaN becomes NaN).
 __device__ __forceinline__ float e4m3_range(float x, float inv) {
-  const float v = x * inv;
-  const float c = __builtin_amdgcn_fmed3f(v, -448.0f, 448.0f);
+  const float c = __builtin_amdgcn_fmed3f(x * inv, -448.0f, 448.0f);
   return finite_bits(x) != 0u || x == 0.0f ? c : __uint_as_float(0x7FC00000u);
 }
+template <bool kAny>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv) {
   uint32_t w = 0;
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(a, inv), e4m3_range(b, inv), w, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(c, inv), e4m3_range(d, inv), w, true);
+  if constexpr (kAny) {
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(a, inv), e4m3_range(b, inv), w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(c, inv), e4m3_range(d, inv), w, true);
+  } else {
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, w, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, w, true);
+  }
   return w;
 }
+
+// The largest over the 16 lanes of a row, in each of them. (DPP moves: no LDS.)
+__device__ __forceinline__ uint32_t row_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x121, 0xF, 0xF, true)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x122, 0xF, 0xF, true)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x124, 0xF, 0xF, true)));
+  return max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, true)));
+}
+// ... over the wave.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+  v = row_max(v);
+  const uint32_t a = max(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 0)),
+                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 16)));
+  const uint32_t b = max(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 32)),
+                         static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 48)));
+  return max(a, b);
+}
+
+// Past this a block's values are looked at one by one (the clamped exponent, infinities); below, the largest
+// magnitude that is no NaN is the largest finite one, and times 2^-e nothing is past 448.
+constexpr uint32_t kPlainMost = 0x7F600000u;  // 1.75 2^127
+// The largest magnitude of n values as bits, NaN left out.
+template <int n>
+__device__ __forceinline__ uint32_t largest(const float* x) {
+  float m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < n; ++i) m = fmaxf(m, fabsf(x[i]));
+  return __float_as_uint(m);
+}
+template <int n>
+__device__ __forceinline__ uint32_t largest_finite(const float* x) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < n; ++i) m = max(m, finite_bits(x[i]));
+  return m;
+}
+
 // Four e4m3 bytes times `scale` (2^e), exact.
 __device__ __forceinline__ f32x4 decode4(uint32_t w, float scale) {
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);

@@ -24,6 +24,11 @@ int act_fail(int code, const char* fmt, A... args) {
   return tm_internal_fail(code, fmt, args...);
 }
 
+template <bool kV>
+struct Bool {
+  static constexpr bool value = kV;
+};
+
 // Eight bf16 or fp32 values of a row; `left` of them exist (zeros after), vec: 16-byte pieces.
 template <bool kF32>
 __device__ __forceinline__ void get8(float (&x)[8], const void* base, int64_t at, int left, bool vec) {
@@ -91,33 +96,51 @@ __global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ val
   if (n0 >= cols) return;
   const int64_t m = band * 32 + (lane >> 3);
   float x[4][8];
-  uint32_t most = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const bool in = m + 8 * i < rows;
     get8<kF32>(x[i], src, in ? (m + 8 * i) * lds + n : 0, in ? cols - n : 0, vec != 0);
   }
+  // over the block's lanes: l, l ^ 1, l ^ 2, l ^ 8 in a row of 16, and the four rows
+  auto over_block = [](uint32_t v) {
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0xB1, 0xF, 0xF, true)));
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x4E, 0xF, 0xF, true)));
+    v = max(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x128, 0xF, 0xF, true)));
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int d : {16, 32}) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d)));
+    return v;
+  };
+  uint32_t most = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) most = max(most, tm_act::finite_bits(x[i][e]));
+  for (int i = 0; i < 4; ++i) most = max(most, tm_act::largest<8>(x[i]));
+  most = over_block(most);
+  auto encode = [&](auto any) {
+    constexpr bool kAny = decltype(any)::value;
+    const int e2 = tm_act::block_exponent(most);
+    const float inv = tm_act::two_to(-e2);
 #pragma unroll
-  for (int d : {1, 2, 8, 16, 32}) most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), d)));
-  const int e2 = tm_act::block_exponent(most);
-  const float inv = tm_act::two_to(-e2);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (m + 8 * i >= rows) continue;
-    if (n < ldv) {
-      const u32x2 w = {tm_act::encode4(x[i][0], x[i][1], x[i][2], x[i][3], inv),
-                       tm_act::encode4(x[i][4], x[i][5], x[i][6], x[i][7], inv)};
-      *reinterpret_cast<u32x2*>(values + (m + 8 * i) * ldv + n) = w;
+    for (int i = 0; i < 4; ++i) {
+      if (m + 8 * i >= rows) continue;
+      if (n < ldv) {
+        const u32x2 w = {tm_act::encode4<kAny>(x[i][0], x[i][1], x[i][2], x[i][3], inv),
+                         tm_act::encode4<kAny>(x[i][4], x[i][5], x[i][6], x[i][7], inv)};
+        *reinterpret_cast<u32x2*>(values + (m + 8 * i) * ldv + n) = w;
+      }
+      if (copy && n < ldc) put8<false>(copy, (m + 8 * i) * ldc + n, x[i], 8, true);
     }
-    if (copy && n < ldc) put8<false>(copy, (m + 8 * i) * ldc + n, x[i], 8, true);
+    const int block = (n0 >> 5) + ((lane >> 2) & 1);
+    if ((lane & ~4) == 0 && block * 32 < cols)
+      exps[band * ((cols + 31) / 32) + block] = static_cast<uint8_t>(e2 + 127);
+  };
+  if (__builtin_amdgcn_ballot_w64(most >= tm_act::kPlainMost) == 0) {
+    encode(Bool<false>{});
+  } else {  // some block with an infinity or values next to the type's largest
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = max(most, tm_act::largest_finite<8>(x[i]));
+    most = over_block(most);
+    encode(Bool<true>{});
   }
-  const int block = (n0 >> 5) + ((lane >> 2) & 1);
-  if ((lane & ~4) == 0 && block * 32 < cols)
-    exps[band * ((cols + 31) / 32) + block] = static_cast<uint8_t>(e2 + 127);
 }
 
 template <bool kF32>

@@ -333,13 +333,6 @@ __device__ __forceinline__ void put8(char* p, const float* x, bool f32, int left
   }
 }
 
-// The largest of a value over the wave's lanes.
-__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d)));
-  return v;
-}
-
 // Where a block is, and which of a lane's values exist (kWhole: all).
 struct Spot {
   int m0, n0;
@@ -378,18 +371,21 @@ __device__ __forceinline__ void hold(const End& g, const Lane& l, const Block& b
       if (kWhole || (s.row[i] && s.n0 + 8 * (lane & 3) < g.ldz))
         put8(at_block(z, g.ldz, 2, s, i) + l.z, b.v + 8 * i, false);
   } else {
-    uint32_t most = 0;
+    auto encode = [&](uint32_t most, auto any) {
+      const int e = tm_act::block_exponent(most);
+      const float inv = tm_act::two_to(-e);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) most = max(most, tm_act::finite_bits(b.v[i]));
-    const int e = tm_act::block_exponent(wave_max(most));
-    const float inv = tm_act::two_to(-e);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const float* x = b.v + 8 * i;
-      const u32x2 w = {tm_act::encode4(x[0], x[1], x[2], x[3], inv), tm_act::encode4(x[4], x[5], x[6], x[7], inv)};
-      if (kWhole || s.row[i]) *reinterpret_cast<u32x2*>(at_block(z, g.ldz, 1, s, i) + l.z) = w;
-    }
-    if (lane == 0) exps[exponent_at(g, s)] = static_cast<uint8_t>(e + 127);
+      for (int i = 0; i < 2; ++i) {
+        const float* x = b.v + 8 * i;
+        const u32x2 w = {tm_act::encode4<decltype(any)::value>(x[0], x[1], x[2], x[3], inv),
+                         tm_act::encode4<decltype(any)::value>(x[4], x[5], x[6], x[7], inv)};
+        if (kWhole || s.row[i]) *reinterpret_cast<u32x2*>(at_block(z, g.ldz, 1, s, i) + l.z) = w;
+      }
+      if (lane == 0) exps[exponent_at(g, s)] = static_cast<uint8_t>(e + 127);
+    };
+    const uint32_t most = tm_act::wave_max(tm_act::largest<16>(b.v));
+    if (most < tm_act::kPlainMost) encode(most, Bool<false>{});
+    else encode(tm_act::wave_max(tm_act::largest_finite<16>(b.v)), Bool<true>{});
   }
 }
 
