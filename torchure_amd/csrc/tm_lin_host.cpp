@@ -89,7 +89,7 @@ Tensor room(const Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
 }
 
 // A tensor as rows of its last dimension, the elements of a row next to each other, rows apart by at least their
-// length. (The tensor is kept alive by its own storage where no copy is made.)
+// length and less than 2^23 elements. (The tensor is kept alive by its own storage where no copy is made.)
 struct Rows {
   Tensor t;
   i64 n = 0, d = 0, ld = 0;
@@ -100,7 +100,8 @@ Rows rows_of(const Tensor& given) {
   if (t.is_neg()) t = t.resolve_neg();
   const i64 d = t.size(-1), n = d ? t.numel() / d : 0;
   if (t.dim() != 2) t = t.reshape({n, d});
-  if ((d > 1 && t.stride(1) != 1) || (n > 1 && t.stride(0) < d)) t = t.contiguous();
+  if ((d > 1 && t.stride(1) != 1) || (n > 1 && (t.stride(0) < d || t.stride(0) >= (1 << 23))))
+    t = t.contiguous();
   return {t, n, d, n > 1 ? t.stride(0) : d};
 }
 

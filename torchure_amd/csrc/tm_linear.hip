@@ -213,12 +213,14 @@ struct Block {
 // in each matrix (rows 16 on: 16 rows more).
 struct Lane {
   uint32_t w[2], r[2];
+  uint32_t strip;
   uint32_t out, out1, res, z;
 };
 
 template <int kMode>
 __device__ __forceinline__ Lane lane_of(const End& g, uint32_t stg, int lane) {
   Lane l;
+  l.strip = stg;
   const uint32_t row = lane & 15, r = lane >> 2, sr = (r >> 1) & 7, c = 2 * (lane & 3), col = 8 * (lane & 3);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -276,12 +278,16 @@ struct Raw8 {
   u32x4 w[2];
 };
 
-__device__ __forceinline__ Raw8 raw8(const char* p, bool f32) {  // 16-byte aligned
-  Raw8 r;
-  r.w[0] = *reinterpret_cast<const u32x4*>(p);
-  r.w[1] = u32x4{0, 0, 0, 0};
-  if (f32) r.w[1] = *reinterpret_cast<const u32x4*>(p + 16);
-  return r;
+// What is at p is in memory: the compiler cannot tell from a pointer that the kernel's arguments hold, and its
+// flat accesses would count as LDS accesses too, which the strip's reads wait for.
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(1))) T* mem(const void* p) {
+  return (__attribute__((address_space(1))) T*)reinterpret_cast<uintptr_t>(p);
+}
+
+// 16-byte aligned. No branch: where two ways of loading meet, the loads are waited for, early or not.
+__device__ __forceinline__ Raw8 raw8(const char* p, bool f32) {
+  return {{*mem<u32x4>(p), *mem<u32x4>(p + (f32 ? 16 : 0))}};
 }
 
 __device__ __forceinline__ Raw8 raw8(const char* p, bool f32, int left, bool vec) {  // `left` of them exist
@@ -290,8 +296,8 @@ __device__ __forceinline__ Raw8 raw8(const char* p, bool f32, int left, bool vec
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     if (e < left) {
-      if (f32) w[e] = reinterpret_cast<const uint32_t*>(p)[e];
-      else w[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
+      if (f32) w[e] = mem<uint32_t>(p)[e];
+      else w[e / 2] |= static_cast<uint32_t>(mem<uint16_t>(p)[e]) << (16 * (e & 1));
     }
   return {{u32x4{w[0], w[1], w[2], w[3]}, u32x4{w[4], w[5], w[6], w[7]}}};
 }
@@ -312,24 +318,41 @@ __device__ __forceinline__ void values8(float* x, const Raw8& r, bool f32) {
 
 __device__ __forceinline__ void put8(char* p, const float* x, bool f32) {  // 16-byte aligned
   if (f32) {
-    reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-    reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+    mem<f32x4>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
+    mem<f32x4>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
   } else {
-    *reinterpret_cast<u32x4*>(p) =
+    *mem<u32x4>(p) =
         u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
   }
 }
 
-__device__ __forceinline__ void put8(char* p, const float* x, bool f32, int left, bool vec) {
-  if (vec && left >= 8) {
-    put8(p, x, f32);
-  } else {
+// Rows that do not start on 16 bytes, or end within a lane's 8 columns: half a block (16 rows) through the
+// strip, so that a lane has one column of row pairs and an access two whole rows of 32 columns.
+__device__ __forceinline__ uint32_t column_at(const Lane& l, int row, int lane) {
+  return l.strip + row * 128 + ((((lane & 31) >> 2) ^ (row >> 1)) << 4) + (lane & 3) * 4;
+}
+
+__device__ __forceinline__ void put_columns(const Lane& l, char* p, uint32_t ld, const float* x, bool f32, int rows,
+                                            int cols, int lane) {
+  asm volatile("ds_write_b128 %0, %2\n\tds_write_b128 %1, %3" ::"v"(l.r[0]), "v"(l.r[1]),
+               "v"(f32x4{x[0], x[1], x[2], x[3]}), "v"(f32x4{x[4], x[5], x[6], x[7]})
+               : "memory");
+  const int c = lane & 31;
+#pragma unroll 1
+  for (int r0 = lane >> 5; r0 < 16; r0 += 4) {
+    float v[2];
+    asm volatile("ds_read_b32 %0, %2\n\tds_read_b32 %1, %3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(v[0]), "=&v"(v[1])
+                 : "v"(column_at(l, r0, lane)), "v"(column_at(l, r0 + 2, lane))
+                 : "memory");
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < left) {
-        if (f32) reinterpret_cast<float*>(p)[e] = x[e];
-        else reinterpret_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(pack_bf16(x[e], 0.0f));
-      }
+    for (int i = 0; i < 2; ++i) {
+      const int r = r0 + 2 * i;
+      if (r >= rows || c >= cols) continue;
+      const uint32_t at = static_cast<uint32_t>(r) * ld + c;
+      if (f32) *mem<float>(p + at * 4u) = v[i];
+      else *mem<uint16_t>(p + at * 2u) = static_cast<uint16_t>(pack_bf16(v[i], 0.0f));
+    }
   }
 }
 
@@ -379,9 +402,9 @@ __device__ __forceinline__ void hold(const End& g, const Lane& l, const Block& b
         const float* x = b.v + 8 * i;
         const u32x2 w = {tm_act::encode4<decltype(any)::value>(x[0], x[1], x[2], x[3], inv),
                          tm_act::encode4<decltype(any)::value>(x[4], x[5], x[6], x[7], inv)};
-        if (kWhole || s.row[i]) *reinterpret_cast<u32x2*>(at_block(z, g.ldz, 1, s, i) + l.z) = w;
+        if (kWhole || s.row[i]) *mem<u32x2>(at_block(z, g.ldz, 1, s, i) + l.z) = w;
       }
-      if (lane == 0) exps[exponent_at(g, s)] = static_cast<uint8_t>(e + 127);
+      if (lane == 0) *mem<uint8_t>(exps + exponent_at(g, s)) = static_cast<uint8_t>(e + 127);
     };
     const uint32_t most = tm_act::wave_max(tm_act::largest<16>(b.v));
     if (most < tm_act::kPlainMost) encode(most, Bool<false>{});
@@ -402,7 +425,6 @@ __device__ __forceinline__ Early early_of(const End& g, const Lane& l, int m0, i
   if (!kWhole && (m0 >= g.m || n0 >= g.n)) return r;
   const Spot s = spot_of(g, m0, n0, lane);
   if constexpr (kMode <= kResidual) {
-    if (kMode == kLinear && !g.res) return r;
     const int size = g.res_f32 ? 4 : 2;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -418,23 +440,22 @@ __device__ __forceinline__ Early early_of(const End& g, const Lane& l, int m0, i
     for (int i = 0; i < 2; ++i) {
       if (!kWhole && !(s.row[i] && (!bf16 || s.n0 + 8 * (lane & 3) < g.ldz))) continue;
       const char *pg = at_block(g.z0, g.ldz, bf16 ? 2 : 1, s, i), *pu = at_block(g.z1, g.ldz, bf16 ? 2 : 1, s, i);
-      if (bf16) {
-        r.a[i].w[0] = *reinterpret_cast<const u32x4*>(pg + l.z);
-        r.b[i].w[0] = *reinterpret_cast<const u32x4*>(pu + l.z);
-      } else {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(pg + l.z), y = *reinterpret_cast<const u32x2*>(pu + l.z);
-        r.a[i].w[0] = u32x4{x.x, x.y, 0, 0};
-        r.b[i].w[0] = u32x4{y.x, y.y, 0, 0};
-      }
+      auto load = [&](const char* p) {
+        const u32x2 x = *mem<u32x2>(p), y = *mem<u32x2>(p + (bf16 ? 8 : 0));
+        return u32x4{x.x, x.y, y.x, y.y};
+      };
+      r.a[i].w[0] = load(pg + l.z);
+      r.b[i].w[0] = load(pu + l.z);
     }
-    if (!bf16) {
-      r.exps[0] = g.s0[exponent_at(g, s)];
-      r.exps[1] = g.s1[exponent_at(g, s)];
-    }
+    const char *p0 = bf16 ? g.z0 : reinterpret_cast<const char*>(g.s0), *p1 = bf16 ? g.z1 : reinterpret_cast<const char*>(g.s1);
+    const int64_t at = bf16 ? 0 : exponent_at(g, s);
+    r.exps[0] = *mem<uint8_t>(p0 + at);
+    r.exps[1] = *mem<uint8_t>(p1 + at);
   }
   return r;
 }
 
+template <bool kWhole>
 __device__ __forceinline__ void add_residual(const End& g, Block& b, const Early& early) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -449,7 +470,7 @@ __device__ __forceinline__ void add_residual(const End& g, Block& b, const Early
 // is rounded to what the backward pass reads.
 template <bool kWhole>
 __device__ __forceinline__ void end_linear(const End& g, const Lane& l, Block& b, const Spot& s, const Raw8& bias,
-                                           const Early& early, int lane) {
+                                           int lane) {
   if (g.bias) {
     float x[8];
     values8(x, bias, g.bias_f32);
@@ -469,7 +490,10 @@ __device__ __forceinline__ void end_linear(const End& g, const Lane& l, Block& b
   else if (act == tm_act::kSilu) each([](float z) { return tm_act::act1(tm_act::kSilu, z); });
   else if (act == tm_act::kGelu) each([](float z) { return tm_act::act1(tm_act::kGelu, z); });
   else if (act == tm_act::kGeluTanh) each([](float z) { return tm_act::act1(tm_act::kGeluTanh, z); });
-  if (g.res) add_residual(g, b, early);
+  if (g.res) {  // read here, not early: the registers are the activation's
+    if (kWhole && g.res_vec) add_residual<true>(g, b, early_of<kLinear, true>(g, l, s.m0, s.n0, lane));
+    else add_residual<false>(g, b, early_of<kLinear, false>(g, l, s.m0, s.n0, lane));
+  }
 }
 
 // A block of y, of a gradient: kWhole, in 16-byte pieces.
@@ -480,9 +504,7 @@ __device__ __forceinline__ void store_block(const End& g, const Lane& l, char* o
   for (int i = 0; i < 2; ++i) {
     char* p = at_block(out, g.ldo, size, s, i);
     if (kWhole) put8(p + l.out, b.v + 8 * i, g.out_f32);
-    else if (s.row[i] && s.cols > 0)
-      put8(p + (static_cast<int64_t>(lane >> 2) * g.ldo + 8 * (lane & 3)) * size, b.v + 8 * i, g.out_f32, s.cols,
-           g.out_vec);
+    else put_columns(l, p, static_cast<uint32_t>(g.ldo), b.v + 8 * i, g.out_f32, g.m - s.m0 - 16 * i, g.n - s.n0, lane);
   }
 }
 
@@ -553,8 +575,8 @@ template <int kMode, bool kWhole>
 __device__ __forceinline__ void end_block(const End& g, const Lane& l, int batch, Block& x, Block& y, int m, int n,
                                           const Raw8& bias, const Early& early, int lane) {
   const Spot s = spot_of(g, m, n, lane);
-  if constexpr (kMode == kLinear) end_linear<kWhole>(g, l, x, s, bias, early, lane);
-  if constexpr (kMode == kResidual) add_residual(g, x, early);
+  if constexpr (kMode == kLinear) end_linear<kWhole>(g, l, x, s, bias, lane);
+  if constexpr (kMode == kResidual) add_residual<kWhole>(g, x, early);
   if constexpr (kMode <= kPlain) store_block<kWhole>(g, l, kMode == kPlain && batch ? g.o1 : g.o0, x, s, lane);
   else if constexpr (kMode == kGate) end_gate<kWhole>(g, l, x, y, s, lane);
   else end_gate_grad<kWhole>(g, l, x, s, early, lane);
@@ -603,19 +625,22 @@ __device__ __forceinline__ void finish(f32x4 (&acc)[2 * kRowBlocks][2 * kColBloc
 #pragma unroll 1
   for (int b = 0; b < kBlocks; ++b) {
     const int m = m0 + b % kRowBlocks * 32, n = n0 + b / kRowBlocks * 32;
+    if (m >= g.m || n >= (kMode >= kGate ? g.n_store : g.n)) continue;
     if constexpr (kMode == kLinear)
       if (g.bias && b % kRowBlocks == 0)
         bias = raw8(g.bias + (static_cast<int64_t>(n) + 8 * (lane & 3)) * (g.bias_f32 ? 4 : 2), g.bias_f32,
                     g.n - n - 8 * (lane & 3), g.bias_vec);
-    const Early early = early_of<kMode, false>(g, l, m, n, lane);
+    Early early = {};
+    if constexpr (kReads) early = early_of<kMode, false>(g, l, m, n, lane);
     Block x, y;
 #pragma unroll
     for (int c = 0; c < kBlocks; ++c)
       if (b == c) pick(x, y, c);
-    if (m >= g.m || n >= (kMode >= kGate ? g.n_store : g.n)) continue;
     if (kMode == kLinear && whole) end_block<kMode, kMode == kLinear>(g, l, batch, x, y, m, n, bias, early, lane);
     else end_block<kMode, false>(g, l, batch, x, y, m, n, bias, early, lane);
   }
+  // vmcnt(0): else the slices' loop may wait in every slice for a load whose use a branch here has passed by.
+  __builtin_amdgcn_s_waitcnt(0x0f70);
 }
 
 // ------------------------------------------------------------------------------ the product
@@ -1195,7 +1220,9 @@ Plan plan_of(const Product& q, const Cost& c, int64_t whole, int64_t splits) {
     return ceil_div(n, 64) * (slices * c.slice + end);
   };
   us += rounds(whole, q.slices, true) * (whole > 0) + rounds(rest, per, splits == 1) * (rest > 0);
-  if (parts) us += kUsReduce + static_cast<double>(parts) * (64 * c.mb * 128 * c.nb) * 8.0 / kBytesPerUs;
+  if (parts)  // written, read and added up, and the split tiles' ends
+    us += kUsReduce + static_cast<double>(parts) * (64 * c.mb * 128 * c.nb) *
+                          (8.0 + 2.0 * (q.ends - 1.0) / static_cast<double>(splits)) / kBytesPerUs;
   return {c.mb, c.nb, whole, splits, us};
 }
 
@@ -1461,15 +1488,17 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
     return lin_fail(TM_EINVAL, "tm_lin: output rows %lld elements apart for %lld columns", (long long)d->ldo,
                     (long long)cols);
   }
-  const int64_t kNear = 1 << 24;  // rows this near keep a lane's offsets in 32 bits
-  g.out_vec = d->ldo < kNear && d->ldo % (g.out_f32 ? 4 : 8) == 0 && aligned(d->o0, 16) && aligned(d->o1, 16);
+  if (d->ldo >= (1 << 24) || d->ldr >= (1 << 24) || (d->res && d->ldr < cols))  // a lane's offsets have 32 bits
+    return lin_fail(TM_EINVAL, "tm_lin: output rows %lld and residual rows %lld elements apart, less than 2^24, at least "
+                    "%lld", (long long)d->ldo, (long long)d->ldr, (long long)cols);
+  g.out_vec = d->ldo % (g.out_f32 ? 4 : 8) == 0 && aligned(d->o0, 16) && aligned(d->o1, 16);
   g.bias = static_cast<const char*>(d->bias);
   g.bias_f32 = d->bias_f32 != 0;
-  g.bias_vec = aligned(d->bias, g.bias_f32 ? 16 : 8);
+  g.bias_vec = aligned(d->bias, 16);
   g.res = static_cast<const char*>(d->res);
   g.res_f32 = d->res_f32 != 0;
   g.ldr = d->ldr;
-  g.res_vec = d->ldr < kNear && d->ldr % (g.res_f32 ? 4 : 8) == 0 && aligned(d->res, 16);
+  g.res_vec = d->ldr % (g.res_f32 ? 4 : 8) == 0 && aligned(d->res, 16);
 
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (few_rows(op, d->rows, d->inp)) {
