@@ -22,6 +22,8 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));  // where rows start at any bf16, at any fp32
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 enum Act { kNone = 0, kRelu = 1, kSilu = 2, kGelu = 3, kGeluTanh = 4 };

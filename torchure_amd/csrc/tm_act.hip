@@ -18,66 +18,84 @@ using tm_act::f32x4;
 using tm_act::pack_bf16;
 using tm_act::u32x2;
 using tm_act::u32x4;
+using tm_act::u32x4_at2;
+using tm_act::u32x4_at4;
 
 template <typename... A>
 int act_fail(int code, const char* fmt, A... args) {
   return tm_internal_fail(code, fmt, args...);
 }
 
-template <bool kV>
-struct Bool {
-  static constexpr bool value = kV;
+template <int kV>
+struct Int {
+  static constexpr int value = kV;
 };
 
-// Eight bf16 or fp32 values of a row; `left` of them exist (zeros after), vec: 16-byte pieces.
+// Eight bf16 or fp32 values of a row; `left` of them exist (zeros after). Rows may start at any element: an access of
+// 16 bytes need not be aligned to them. (6001 x 1237 values back to fp32, whose rows are odd: 10.9 us so, 25.4 us
+// with an access an element.)
 template <bool kF32>
-__device__ __forceinline__ void get8(float (&x)[8], const void* base, int64_t at, int left, bool vec) {
-  if (vec && left >= 8) {
-    if constexpr (kF32) {
-      const f32x4* p = reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + at);
-      const f32x4 a = p[0], b = p[1];
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-      x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+struct Raw8 {
+  u32x4 w[kF32 ? 2 : 1];
+};
+
+template <bool kF32>
+__device__ __forceinline__ Raw8<kF32> get8(const void* base, int64_t at, int left) {
+  Raw8<kF32> r = {};
+  if constexpr (kF32) {
+    const float* p = static_cast<const float*>(base) + at;
+    if (left >= 8) {
+      r.w[0] = reinterpret_cast<const u32x4_at4*>(p)[0];
+      r.w[1] = reinterpret_cast<const u32x4_at4*>(p)[1];
     } else {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(base) + at);
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[2 * e] = tm_act::bf16_lo(w[e]);
-        x[2 * e + 1] = tm_act::bf16_hi(w[e]);
-      }
+      for (int e = 0; e < 7; ++e)
+        if (e < left) r.w[e / 4][e % 4] = reinterpret_cast<const uint32_t*>(p)[e];
     }
   } else {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if (left >= 8) {
+      r.w[0] = *reinterpret_cast<const u32x4_at2*>(p);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = 0.0f;
-      if (e < left)
-        x[e] = kF32 ? static_cast<const float*>(base)[at + e]
-                    : __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(base)[at + e]) << 16);
+      for (int e = 0; e < 7; ++e)
+        if (e < left) r.w[0][e / 2] |= static_cast<uint32_t>(p[e]) << (16 * (e % 2));
     }
+  }
+  return r;
+}
+
+template <bool kF32>
+__device__ __forceinline__ void values8(float (&x)[8], const Raw8<kF32>& r) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (kF32) x[e] = __uint_as_float(r.w[e / 4][e % 4]);
+    else x[e] = e % 2 ? tm_act::bf16_hi(r.w[0][e / 2]) : tm_act::bf16_lo(r.w[0][e / 2]);
   }
 }
 
 template <bool kF32>
-__device__ __forceinline__ void put8(void* base, int64_t at, const float (&x)[8], int left, bool vec) {
+__device__ __forceinline__ void put8(void* base, int64_t at, const float (&x)[8], int left) {
   if constexpr (kF32) {
     float* p = static_cast<float*>(base) + at;
-    if (vec && left >= 8) {
-      reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-      reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+    if (left >= 8) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        reinterpret_cast<u32x4_at4*>(p)[h] = u32x4{__float_as_uint(x[4 * h]), __float_as_uint(x[4 * h + 1]),
+                                                   __float_as_uint(x[4 * h + 2]), __float_as_uint(x[4 * h + 3])};
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < 7; ++e)
         if (e < left) p[e] = x[e];
     }
   } else {
     uint16_t* p = static_cast<uint16_t*>(base) + at;
     const uint32_t w[4] = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
-    if (vec && left >= 8) {
-      *reinterpret_cast<u32x4*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+    if (left >= 8) {
+      *reinterpret_cast<u32x4_at2*>(p) = u32x4{w[0], w[1], w[2], w[3]};
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int e = 0; e < 7; ++e)
         if (e < left) p[e] = static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1)));
     }
   }
@@ -88,7 +106,7 @@ __device__ __forceinline__ void put8(void* base, int64_t at, const float (&x)[8]
 template <bool kF32>
 __global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
                                                        int64_t ldv, const void* __restrict__ src, int64_t lds,
-                                                       int64_t rows, int cols, int vec, int wide,
+                                                       int64_t rows, int cols, int wide,
                                                        uint16_t* __restrict__ copy, int64_t ldc) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t band = blockIdx.x / wide;
@@ -99,7 +117,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ val
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const bool in = m + 8 * i < rows;
-    get8<kF32>(x[i], src, in ? (m + 8 * i) * lds + n : 0, in ? cols - n : 0, vec != 0);
+    values8<kF32>(x[i], get8<kF32>(src, in ? (m + 8 * i) * lds + n : 0, in ? cols - n : 0));
   }
   // over the block's lanes: l, l ^ 1, l ^ 2, l ^ 8 in a row of 16, and the four rows
   auto over_block = [](uint32_t v) {
@@ -115,7 +133,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ val
   for (int i = 0; i < 4; ++i) most = max(most, tm_act::largest<8>(x[i]));
   most = over_block(most);
   auto encode = [&](auto any) {
-    constexpr bool kAny = decltype(any)::value;
+    constexpr bool kAny = decltype(any)::value != 0;
     const int e2 = tm_act::block_exponent(most);
     const float inv = tm_act::two_to(-e2);
 #pragma unroll
@@ -126,20 +144,20 @@ __global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ val
                          tm_act::encode4<kAny>(x[i][4], x[i][5], x[i][6], x[i][7], inv)};
         *reinterpret_cast<u32x2*>(values + (m + 8 * i) * ldv + n) = w;
       }
-      if (copy && n < ldc) put8<false>(copy, (m + 8 * i) * ldc + n, x[i], 8, true);
+      if (copy && n < ldc) put8<false>(copy, (m + 8 * i) * ldc + n, x[i], 8);
     }
     const int block = (n0 >> 5) + ((lane >> 2) & 1);
     if ((lane & ~4) == 0 && block * 32 < cols)
       exps[band * ((cols + 31) / 32) + block] = static_cast<uint8_t>(e2 + 127);
   };
   if (__builtin_amdgcn_ballot_w64(most >= tm_act::kPlainMost) == 0) {
-    encode(Bool<false>{});
+    encode(Int<0>{});
   } else {  // some block with an infinity or values next to the type's largest
     most = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) most = max(most, tm_act::largest_finite<8>(x[i]));
     most = over_block(most);
-    encode(Bool<true>{});
+    encode(Int<1>{});
   }
 }
 
@@ -147,7 +165,7 @@ template <bool kF32>
 __global__ __launch_bounds__(256) void dequantize_kernel(void* __restrict__ dst, int64_t ldd,
                                                          const uint8_t* __restrict__ values,
                                                          const uint8_t* __restrict__ exps, int64_t ldv, int64_t rows,
-                                                         int cols, int vec, int wide) {
+                                                         int cols, int wide) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t band = blockIdx.x / wide;
   const int n0 = (static_cast<int>(blockIdx.x % wide) * 4 + wave) * 64, n = n0 + 8 * (lane & 7);
@@ -163,7 +181,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(void* __restrict__ dst,
     if (m + 8 * i >= rows) continue;
     const f32x4 a = tm_act::decode4(w[i].x, scale), b = tm_act::decode4(w[i].y, scale);
     const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    put8<kF32>(dst, (m + 8 * i) * ldd + n, x, cols - n, vec != 0);
+    put8<kF32>(dst, (m + 8 * i) * ldd + n, x, cols - n);
   }
 }
 
@@ -171,13 +189,15 @@ __global__ __launch_bounds__(256) void dequantize_kernel(void* __restrict__ dst,
 // with 128 rows, whose 256 workgroups leave a CU with four waves.)
 constexpr int kBandRows = 64, kPlainRows = 32;
 
-// A workgroup takes `band_rows` rows x 256 columns: thread t the columns 8 (t % 32) .. + 7 of rows t / 32, + 8, ...
-template <bool kF32>
+// A workgroup takes `band_rows` rows x 256 columns: thread t the columns 8 (t % 32) .. + 7 of rows t / 32, + 8, ...,
+// four rows' loads at once, without branches (where the ways of reading z met, each row's loads were waited for:
+// 8192 x 9728 bf16 dy and 8-bit z, silu, 103 us then, 83 us now, 4.8 TB/s).
+template <bool kF32, int kAct, bool kE4m3>
 __global__ __launch_bounds__(256) void act_grad_kernel(uint16_t* __restrict__ dz, int64_t lddz,
                                                        float* __restrict__ sums, const void* __restrict__ dy,
-                                                       int64_t ldy, int vec, const uint8_t* __restrict__ z,
-                                                       const uint8_t* __restrict__ exps, int64_t ldz, int held, int act,
-                                                       int64_t rows, int cols, int wide, int band_rows) {
+                                                       int64_t ldy, const uint8_t* __restrict__ z,
+                                                       const uint8_t* __restrict__ exps, int64_t ldz, int64_t rows,
+                                                       int cols, int wide, int band_rows) {
   const int t = threadIdx.x;
   const int64_t band = blockIdx.x / wide;
   const int n = static_cast<int>(blockIdx.x % wide) * 256 + 8 * (t & 31);
@@ -185,41 +205,49 @@ __global__ __launch_bounds__(256) void act_grad_kernel(uint16_t* __restrict__ dz
   const int blocks = (cols + 31) / 32;
   float total[8] = {};
   if (n < cols) {
-#pragma unroll 4
-    for (int64_t m = band * band_rows + (t >> 5); m < m_end; m += 8) {
-      float d[8];
-      get8<kF32>(d, dy, m * ldy + n, cols - n, vec != 0);
-      if (act != TM_ACT_NONE) {
-        float x[8];
-        if (held == TM_HELD_BF16) {
-          get8<false>(x, z, m * ldz + n, 8, true);
-        } else {
+    for (int64_t m0 = band * band_rows; m0 < m_end; m0 += 32) {
+      Raw8<kF32> d4[4];
+      Raw8<false> z4[4];
+      uint32_t exp = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t m = min(m0 + (t >> 5) + 8 * i, m_end - 1);
+        d4[i] = get8<kF32>(dy, m * ldy + n, cols - n);
+        if constexpr (kAct != TM_ACT_NONE && kE4m3) {
           const u32x2 w = *reinterpret_cast<const u32x2*>(z + m * ldz + n);
-          const float scale = tm_act::two_to(static_cast<int>(exps[(m >> 5) * blocks + (n >> 5)]) - 127);
-          const f32x4 a = tm_act::decode4(w.x, scale), b = tm_act::decode4(w.y, scale);
-          x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-          x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+          z4[i].w[0] = u32x4{w.x, w.y, 0, 0};
+        } else if constexpr (kAct != TM_ACT_NONE) {
+          z4[i].w[0] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(z) + m * ldz + n);
         }
-        auto each = [&](auto f) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] *= f(x[e]);
-        };
-        if (act == tm_act::kRelu) each([](float v) { return tm_act::act1_grad(tm_act::kRelu, v); });
-        else if (act == tm_act::kSilu) each([](float v) { return tm_act::act1_grad(tm_act::kSilu, v); });
-        else if (act == tm_act::kGelu) each([](float v) { return tm_act::act1_grad(tm_act::kGelu, v); });
-        else each([](float v) { return tm_act::act1_grad(tm_act::kGeluTanh, v); });
-        if (cols - n < 8)
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e >= cols) d[e] = 0.0f;
       }
+      if constexpr (kAct != TM_ACT_NONE && kE4m3) exp = exps[(m0 >> 5) * blocks + (n >> 5)];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) total[e] += d[e];
-      if (dz) put8<false>(dz, m * lddz + n, d, 8, true);
+      for (int i = 0; i < 4; ++i) {
+        const int64_t m = m0 + (t >> 5) + 8 * i;
+        if (m >= m_end) break;
+        float d[8];
+        values8<kF32>(d, d4[i]);
+        if constexpr (kAct != TM_ACT_NONE) {
+          float x[8];
+          if constexpr (kE4m3) {
+            const float scale = tm_act::two_to(static_cast<int>(exp) - 127);
+            const f32x4 a = tm_act::decode4(z4[i].w[0].x, scale), b = tm_act::decode4(z4[i].w[0].y, scale);
+            x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+            x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+          } else {
+            values8<false>(x, z4[i]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) d[e] = n + e < cols ? d[e] * tm_act::act1_grad(kAct, x[e]) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) total[e] += d[e];
+        if (dz) put8<false>(dz, m * lddz + n, d, 8);
+      }
     }
   } else if (dz && n < lddz) {  // whole groups of padding
     const float none[8] = {};
-    for (int64_t m = band * band_rows + (t >> 5); m < m_end; m += 8) put8<false>(dz, m * lddz + n, none, 8, true);
+    for (int64_t m = band * band_rows + (t >> 5); m < m_end; m += 8) put8<false>(dz, m * lddz + n, none, 8);
   }
   if (!sums) return;
   __shared__ float part[8][256];
@@ -285,15 +313,14 @@ int tm_quantize_e4m3(uint8_t* d_values, uint8_t* d_exponents, int64_t ldv, const
   if (d_copy && (ldc != ceil_div(cols, 8) * 8 || !aligned(d_copy, 16)))
     return act_fail(TM_EINVAL, "%s: copy rows %lld apart for %lld columns: the next multiple of 8, 16-byte aligned", who,
                     (long long)ldc, (long long)cols);
-  const int vec = lds % (src_f32 ? 4 : 8) == 0 && aligned(d_src, 16);
   const dim3 grid(static_cast<uint32_t>(groups));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (src_f32)
     hipLaunchKernelGGL(quantize_kernel<true>, grid, dim3(256), 0, s, d_values, d_exponents, ldv, d_src, lds, rows,
-                       static_cast<int>(cols), vec, static_cast<int>(wide), d_copy, ldc);
+                       static_cast<int>(cols), static_cast<int>(wide), d_copy, ldc);
   else
     hipLaunchKernelGGL(quantize_kernel<false>, grid, dim3(256), 0, s, d_values, d_exponents, ldv, d_src, lds, rows,
-                       static_cast<int>(cols), vec, static_cast<int>(wide), d_copy, ldc);
+                       static_cast<int>(cols), static_cast<int>(wide), d_copy, ldc);
   return launched(who);
 }
 
@@ -307,15 +334,14 @@ int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_v
   if (ldv != ceil_div(cols, 32) * 32 || !aligned(d_values, 16) || ldd < cols || !aligned(d_dst, dst_f32 ? 4 : 2))
     return act_fail(TM_EINVAL, "%s: values (rows %lld apart) need rows of the next multiple of 32 to %lld, 16-byte "
                     "aligned; output rows are %lld apart", who, (long long)ldv, (long long)cols, (long long)ldd);
-  const int vec = ldd % (dst_f32 ? 4 : 8) == 0 && aligned(d_dst, 16);
   const dim3 grid(static_cast<uint32_t>(groups));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dst_f32)
     hipLaunchKernelGGL(dequantize_kernel<true>, grid, dim3(256), 0, s, d_dst, ldd, d_values, d_exponents, ldv, rows,
-                       static_cast<int>(cols), vec, static_cast<int>(wide));
+                       static_cast<int>(cols), static_cast<int>(wide));
   else
     hipLaunchKernelGGL(dequantize_kernel<false>, grid, dim3(256), 0, s, d_dst, ldd, d_values, d_exponents, ldv, rows,
-                       static_cast<int>(cols), vec, static_cast<int>(wide));
+                       static_cast<int>(cols), static_cast<int>(wide));
   return launched(who);
 }
 
@@ -350,18 +376,29 @@ int tm_act_grad(uint16_t* d_dz, int64_t lddz, void* d_bias, int bias_f32, const 
   const size_t need = d_bias ? tm_act_grad_workspace_bytes(rows, cols) : 0;
   if (need && (!d_ws || ws_bytes < need || !aligned(d_ws, 4)))
     return act_fail(TM_EINVAL, "%s: workspace of %zu bytes, %zu needed", who, ws_bytes, need);
-  const int vec = ldy % (dy_f32 ? 4 : 8) == 0 && aligned(d_dy, 16);
   float* sums = d_bias ? static_cast<float*>(d_ws) : nullptr;
   const dim3 grid(static_cast<uint32_t>(bands * wide));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dy_f32)
-    hipLaunchKernelGGL(act_grad_kernel<true>, grid, dim3(256), 0, s, d_dz, lddz, sums, d_dy, ldy, vec,
-                       static_cast<const uint8_t*>(d_z), d_exponents, ldz, held, act, rows, static_cast<int>(cols),
-                       static_cast<int>(wide), band_rows);
-  else
-    hipLaunchKernelGGL(act_grad_kernel<false>, grid, dim3(256), 0, s, d_dz, lddz, sums, d_dy, ldy, vec,
-                       static_cast<const uint8_t*>(d_z), d_exponents, ldz, held, act, rows, static_cast<int>(cols),
-                       static_cast<int>(wide), band_rows);
+  auto launch = [&](auto f32, auto a, auto e4m3) {
+    hipLaunchKernelGGL((act_grad_kernel<decltype(f32)::value != 0, decltype(a)::value, decltype(e4m3)::value != 0>), grid,
+                       dim3(256), 0, s, d_dz, lddz, sums, d_dy, ldy, static_cast<const uint8_t*>(d_z), d_exponents, ldz,
+                       rows, static_cast<int>(cols), static_cast<int>(wide), band_rows);
+  };
+  auto by_held = [&](auto f32, auto a) {
+    if (held == TM_HELD_E4M3) launch(f32, a, Int<1>{});
+    else launch(f32, a, Int<0>{});
+  };
+  auto by_act = [&](auto f32) {
+    switch (act) {
+      case TM_ACT_NONE: return launch(f32, Int<TM_ACT_NONE>{}, Int<0>{});
+      case TM_ACT_RELU: return by_held(f32, Int<TM_ACT_RELU>{});
+      case TM_ACT_SILU: return by_held(f32, Int<TM_ACT_SILU>{});
+      case TM_ACT_GELU: return by_held(f32, Int<TM_ACT_GELU>{});
+      default: return by_held(f32, Int<TM_ACT_GELU_TANH>{});
+    }
+  };
+  if (dy_f32) by_act(Int<1>{});
+  else by_act(Int<0>{});
   if (const int rc = launched(who)) return rc;
   if (!d_bias) return TM_OK;
   hipLaunchKernelGGL(col_sum_kernel, dim3(static_cast<uint32_t>(ceil_div(cols, 64))), dim3(256), 0, s, d_bias, bias_f32,

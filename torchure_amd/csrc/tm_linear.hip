@@ -48,6 +48,8 @@ using tm_act::f32x4;
 using tm_act::pack_bf16;
 using tm_act::u32x2;
 using tm_act::u32x4;
+using tm_act::u32x4_at2;
+using tm_act::u32x4_at4;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
@@ -83,12 +85,12 @@ struct Args {
   char* o0;
   char* o1;                 // batch 1's output; gate_grad: silu(g) u
   int64_t ldo, ldo1;        // elements
-  int out_f32, out_vec, act;
+  int out_f32, act;
   int n_store;              // columns of an output row that are written (past n: zeros)
   const char* bias;
   const char* res;
   int64_t ldr;
-  int bias_f32, bias_vec, res_f32, res_vec;
+  int bias_f32, res_f32;
   char* z0;                 // pre-activations (gate products), up products
   char* z1;
   uint8_t* s0;              // their block exponents, where they are held as e4m3
@@ -129,16 +131,13 @@ struct End {
   int64_t ldo;
   int64_t ldo1;
   int out_f32;
-  int out_vec;
   int act;
   int n_store;
   const char* bias;
   const char* res;
   int64_t ldr;
   int bias_f32;
-  int bias_vec;
   int res_f32;
-  int res_vec;
   char* z0;
   char* z1;
   uint8_t* s0;
@@ -155,16 +154,16 @@ __device__ __forceinline__ End end_of() {
   End e = {};
 #define TM_TAKE(field) e.field = g->field
   if constexpr (kMode == kLinear) {
-    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(ldo); TM_TAKE(out_f32); TM_TAKE(out_vec); TM_TAKE(act);
-    TM_TAKE(bias); TM_TAKE(res); TM_TAKE(ldr); TM_TAKE(bias_f32); TM_TAKE(bias_vec); TM_TAKE(res_f32);
-    TM_TAKE(res_vec); TM_TAKE(z0); TM_TAKE(s0); TM_TAKE(ldz); TM_TAKE(held); TM_TAKE(blocks);
+    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(ldo); TM_TAKE(out_f32); TM_TAKE(act);
+    TM_TAKE(bias); TM_TAKE(res); TM_TAKE(ldr); TM_TAKE(bias_f32); TM_TAKE(res_f32);
+    TM_TAKE(z0); TM_TAKE(s0); TM_TAKE(ldz); TM_TAKE(held); TM_TAKE(blocks);
   }
   if constexpr (kMode == kResidual) {
-    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(ldo); TM_TAKE(out_f32); TM_TAKE(out_vec); TM_TAKE(res);
-    TM_TAKE(ldr); TM_TAKE(res_f32); TM_TAKE(res_vec);
+    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(ldo); TM_TAKE(out_f32); TM_TAKE(res);
+    TM_TAKE(ldr); TM_TAKE(res_f32);
   }
   if constexpr (kMode == kPlain) {
-    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(o1); TM_TAKE(ldo); TM_TAKE(out_f32); TM_TAKE(out_vec);
+    TM_TAKE(m); TM_TAKE(n); TM_TAKE(o0); TM_TAKE(o1); TM_TAKE(ldo); TM_TAKE(out_f32);
   }
   if constexpr (kMode == kGate) {
     TM_TAKE(m); TM_TAKE(n); TM_TAKE(n_store); TM_TAKE(o0); TM_TAKE(ldo); TM_TAKE(z0); TM_TAKE(z1);
@@ -177,16 +176,16 @@ __device__ __forceinline__ End end_of() {
 #undef TM_TAKE
 #define TM_KEEP(field) asm volatile("" : "+s"(e.field))
   if constexpr (kMode == kLinear) {
-    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(ldo); TM_KEEP(out_f32); TM_KEEP(out_vec); TM_KEEP(act);
-    TM_KEEP(bias); TM_KEEP(res); TM_KEEP(ldr); TM_KEEP(bias_f32); TM_KEEP(bias_vec); TM_KEEP(res_f32);
-    TM_KEEP(res_vec); TM_KEEP(z0); TM_KEEP(s0); TM_KEEP(ldz); TM_KEEP(held); TM_KEEP(blocks);
+    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(ldo); TM_KEEP(out_f32); TM_KEEP(act);
+    TM_KEEP(bias); TM_KEEP(res); TM_KEEP(ldr); TM_KEEP(bias_f32); TM_KEEP(res_f32);
+    TM_KEEP(z0); TM_KEEP(s0); TM_KEEP(ldz); TM_KEEP(held); TM_KEEP(blocks);
   }
   if constexpr (kMode == kResidual) {
-    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(ldo); TM_KEEP(out_f32); TM_KEEP(out_vec); TM_KEEP(res);
-    TM_KEEP(ldr); TM_KEEP(res_f32); TM_KEEP(res_vec);
+    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(ldo); TM_KEEP(out_f32); TM_KEEP(res);
+    TM_KEEP(ldr); TM_KEEP(res_f32);
   }
   if constexpr (kMode == kPlain) {
-    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(o1); TM_KEEP(ldo); TM_KEEP(out_f32); TM_KEEP(out_vec);
+    TM_KEEP(m); TM_KEEP(n); TM_KEEP(o0); TM_KEEP(o1); TM_KEEP(ldo); TM_KEEP(out_f32);
   }
   if constexpr (kMode == kGate) {
     TM_KEEP(m); TM_KEEP(n); TM_KEEP(n_store); TM_KEEP(o0); TM_KEEP(ldo); TM_KEEP(z0); TM_KEEP(z1);
@@ -213,14 +212,12 @@ struct Block {
 // in each matrix (rows 16 on: 16 rows more).
 struct Lane {
   uint32_t w[2], r[2];
-  uint32_t strip;
   uint32_t out, out1, res, z;
 };
 
 template <int kMode>
 __device__ __forceinline__ Lane lane_of(const End& g, uint32_t stg, int lane) {
   Lane l;
-  l.strip = stg;
   const uint32_t row = lane & 15, r = lane >> 2, sr = (r >> 1) & 7, c = 2 * (lane & 3), col = 8 * (lane & 3);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -285,16 +282,18 @@ __device__ __forceinline__ __attribute__((address_space(1))) T* mem(const void* 
   return (__attribute__((address_space(1))) T*)reinterpret_cast<uintptr_t>(p);
 }
 
-// 16-byte aligned. No branch: where two ways of loading meet, the loads are waited for, early or not.
+// Rows may start at any element: an access of 16 bytes need not be aligned to them. (1237 x 777 -> 1001 with a residual,
+// whose rows are odd: 15.4 us so, 21.5 us with an access an element.) No branch: where two ways of loading meet, the loads are
+// waited for, early or not.
 __device__ __forceinline__ Raw8 raw8(const char* p, bool f32) {
-  return {{*mem<u32x4>(p), *mem<u32x4>(p + (f32 ? 16 : 0))}};
+  return {{*mem<u32x4_at2>(p), *mem<u32x4_at2>(p + (f32 ? 16 : 0))}};
 }
 
-__device__ __forceinline__ Raw8 raw8(const char* p, bool f32, int left, bool vec) {  // `left` of them exist
-  if (vec && left >= 8) return raw8(p, f32);
+__device__ __forceinline__ Raw8 raw8(const char* p, bool f32, int left) {  // `left` of them exist
+  if (left >= 8) return raw8(p, f32);
   uint32_t w[8] = {};
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
+  for (int e = 0; e < 7; ++e)
     if (e < left) {
       if (f32) w[e] = mem<uint32_t>(p)[e];
       else w[e / 2] |= static_cast<uint32_t>(mem<uint16_t>(p)[e]) << (16 * (e & 1));
@@ -316,44 +315,26 @@ __device__ __forceinline__ void values8(float* x, const Raw8& r, bool f32) {
   }
 }
 
-__device__ __forceinline__ void put8(char* p, const float* x, bool f32) {  // 16-byte aligned
+__device__ __forceinline__ void put8(char* p, const float* x, bool f32) {
   if (f32) {
-    mem<f32x4>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
-    mem<f32x4>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      mem<u32x4_at4>(p)[h] = u32x4{__float_as_uint(x[4 * h]), __float_as_uint(x[4 * h + 1]), __float_as_uint(x[4 * h + 2]),
+                                   __float_as_uint(x[4 * h + 3])};
   } else {
-    *mem<u32x4>(p) =
+    *mem<u32x4_at2>(p) =
         u32x4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
   }
 }
 
-// Rows that do not start on 16 bytes, or end within a lane's 8 columns: half a block (16 rows) through the
-// strip, so that a lane has one column of row pairs and an access two whole rows of 32 columns.
-__device__ __forceinline__ uint32_t column_at(const Lane& l, int row, int lane) {
-  return l.strip + row * 128 + ((((lane & 31) >> 2) ^ (row >> 1)) << 4) + (lane & 3) * 4;
-}
-
-__device__ __forceinline__ void put_columns(const Lane& l, char* p, uint32_t ld, const float* x, bool f32, int rows,
-                                            int cols, int lane) {
-  asm volatile("ds_write_b128 %0, %2\n\tds_write_b128 %1, %3" ::"v"(l.r[0]), "v"(l.r[1]),
-               "v"(f32x4{x[0], x[1], x[2], x[3]}), "v"(f32x4{x[4], x[5], x[6], x[7]})
-               : "memory");
-  const int c = lane & 31;
-#pragma unroll 1
-  for (int r0 = lane >> 5; r0 < 16; r0 += 4) {
-    float v[2];
-    asm volatile("ds_read_b32 %0, %2\n\tds_read_b32 %1, %3\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(v[0]), "=&v"(v[1])
-                 : "v"(column_at(l, r0, lane)), "v"(column_at(l, r0 + 2, lane))
-                 : "memory");
+__device__ __forceinline__ void put8(char* p, const float* x, bool f32, int left) {
+  if (left >= 8) return put8(p, x, f32);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = r0 + 2 * i;
-      if (r >= rows || c >= cols) continue;
-      const uint32_t at = static_cast<uint32_t>(r) * ld + c;
-      if (f32) *mem<float>(p + at * 4u) = v[i];
-      else *mem<uint16_t>(p + at * 2u) = static_cast<uint16_t>(pack_bf16(v[i], 0.0f));
+  for (int e = 0; e < 7; ++e)
+    if (e < left) {
+      if (f32) mem<float>(p)[e] = x[e];
+      else mem<uint16_t>(p)[e] = static_cast<uint16_t>(pack_bf16(x[e], 0.0f));
     }
-  }
 }
 
 // Where a block is, and which of a lane's values exist (kWhole: all).
@@ -431,7 +412,7 @@ __device__ __forceinline__ Early early_of(const End& g, const Lane& l, int m0, i
       const char* p = at_block(g.res, g.ldr, size, s, i);
       if (kWhole) r.a[i] = raw8(p + l.res, g.res_f32);
       else if (s.row[i] && s.cols > 0)
-        r.a[i] = raw8(p + (static_cast<int64_t>(lane >> 2) * g.ldr + 8 * (lane & 3)) * size, g.res_f32, s.cols, g.res_vec);
+        r.a[i] = raw8(p + l.res, g.res_f32, s.cols);
     }
   }
   if constexpr (kMode == kGateGrad) {
@@ -491,7 +472,7 @@ __device__ __forceinline__ void end_linear(const End& g, const Lane& l, Block& b
   else if (act == tm_act::kGelu) each([](float z) { return tm_act::act1(tm_act::kGelu, z); });
   else if (act == tm_act::kGeluTanh) each([](float z) { return tm_act::act1(tm_act::kGeluTanh, z); });
   if (g.res) {  // read here, not early: the registers are the activation's
-    if (kWhole && g.res_vec) add_residual<true>(g, b, early_of<kLinear, true>(g, l, s.m0, s.n0, lane));
+    if (kWhole) add_residual<true>(g, b, early_of<kLinear, true>(g, l, s.m0, s.n0, lane));
     else add_residual<false>(g, b, early_of<kLinear, false>(g, l, s.m0, s.n0, lane));
   }
 }
@@ -504,7 +485,7 @@ __device__ __forceinline__ void store_block(const End& g, const Lane& l, char* o
   for (int i = 0; i < 2; ++i) {
     char* p = at_block(out, g.ldo, size, s, i);
     if (kWhole) put8(p + l.out, b.v + 8 * i, g.out_f32);
-    else put_columns(l, p, static_cast<uint32_t>(g.ldo), b.v + 8 * i, g.out_f32, g.m - s.m0 - 16 * i, g.n - s.n0, lane);
+    else if (s.row[i] && s.cols > 0) put8(p + l.out, b.v + 8 * i, g.out_f32, s.cols);
   }
 }
 
@@ -594,9 +575,7 @@ __device__ __forceinline__ void finish(f32x4 (&acc)[2 * kRowBlocks][2 * kColBloc
   const Lane l = lane_of<kMode>(g, stg, lane);
   constexpr int kPer = kMode == kGate ? 2 : 1, kCols = kColBlocks / kPer, kBlocks = kRowBlocks * kCols;
   constexpr bool kReads = kMode == kResidual || kMode == kGateGrad;
-  bool whole = m0 + 32 * kRowBlocks <= g.m && n0 + 32 * kCols <= g.n;
-  if (kMode <= kPlain) whole = whole && g.out_vec;
-  if (kMode == kResidual) whole = whole && g.res_vec;
+  const bool whole = m0 + 32 * kRowBlocks <= g.m && n0 + 32 * kCols <= g.n;
   auto pick = [&](Block& x, Block& y, int c) {
     const int jj = 2 * (c % kRowBlocks), ii = 2 * kPer * (c / kRowBlocks);
     const f32x4 t[2][2] = {{acc[jj][ii], acc[jj][ii + 1]}, {acc[jj + 1][ii], acc[jj + 1][ii + 1]}};
@@ -629,7 +608,7 @@ __device__ __forceinline__ void finish(f32x4 (&acc)[2 * kRowBlocks][2 * kColBloc
     if constexpr (kMode == kLinear)
       if (g.bias && b % kRowBlocks == 0)
         bias = raw8(g.bias + (static_cast<int64_t>(n) + 8 * (lane & 3)) * (g.bias_f32 ? 4 : 2), g.bias_f32,
-                    g.n - n - 8 * (lane & 3), g.bias_vec);
+                    g.n - n - 8 * (lane & 3));
     Early early = {};
     if constexpr (kReads) early = early_of<kMode, false>(g, l, m, n, lane);
     Block x, y;
@@ -1484,21 +1463,21 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
       return lin_fail(TM_EINVAL, "tm_lin: the gate's outputs are bf16, 16-byte aligned, rows %lld and %lld elements apart "
                       "a multiple of 8 that holds %lld columns each", (long long)d->ldo, (long long)d->ldo1,
                       (long long)pad);
-  } else if (d->ldo < cols || (g.out_f32 && (!aligned(d->o0, 4) || !aligned(d->o1, 4)))) {
+  } else if (d->ldo < cols) {
     return lin_fail(TM_EINVAL, "tm_lin: output rows %lld elements apart for %lld columns", (long long)d->ldo,
                     (long long)cols);
   }
+  if (!aligned(d->o0, g.out_f32 ? 4 : 2) || !aligned(d->o1, g.out_f32 ? 4 : 2) || !aligned(d->res, d->res_f32 ? 4 : 2) ||
+      !aligned(d->bias, d->bias_f32 ? 4 : 2))
+    return lin_fail(TM_EINVAL, "tm_lin: outputs, residual and bias must be aligned to their elements");
   if (d->ldo >= (1 << 24) || d->ldr >= (1 << 24) || (d->res && d->ldr < cols))  // a lane's offsets have 32 bits
     return lin_fail(TM_EINVAL, "tm_lin: output rows %lld and residual rows %lld elements apart, less than 2^24, at least "
                     "%lld", (long long)d->ldo, (long long)d->ldr, (long long)cols);
-  g.out_vec = d->ldo % (g.out_f32 ? 4 : 8) == 0 && aligned(d->o0, 16) && aligned(d->o1, 16);
   g.bias = static_cast<const char*>(d->bias);
   g.bias_f32 = d->bias_f32 != 0;
-  g.bias_vec = aligned(d->bias, 16);
   g.res = static_cast<const char*>(d->res);
   g.res_f32 = d->res_f32 != 0;
   g.ldr = d->ldr;
-  g.res_vec = d->ldr % (g.res_f32 ? 4 : 8) == 0 && aligned(d->res, 16);
 
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (few_rows(op, d->rows, d->inp)) {
