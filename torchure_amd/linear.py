@@ -215,7 +215,7 @@ def fused_linear(
     types; what no gradient needs is neither kept nor computed. Differentiable once."""
     host = _native.lin_host()
     act, kind = _ACTS.get(activation), _HELD.get(checkpoint)
-    if act is None or kind is None or torch.is_autocast_enabled("cuda") or not host.lin_plain(
+    if act is None or kind is None or torch.is_autocast_enabled("cuda") or not x.is_cuda or not host.lin_plain(
             x, (weight,), bias, residual, weight.shape[0] if weight.dim() else 0,
             torch.cuda.current_device()) or weight.shape[1] != x.shape[-1]:
         who = "fused_linear"
@@ -286,7 +286,7 @@ def swiglu_mlp(
     kind = _HELD.get(checkpoint)
     shapes_fit = (w_gate.dim() == 2 and w_up.shape == w_gate.shape and w_down.dim() == 2 and x.dim() > 0
                   and w_down.shape[1] == w_gate.shape[0] and w_gate.shape[1] == x.shape[-1])
-    if kind is None or not shapes_fit or torch.is_autocast_enabled("cuda") or not host.lin_plain(
+    if kind is None or not shapes_fit or torch.is_autocast_enabled("cuda") or not x.is_cuda or not host.lin_plain(
             x, (w_gate, w_up, w_down), None, residual, w_down.shape[0], torch.cuda.current_device()):
         who = "swiglu_mlp"
         if not shapes_fit:
