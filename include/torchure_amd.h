@@ -467,7 +467,9 @@ int tm_ce_grad_w_ld_bf16(uint16_t* d_grad_w, const uint16_t* d_grad_logits, int6
  *                     [d0 | d1] as in TM_LIN_GRAD_X, o0 = d0^T b0 and o1 = d1^T b0.
  * held: TM_HELD_BF16, rows of the next multiple of 8 columns; TM_HELD_E4M3, rows of the next multiple of
  * 32, with exponents s0 and s1 (see tm_quantize_e4m3); padding columns zero.
- * d_ws holds tm_lin_workspace_bytes(op, rows, inp, out, two) bytes, two: b1 (TM_LIN_GRAD_X) or o1
+ * Limits: rows <= 2^30, inp and out <= 2^22, operand rows less than 2^23 and output and residual rows less than 2^24
+ * elements apart; TM_LIN_FORWARD's and the gradients' outputs, bias and residual need their elements' alignment
+ * only, the gate's outputs and what is held 16 bytes. d_ws holds tm_lin_workspace_bytes(op, rows, inp, out, two) bytes, two: b1 (TM_LIN_GRAD_X) or o1
  * (TM_LIN_GRAD_W) is given. Calls that share a workspace on one stream are ordered.
  */
 #define TM_LIN_FORWARD 0
