@@ -464,7 +464,8 @@ int tm_ce_grad_w_ld_bf16(uint16_t* d_grad_w, const uint16_t* d_grad_logits, int6
  *                     with zeros up to the next multiple of 64; o1 (bf16, optional, rows ldo1
  *                     apart, zeros likewise) = silu(g) u.
  *   TM_LIN_GRAD_W     o0 (out x inp) = a^T b0, a rows x out, b0 rows x inp. With o1: a's rows are
- *                     [d0 | d1] as in TM_LIN_GRAD_X, o0 = d0^T b0 and o1 = d1^T b0.
+ *                     [d0 | d1] as in TM_LIN_GRAD_X, o0 = d0^T b0 and o1 = d1^T b0, in rows of the
+ *                     same distance.
  * held: TM_HELD_BF16, rows of the next multiple of 8 columns; TM_HELD_E4M3, rows of the next multiple of
  * 32, with exponents s0 and s1 (see tm_quantize_e4m3); padding columns zero.
  * Limits: rows <= 2^30, inp and out <= 2^22, operand rows less than 2^23 and output and residual rows less than 2^24

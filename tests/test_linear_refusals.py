@@ -184,3 +184,30 @@ def test_activation_checks_without_gpu():
         args = list(good)
         args[at] = bad
         assert lib.tm_act_grad(*args) < 0, at
+
+
+@pytest.mark.parametrize("fields", [
+    dict(op=GRAD_W, o1=FAKE, lda=128, ldo=40, ldo1=48),  # two outputs, one distance
+    dict(op=GRAD_W, o1=FAKE, lda=128, ldo=40),
+    dict(op=GATE_GRAD, lda=48, ldo=128, held=1, z0=FAKE, z1=FAKE, ldz=40, o1=FAKE, ldo1=1 << 24),
+])
+def test_second_output_rows_without_gpu(fields):
+    rc, text = lin(**fields)
+    assert rc < 0 and b"2^24" in text, text
+
+
+def test_launches_of_2_to_the_32_work_items_without_gpu():
+    lib = _native.lib()
+    rows = 1 << 30  # of one column: 2^25 bands of 32 rows
+    assert lib.tm_quantize_e4m3(FAKE, FAKE, 32, FAKE, 0, 1, rows, 1, None, 0, None) < 0
+    assert b"too large" in lib.tm_last_error()
+    assert lib.tm_dequantize_e4m3(FAKE, 0, 1, FAKE, FAKE, 32, rows, 1, None) < 0
+    need = lib.tm_act_grad_workspace_bytes(1, 1 << 30)
+    assert lib.tm_act_grad(None, 0, FAKE, 0, FAKE, 0, 1 << 30, None, None, 0, 0, 0, 1, 1 << 30, FAKE, need, None) < 0
+    assert lib.tm_act_grad(FAKE, 8, None, 0, FAKE, 0, 1, None, None, 0, 0, 0, rows, 1, None, 0, None) < 0
+
+
+def test_a_quantized_activation_without_dimensions(no_device):
+    one = torch.zeros(1, 32, dtype=torch.uint8)
+    with pytest.raises(RuntimeError, match="not those"):
+        ta.dequantize_activation(ta.QuantizedActivation(one, one[:, :1], torch.Size(()), BF16))

@@ -1475,9 +1475,11 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
   if (!aligned(d->o0, g.out_f32 ? 4 : 2) || !aligned(d->o1, g.out_f32 ? 4 : 2) || !aligned(d->res, d->res_f32 ? 4 : 2) ||
       !aligned(d->bias, d->bias_f32 ? 4 : 2))
     return lin_fail(TM_EINVAL, "tm_lin: outputs, residual and bias must be aligned to their elements");
-  if (d->ldo >= (1 << 24) || d->ldr >= (1 << 24) || (d->res && d->ldr < cols))  // a lane's offsets have 32 bits
-    return lin_fail(TM_EINVAL, "tm_lin: output rows %lld and residual rows %lld elements apart, less than 2^24, at least "
-                    "%lld", (long long)d->ldo, (long long)d->ldr, (long long)cols);
+  if (d->ldo >= (1 << 24) || d->ldo1 >= (1 << 24) || d->ldr >= (1 << 24) || (d->res && d->ldr < cols) ||
+      (two_out && d->ldo1 != d->ldo))  // a lane's offsets have 32 bits
+    return lin_fail(TM_EINVAL, "tm_lin: output rows %lld, %lld (the same where a gradient has two outputs) and residual "
+                    "rows %lld elements apart, less than 2^24, at least %lld", (long long)d->ldo, (long long)d->ldo1,
+                    (long long)d->ldr, (long long)cols);
   g.bias = static_cast<const char*>(d->bias);
   g.bias_f32 = d->bias_f32 != 0;
   g.res = static_cast<const char*>(d->res);

@@ -95,8 +95,8 @@ def dequantize_activation(q: QuantizedActivation, dtype: torch.dtype | None = No
         raise NotImplementedError(f"{who}: dtype must be bfloat16 or float32, got {dtype}")
     v, e = q.values, q.exponents
     _on_gpu(v, who, "values")
-    rows, cols = q.shape[:-1].numel(), q.shape[-1]
-    if (v.dtype != torch.uint8 or e.dtype != torch.uint8 or e.device != v.device
+    rows, cols = (q.shape[:-1].numel(), q.shape[-1]) if len(q.shape) else (0, 0)
+    if (not len(q.shape) or v.dtype != torch.uint8 or e.dtype != torch.uint8 or e.device != v.device
             or v.shape != (rows, _up(cols, 32)) or e.shape != (-(-rows // 32), -(-cols // 32))
             or not v.is_contiguous() or not e.is_contiguous() or v.data_ptr() % 16):
         raise RuntimeError(f"{who}: values {tuple(v.shape)} and exponents {tuple(e.shape)} are not those of a tensor of "
