@@ -82,6 +82,30 @@ def test_mlp_sizes(rows, dim, ffn, out, res):
         same(grads[k], twice[k], "two runs: " + k)
 
 
+@pytest.mark.parametrize("rows", [1, 7, 16, 17, 32, 33, 64])
+@pytest.mark.parametrize("inp,out,act,bias,res", [
+    (64, 16, None, None, None), (72, 33, "silu", torch.bfloat16, torch.float32), (1000, 9, "gelu", torch.float32, None),
+    (2816, 1024, None, None, torch.bfloat16), (4864, 47, "relu", None, torch.float32), (136, 8200, "gelu_tanh", None, None),
+    (9, 15, None, torch.bfloat16, torch.bfloat16)])
+def test_few_rows_without_gradients(rows, inp, out, act, bias, res):
+    """The forms for single tokens and short ends: every width of a workgroup's columns, to the last and past it."""
+    t, dy = T.linear_case(rows, inp, out, act, bias, res, None, seed=rows + out)
+    want = T.linear_want(t, dy, act, None)["y"]
+    with torch.no_grad():
+        d = {k: None if v is None else v.to(DEV) for k, v in t.items()}
+        T.close(ta.fused_linear(d["x"], d["weight"], d["bias"], d["residual"], act), *want, "y")
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 33, 64])
+@pytest.mark.parametrize("dim,ffn,out", [(64, 16, 40), (72, 47, 33), (1024, 2816, 1024), (2560, 520, 96), (24, 8200, 24)])
+def test_few_rows_of_the_feed_forward_without_gradients(rows, dim, ffn, out):
+    t, dy = T.mlp_case(rows, dim, ffn, out, torch.bfloat16, seed=rows + ffn)
+    want = T.mlp_want(t, dy, None)["y"]
+    with torch.no_grad():
+        y = ta.swiglu_mlp(*(t[k].to(DEV) for k in ("x", "w_gate", "w_up", "w_down", "residual")))
+    T.close(y, *want, "y")
+
+
 @pytest.mark.parametrize("rows,inp,out", [(2304, 512, 2304), (3001, 333, 1237)])
 def test_8_bit_gradients_are_those_of_what_is_held(rows, inp, out):
     """With no activation the weight's gradient reads x as held: the same bits as a call on the held x."""

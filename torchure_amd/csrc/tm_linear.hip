@@ -572,10 +572,15 @@ __device__ __forceinline__ void end_block(const End& g, const Lane& l, int batch
 // matrix, one after the other in straight code (but for kLinear, whose code is long); else in a loop whose
 // first step picks the block's registers. No register may spill here: a spill's reload waits for all
 // stores before it.
-template <int kMode, bool kHalves, int kRowBlocks, int kColBlocks>
+// kNarrow: of the one block's columns the first 16.
+template <int kMode, bool kHalves, int kRowBlocks, int kColBlocks, bool kNarrow = false>
 __device__ __forceinline__ void finish(f32x4 (&acc)[2 * kRowBlocks][2 * kColBlocks], int batch, int m0, int n0, int lane,
                                        uint32_t stg) {
-  const End g = end_of<kMode>();
+  End g = end_of<kMode>();
+  if (kNarrow) {
+    g.n = min(g.n, n0 + 16);
+    if (kMode == kGate) g.n_store = min(g.n_store, n0 + 16);
+  }
   asm volatile("" : "+v"(lane));  // what derives from it is made again for each tile: kept, it spills
   const Lane l = lane_of<kMode>(g, stg, lane);
   constexpr int kPer = kMode == kGate ? 2 : 1, kCols = kColBlocks / kPer, kBlocks = kRowBlocks * kCols;
@@ -1062,28 +1067,33 @@ __global__ __launch_bounds__(256) void lin_finish_kernel(const Args g) {
 //
 // The forward products of up to 16 kMT rows (a token, a short sequence's end): bound by the weight's bytes, or,
 // where those are few, by the latency of one launch. A workgroup takes 32 output columns (with a gate 32 of
-// each weight); its waves take 64 K each in turn and keep the whole result, which they add up in LDS
-// in order. An operand's 64 K of a row are 128 bytes of four lanes, 32 each: the two MFMAs of a step take
-// the lanes' first and second 16 bytes, the same K of both operands. Nothing is loaded twice, so nothing
-// goes through LDS on the way in. The end is the tiles'.
-template <int kMT, int kMode>
+// each weight), kNarrow 16, which puts twice as many CUs to work; its waves take 64 K each in turn and keep
+// the whole result, which they add up in LDS in order. An operand's 64 K of a row are 128 bytes of four
+// lanes, 32 each: the two MFMAs of a step take the lanes' first and second 16 bytes, the same K of both
+// operands. Nothing is loaded twice, so nothing goes through LDS on the way in. The end is the tiles'.
+// (Microseconds with 16 columns / 32: 1 x 1024 -> 2816 3.9 / 5.1, 1 x 2816 -> 1024 6.1 / 8.7, 1 x 9728 -> 2560
+// 14.2 / 22.8, the gate of 1 x 2560 -> 9728 20.4 / 28.4, 4.9 TB/s.)
+template <int kMT, int kMode, bool kNarrow = false>
 struct Few {
-  static constexpr int kWaves = kMT == 4 || kMode == kLinear ? 8 : 16;  // kLinear's end takes over 128 registers
-  static constexpr int lds(int nt) { return kWaves * kMT * nt * 1024 + 8192; }
+  // few registers a wave in 16 waves: kLinear's end takes over 128, kNarrow loads more steps at a time
+  static constexpr int kWaves = kNarrow || kMT == 4 || kMode == kLinear ? 8 : 16;
+  static constexpr int kCols = kNarrow ? 16 : 32;
+  static constexpr int kLds = kWaves * kMT * (kCols / 16 * (kMode == kGate ? 2 : 1)) * 1024 + 8192;
 };
 
-template <int kMT, int kMode>
-__global__ __launch_bounds__((Few<kMT, kMode>::kWaves * 64)) void lin_rows_kernel(const Args g) {
+template <int kMT, int kMode, bool kNarrow>
+__global__ __launch_bounds__((Few<kMT, kMode, kNarrow>::kWaves * 64)) void lin_rows_kernel(const Args g) {
+  using F = Few<kMT, kMode, kNarrow>;
   constexpr bool kPairs = kMode == kGate;
-  constexpr int kNT = kPairs ? 4 : 2, kWaves = Few<kMT, kMode>::kWaves, kSums = (kMT + 1) / 2;
+  constexpr int kFrags = F::kCols / 16, kNT = kPairs ? 2 * kFrags : kFrags, kWaves = F::kWaves, kSums = (kMT + 1) / 2;
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int n0 = static_cast<int>(blockIdx.x) * 32, r = lane & 15, c = lane >> 4;
+  const int n0 = static_cast<int>(blockIdx.x) * F::kCols, r = lane & 15, c = lane >> 4;
   const char *pw[kNT], *px[kMT];
 #pragma unroll
   for (int t = 0; t < kNT; ++t)
-    pw[t] = (t >= 2 ? g.b1 : g.b0) + min(n0 + 16 * (t & 1) + r, g.n - 1) * g.b_ld + c * 32;
+    pw[t] = (t >= kFrags ? g.b1 : g.b0) + min(n0 + 16 * (t % kFrags) + r, g.n - 1) * g.b_ld + c * 32;
 #pragma unroll
   for (int t = 0; t < kMT; ++t) px[t] = g.a + min(16 * t + r, g.m - 1) * g.a_ld + c * 32;
   f32x4 acc[kMT][kNT];
@@ -1092,7 +1102,8 @@ __global__ __launch_bounds__((Few<kMT, kMode>::kWaves * 64)) void lin_rows_kerne
 #pragma unroll
     for (int j = 0; j < kNT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   // several steps' loads at a time in flight
-  constexpr int kBatch = kMT == 4 ? 1 : (kMT == 2 ? 2 : 4) / (kPairs ? 2 : 1), kStep = kWaves * kSliceK;
+  constexpr int kWide = kMT == 4 ? 1 : (kMT == 2 ? 2 : 4) / (kPairs ? 2 : 1);
+  constexpr int kBatch = !kNarrow ? kWide : kMT == 4 ? 2 : kMT == 2 ? (kPairs ? 2 : 4) : (kPairs ? 4 : 6), kStep = kWaves * kSliceK;
   for (int k0 = wave * kSliceK; k0 < g.ka; k0 += kBatch * kStep) {
     bf16x8 w[kBatch][kNT][2], x[kBatch][kMT][2];
 #pragma unroll
@@ -1133,19 +1144,19 @@ __global__ __launch_bounds__((Few<kMT, kMode>::kWaves * 64)) void lin_rows_kerne
     for (int j = 0; j < kNT; ++j) part[((wave * kMT + i) * kNT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
   if (wave >= kSums) return;
-  f32x4 sum[2][kNT];
+  f32x4 sum[2][kPairs ? 4 : 2] = {};
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
-      sum[h][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (2 * wave + h >= kMT) continue;
+      f32x4& to = sum[h][j / kFrags * 2 + j % kFrags];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) sum[h][j] += part[((w * kMT + 2 * wave + h) * kNT + j) * 64 + lane];
+      for (int w = 0; w < kWaves; ++w) to += part[((w * kMT + 2 * wave + h) * kNT + j) * 64 + lane];
     }
-  finish<kMode, false, 1, kNT / 2>(sum, 0, wave * 32, n0, lane,
-                                   static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) +
-                                       kWaves * kMT * kNT * 1024 + wave * 4096);
+  finish<kMode, false, 1, kPairs ? 2 : 1, kNarrow>(sum, 0, wave * 32, n0, lane,
+                                                   static_cast<uint32_t>(reinterpret_cast<uintptr_t>(smem)) +
+                                                       kWaves * kMT * kNT * 1024 + wave * 4096);
 }
 
 // ------------------------------------------------------------------------------ the host's side
@@ -1248,14 +1259,17 @@ Product product_of(int op, int64_t rows, int64_t inp, int64_t out, bool two) {
   }
 }
 
-// What lin_rows_kernel takes: up to 16 rows, and up to 64 of short K. (Microseconds against 128 x 128 tiles:
-// 1 x 1024 -> 2816 5.1 / 12.6, 1 x 2816 -> 1024 8.7 / 14.7, 64 x 1024 -> 2816 9.0 / 12.7, but 64 x 2816 -> 1024
-// 18.3 / 14.7 and 64 x 9728 -> 2560 53 / 22.)
-bool few_rows(int op, int64_t rows, int64_t inp) {
-  return op <= TM_LIN_GATE && (rows <= 16 || (rows <= 64 && inp <= 1536));
+// What lin_rows_kernel takes: up to 16 rows, and up to 64 of short K; of somewhat longer K where nothing is held and
+// 32 columns to a workgroup do not fill the CUs. (Microseconds against 128 x 128 tiles: 64 x 1024 -> 2816 7.8 / 12.7,
+// 32 x 2816 -> 1024 10.6 / 15.0, 64 x 2560 -> 2560 14.4 / 16.6, but 64 x 2816 -> 1024 16.0 / 15.1, 32 x 9728 -> 2560
+// 29.9 / 23.3, 32 x 2560 -> 9728 24.3 / 20.4.)
+constexpr int64_t kNarrowCols = 8192, kFewElements = 64 * 2560;
+bool few_rows(int op, int64_t rows, int64_t inp, int64_t out, bool held) {
+  if (op > TM_LIN_GATE || rows > 64) return false;
+  return rows <= 16 || inp <= 1536 || (!held && out <= kNarrowCols && rows * inp <= kFewElements);
 }
 
-constexpr int kMaxDevices = 64, kKernels = 54;
+constexpr int kMaxDevices = 64, kKernels = 66;
 std::mutex g_mu;
 bool g_lds_set[kKernels][kMaxDevices] = {};
 int g_cus[kMaxDevices] = {};
@@ -1319,22 +1333,30 @@ int launch(int which, Args& g, hipStream_t s) {
   return launch_one<kMB, kNB, kAK, kBK, true, kMode>(2 * which + 1, g, s);
 }
 
-template <int kMT, int kMode>
+template <int kMT, int kMode, bool kNarrow = false>
 int launch_rows(int which, Args& g, hipStream_t s) {
-  constexpr int kLds = Few<kMT, kMode>::lds(kMode == kGate ? 4 : 2);
+  using F = Few<kMT, kMode, kNarrow>;
   int cus = 0;
-  hipError_t e = allow_lds(s, which, reinterpret_cast<const void*>(lin_rows_kernel<kMT, kMode>), kLds, &cus);
+  hipError_t e = allow_lds(s, which, reinterpret_cast<const void*>(lin_rows_kernel<kMT, kMode, kNarrow>), F::kLds, &cus);
   if (e != hipSuccess) return lin_fail(TM_ELAUNCH, "tm_lin: LDS attribute: %s", hipGetErrorString(e));
   const int cols = kMode == kGate ? g.n_store : g.n;
-  hipLaunchKernelGGL((lin_rows_kernel<kMT, kMode>), dim3(static_cast<uint32_t>(ceil_div(cols, 32))),
-                     dim3(Few<kMT, kMode>::kWaves * 64), kLds, s, g);
+  hipLaunchKernelGGL((lin_rows_kernel<kMT, kMode, kNarrow>), dim3(static_cast<uint32_t>(ceil_div(cols, F::kCols))),
+                     dim3(F::kWaves * 64), F::kLds, s, g);
   e = hipGetLastError();
   return e == hipSuccess ? TM_OK : lin_fail(TM_ELAUNCH, "lin_rows_kernel: launch failed: %s", hipGetErrorString(e));
 }
 
 template <int kMode>
 int launch_few(int which, Args& g, hipStream_t s) {
-  if (g.m <= 16) return launch_rows<1, kMode>(which, g, s);
+  // 16 columns to a workgroup: not of what is held, whose blocks are 32 x 32, nor where 32 fill the CUs and x
+  // is read by each (64 x 1024 -> 9728 16.9 us, 14.6 with 32)
+  if (!g.held && (g.m <= 16 || g.n <= kNarrowCols)) {
+    if (g.m <= 16) return launch_rows<1, kMode, true>(which + 3, g, s);
+    if (g.m <= 32) return launch_rows<2, kMode, true>(which + 4, g, s);
+    return launch_rows<4, kMode, true>(which + 5, g, s);
+  }
+  if constexpr (kMode == kLinear || kMode == kGate)  // what is held
+    if (g.m <= 16) return launch_rows<1, kMode>(which, g, s);
   if (g.m <= 32) return launch_rows<2, kMode>(which + 1, g, s);
   return launch_rows<4, kMode>(which + 2, g, s);
 }
@@ -1352,7 +1374,7 @@ extern "C" {
 
 size_t tm_lin_workspace_bytes(int op, int64_t rows, int64_t inp, int64_t out, int two) {
   if (op < TM_LIN_FORWARD || op > TM_LIN_GRAD_W || rows <= 0 || inp <= 0 || out <= 0) return 0;
-  if (few_rows(op, rows, inp)) return 0;
+  if (few_rows(op, rows, inp, out, true)) return 0;  // then also where nothing is held
   const Product q = product_of(op, rows, inp, out, two != 0);
   return partial_bytes(q, best_plan(q));
 }
@@ -1373,7 +1395,8 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
                     "(%lld, %lld)", (long long)d->lda, (long long)d->ldb);
   const Product q = product_of(op, d->rows, d->inp, d->out, two || two_out);
   const Plan p = best_plan(q);
-  const size_t need = few_rows(op, d->rows, d->inp) ? 0 : partial_bytes(q, p);
+  const bool few = few_rows(op, d->rows, d->inp, d->out, d->held != TM_HELD_NOT);
+  const size_t need = few ? 0 : partial_bytes(q, p);
   if (need && (!d_ws || ws_bytes < need || !aligned(d_ws, 16)))
     return lin_fail(TM_EINVAL, "tm_lin: workspace of %zu bytes, %zu needed, 16-byte aligned", ws_bytes, need);
   auto up8 = [](int64_t v) { return (v + 7) / 8 * 8; };
@@ -1487,10 +1510,10 @@ int tm_lin(const tm_lin_t* d, void* d_ws, size_t ws_bytes, void* stream) {
   g.ldr = d->ldr;
 
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (few_rows(op, d->rows, d->inp)) {
-    if (op == TM_LIN_GATE) return launch_few<kGate>(kKernels - 12, g, s);
-    if (g.bias || g.act || g.held) return launch_few<kLinear>(kKernels - 9, g, s);
-    return g.res ? launch_few<kResidual>(kKernels - 6, g, s) : launch_few<kPlain>(kKernels - 3, g, s);
+  if (few) {
+    if (op == TM_LIN_GATE) return launch_few<kGate>(kKernels - 24, g, s);
+    if (g.bias || g.act || g.held) return launch_few<kLinear>(kKernels - 18, g, s);
+    return g.res ? launch_few<kResidual>(kKernels - 12, g, s) : launch_few<kPlain>(kKernels - 6, g, s);
   }
   switch (op) {
     case TM_LIN_FORWARD:
