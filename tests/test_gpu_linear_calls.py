@@ -577,6 +577,104 @@ def test_nothing_behind_the_last_row_or_column_is_written():
         same(room, want, f"{rows} x {inp} -> {out}")
 
 
+@pytest.mark.parametrize("rows,inp,out,held", [(5, 64, 77, 0), (5, 64, 77, 1), (40, 72, 33, 2), (300, 72, 130, 1), (300, 64, 130, 0)])
+def test_the_gate_writes_its_rows_only(rows, inp, out, held):
+    import ctypes
+
+    from torchure_amd import _native
+    lib = _native.lib()
+    g = torch.Generator().manual_seed(23)
+    a, b0, b1 = (T.grid_values(g, s, 0.125, 6).to(DEV) for s in ((rows, inp), (out, inp), (out, inp)))
+    pad = -(-out // 8) * 8
+    room = torch.full((rows + 6, pad + 24), 7.0, dtype=BF16, device=DEV)
+    width = pad if held < 2 else -(-out // 32) * 32
+    kept = [torch.full((rows + 4, width), 7, dtype=torch.uint8 if held == 2 else BF16, device=DEV) for _ in range(2)]
+    exps = [torch.full((-(-rows // 32) * -(-out // 32) + 9,), 7, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    d = _native.TmLin(rows=rows, inp=inp, out=out, a=a.data_ptr(), b0=b0.data_ptr(), b1=b1.data_ptr(), o0=room[3:, 8:].data_ptr(),
+                      lda=inp, ldb=inp, ldo=pad + 24, op=1, held=held, z0=kept[0].data_ptr(), z1=kept[1].data_ptr(),
+                      s0=exps[0].data_ptr(), s1=exps[1].data_ptr(), ldz=width)
+    ws = torch.empty(max(1, lib.tm_lin_workspace_bytes(1, rows, inp, out, 0)), dtype=torch.uint8, device=DEV)
+    _native.check(lib.tm_lin(ctypes.byref(d), ws.data_ptr(), ws.numel(), _native.stream_handle(torch.device(DEV, 0))), "tm_lin")
+    inside = torch.zeros(room.shape, dtype=torch.bool, device=DEV)
+    inside[3: 3 + rows, 8: 8 + pad] = True
+    assert bool((room[~inside] == 7.0).all())
+    assert not room[3: 3 + rows, 8 + out: 8 + pad].any()  # the padding: zeros
+    gate, up = a.double() @ b0.double().t(), a.double() @ b1.double().t()
+    want = gate / (1 + torch.exp(-gate)) * up
+    bound = want.abs() * 2.0 ** -8 + up.abs() * gate.abs().clamp_min(1) * T.ACT_ERR
+    T.close(room[3: 3 + rows, 8: 8 + out], want.cpu(), bound.cpu(), "the gate's result")
+    n = exps[0].numel() - 9
+    for k, e in zip(kept, exps):
+        assert bool((k[rows:] == 7).all()) and bool((e[n:] == 7).all())
+        if held == 0:
+            assert bool((k == 7).all()) and bool((e == 7).all())
+        else:
+            assert not k[:rows, out:].any()
+
+
+def test_two_threads_on_two_streams():
+    import threading
+
+    t, dy = T.linear_case(700, 256, 520, "silu", BF16, F32, None, seed=24)
+    m, mdy = T.mlp_case(130, 128, 320, 128, BF16, seed=24)
+    sets = [(on_device(t), dy.to(DEV)), (on_device(m), mdy.to(DEV))]
+    want = [linear_grads(*sets[0], "silu", "e4m3"), mlp_grads(*sets[1], "e4m3")]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got[i] = linear_grads(*sets[0], "silu", "e4m3") if i == 0 else mlp_grads(*sets[1], "e4m3")
+        stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join(60)
+        assert not th.is_alive()
+    for (y, grads), (y2, grads2) in zip(want, got):
+        same(y, y2)
+        for k in grads:
+            same(grads[k], grads2[k], k)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_saved_elsewhere_and_recomputed(checkpoint):
+    """What is kept may be moved to the host between the passes, or made again."""
+    from torch.utils.checkpoint import checkpoint as again
+
+    t, dy = T.linear_case(70, 96, 77, "gelu", BF16, F32, None, seed=25)
+    d, dy = on_device(t), dy.to(DEV)
+    wide = torch.zeros(70, 200, dtype=BF16, device=DEV)
+    wide[:, 8:104] = d["x"].detach()
+    d["x"] = wide[:, 8:104].requires_grad_()  # strided rows
+    m, mdy = T.mlp_case(50, 40, 77, 60, BF16, seed=25)
+    m, mdy = on_device(m), mdy.to(DEV)
+    y, grads = linear_grads(d, dy, "gelu", checkpoint)
+    z, mgrads = mlp_grads(m, mdy, checkpoint)
+    with torch.autograd.graph.save_on_cpu():
+        y2, grads2 = linear_grads(d, dy, "gelu", checkpoint)
+        z2, mgrads2 = mlp_grads(m, mdy, checkpoint)
+    y3 = again(ta.fused_linear, d["x"], d["weight"], d["bias"], d["residual"], "gelu", checkpoint, use_reentrant=False)
+    grads3 = dict(zip(d, torch.autograd.grad(y3, list(d.values()), dy)))
+    z3 = again(ta.swiglu_mlp, *m.values(), checkpoint, use_reentrant=False)
+    mgrads3 = dict(zip(m, torch.autograd.grad(z3, list(m.values()), mdy)))
+    for a, b in ((y, y2), (z, z2), (y, y3), (z, z3)):
+        same(a, b)
+    for one, others in ((grads, (grads2, grads3)), (mgrads, (mgrads2, mgrads3))):
+        for k in one:
+            for o in others:
+                same(one[k], o[k], k)
+    # twice from what is kept
+    y = ta.fused_linear(d["x"], d["weight"], d["bias"], d["residual"], "gelu", checkpoint)
+    for _ in range(2):
+        for k, v in zip(d, torch.autograd.grad(y, list(d.values()), dy, retain_graph=True)):
+            same(grads[k], v, k)
+
+
 # ---------------------------------------------------------------------------- together
 
 
