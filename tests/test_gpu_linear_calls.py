@@ -137,6 +137,24 @@ def test_more_elements_than_32_bits():
     same(y[-300:], ta.fused_linear(tall[-300:].clone(), wide, activation="relu"))
 
 
+@pytest.mark.parametrize("rows,cols", [(10_000, 8192), (10_300, 8192), (81_000, 1037)])
+def test_large_8_bit_matrices(rows, cols):
+    """On both sides of the size from which bf16 matrices go past the caches, odd rows among them: as parts of
+    the rows are held by themselves."""
+    g = torch.Generator(device=DEV).manual_seed(26)
+    x = torch.randn(rows, cols, generator=g, device=DEV).to(BF16)
+    q = ta.quantize_activation(x)
+    back, wide = ta.dequantize_activation(q), ta.dequantize_activation(q, F32)
+    assert torch.equal(back.float(), wide)
+    for at in (0, 32 * (rows // 64), 32 * (rows // 32) - 64):
+        part = x[at: at + 96] if at + 96 > rows else x[at: at + 64]
+        p = ta.quantize_activation(part.contiguous())
+        n = part.shape[0]
+        assert torch.equal(q.values[at: at + n], p.values)
+        assert torch.equal(q.exponents[at // 32: at // 32 + p.exponents.shape[0]], p.exponents)
+        same(back[at: at + n], ta.dequantize_activation(p))
+
+
 # ---------------------------------------------------------------------------- layouts, types
 
 

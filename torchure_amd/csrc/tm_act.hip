@@ -39,7 +39,8 @@ struct Raw8 {
   u32x4 w[kF32 ? 2 : 1];
 };
 
-template <bool kF32>
+// kStream: past the caches (bf16 only; see kStreamBytes).
+template <bool kF32, bool kStream = false>
 __device__ __forceinline__ Raw8<kF32> get8(const void* base, int64_t at, int left) {
   Raw8<kF32> r = {};
   if constexpr (kF32) {
@@ -55,7 +56,8 @@ __device__ __forceinline__ Raw8<kF32> get8(const void* base, int64_t at, int lef
   } else {
     const uint16_t* p = static_cast<const uint16_t*>(base) + at;
     if (left >= 8) {
-      r.w[0] = *reinterpret_cast<const u32x4_at2*>(p);
+      const auto* at8 = reinterpret_cast<const u32x4_at2*>(p);
+      r.w[0] = kStream ? __builtin_nontemporal_load(at8) : *at8;
     } else {
 #pragma unroll
       for (int e = 0; e < 7; ++e)
@@ -74,7 +76,7 @@ __device__ __forceinline__ void values8(float (&x)[8], const Raw8<kF32>& r) {
   }
 }
 
-template <bool kF32>
+template <bool kF32, bool kStream = false>
 __device__ __forceinline__ void put8(void* base, int64_t at, const float (&x)[8], int left) {
   if constexpr (kF32) {
     float* p = static_cast<float*>(base) + at;
@@ -92,7 +94,10 @@ __device__ __forceinline__ void put8(void* base, int64_t at, const float (&x)[8]
     uint16_t* p = static_cast<uint16_t*>(base) + at;
     const uint32_t w[4] = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7])};
     if (left >= 8) {
-      *reinterpret_cast<u32x4_at2*>(p) = u32x4{w[0], w[1], w[2], w[3]};
+      auto* at8 = reinterpret_cast<u32x4_at2*>(p);
+      const u32x4_at2 v = u32x4{w[0], w[1], w[2], w[3]};
+      if constexpr (kStream) __builtin_nontemporal_store(v, at8);
+      else *at8 = v;
     } else {
 #pragma unroll
       for (int e = 0; e < 7; ++e)
@@ -103,7 +108,7 @@ __device__ __forceinline__ void put8(void* base, int64_t at, const float (&x)[8]
 
 // A wave takes 32 rows x 64 columns, two blocks side by side: lane l the columns 8 (l % 8) .. + 7 of rows
 // l / 8, + 8, + 16, + 24.
-template <bool kF32>
+template <bool kF32, bool kStream>
 __global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ values, uint8_t* __restrict__ exps,
                                                        int64_t ldv, const void* __restrict__ src, int64_t lds,
                                                        int64_t rows, int cols, int wide,
@@ -117,7 +122,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ val
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const bool in = m + 8 * i < rows;
-    values8<kF32>(x[i], get8<kF32>(src, in ? (m + 8 * i) * lds + n : 0, in ? cols - n : 0));
+    values8<kF32>(x[i], get8<kF32, kStream>(src, in ? (m + 8 * i) * lds + n : 0, in ? cols - n : 0));
   }
   // over the block's lanes: l, l ^ 1, l ^ 2, l ^ 8 in a row of 16, and the four rows
   auto over_block = [](uint32_t v) {
@@ -161,7 +166,7 @@ __global__ __launch_bounds__(256) void quantize_kernel(uint8_t* __restrict__ val
   }
 }
 
-template <bool kF32>
+template <bool kF32, bool kStream>
 __global__ __launch_bounds__(256) void dequantize_kernel(void* __restrict__ dst, int64_t ldd,
                                                          const uint8_t* __restrict__ values,
                                                          const uint8_t* __restrict__ exps, int64_t ldv, int64_t rows,
@@ -181,7 +186,7 @@ __global__ __launch_bounds__(256) void dequantize_kernel(void* __restrict__ dst,
     if (m + 8 * i >= rows) continue;
     const f32x4 a = tm_act::decode4(w[i].x, scale), b = tm_act::decode4(w[i].y, scale);
     const float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-    put8<kF32>(dst, (m + 8 * i) * ldd + n, x, cols - n);
+    put8<kF32, kStream>(dst, (m + 8 * i) * ldd + n, x, cols - n);
   }
 }
 
@@ -284,6 +289,11 @@ bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // A launch has less than 2^32 work-items, 256 a workgroup.
+// bf16 matrices of more bytes than this go past the caches, which then keep the 8-bit values: nobody finds all of such a
+// matrix there afterwards. (Into 8 bits and back, us past / through them: 320 MB 150 / 180, 192 MB 93 / 115, 128 MB 65 / 70,
+// but 96 MB 50 / 47, 64 MB 34 / 33; fp32, whose lanes have 32 bytes each, 202 / 173 at 320 MB.)
+constexpr int64_t kStreamBytes = int64_t(160) << 20;
+
 constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxCols = int64_t(1) << 30, kMaxGroups = (int64_t(1) << 24) - 1;
 
 int check_shape(const char* who, int64_t rows, int64_t cols, int64_t groups) {
@@ -316,12 +326,14 @@ int tm_quantize_e4m3(uint8_t* d_values, uint8_t* d_exponents, int64_t ldv, const
                     (long long)ldc, (long long)cols);
   const dim3 grid(static_cast<uint32_t>(groups));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (src_f32)
-    hipLaunchKernelGGL(quantize_kernel<true>, grid, dim3(256), 0, s, d_values, d_exponents, ldv, d_src, lds, rows,
-                       static_cast<int>(cols), static_cast<int>(wide), d_copy, ldc);
-  else
-    hipLaunchKernelGGL(quantize_kernel<false>, grid, dim3(256), 0, s, d_values, d_exponents, ldv, d_src, lds, rows,
-                       static_cast<int>(cols), static_cast<int>(wide), d_copy, ldc);
+  auto launch = [&](auto f32, auto stream8) {
+    hipLaunchKernelGGL((quantize_kernel<decltype(f32)::value != 0, decltype(stream8)::value != 0>), grid, dim3(256), 0, s,
+                       d_values, d_exponents, ldv, d_src, lds, rows, static_cast<int>(cols), static_cast<int>(wide),
+                       d_copy, ldc);
+  };
+  if (src_f32) launch(Int<1>{}, Int<0>{});
+  else if (rows * cols * 2 > kStreamBytes) launch(Int<0>{}, Int<1>{});
+  else launch(Int<0>{}, Int<0>{});
   return launched(who);
 }
 
@@ -337,12 +349,13 @@ int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_v
                     "aligned; output rows are %lld apart", who, (long long)ldv, (long long)cols, (long long)ldd);
   const dim3 grid(static_cast<uint32_t>(groups));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dst_f32)
-    hipLaunchKernelGGL(dequantize_kernel<true>, grid, dim3(256), 0, s, d_dst, ldd, d_values, d_exponents, ldv, rows,
-                       static_cast<int>(cols), static_cast<int>(wide));
-  else
-    hipLaunchKernelGGL(dequantize_kernel<false>, grid, dim3(256), 0, s, d_dst, ldd, d_values, d_exponents, ldv, rows,
-                       static_cast<int>(cols), static_cast<int>(wide));
+  auto launch = [&](auto f32, auto stream8) {
+    hipLaunchKernelGGL((dequantize_kernel<decltype(f32)::value != 0, decltype(stream8)::value != 0>), grid, dim3(256), 0, s,
+                       d_dst, ldd, d_values, d_exponents, ldv, rows, static_cast<int>(cols), static_cast<int>(wide));
+  };
+  if (dst_f32) launch(Int<1>{}, Int<0>{});
+  else if (rows * cols * 2 > kStreamBytes) launch(Int<0>{}, Int<1>{});
+  else launch(Int<0>{}, Int<0>{});
   return launched(who);
 }
 
