@@ -18,6 +18,7 @@ import contextlib
 import dataclasses
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from torchure_amd import _native
@@ -143,11 +144,15 @@ def _bf16_source(w: torch.Tensor) -> torch.Tensor:
     return w
 
 
-def _wants_grad(*tensors) -> bool:
+def _wants_autograd(*tensors) -> bool:
+    """Whether a call goes through its autograd function: a tensor requires a gradient, or carries a
+    forward-mode tangent, which the function refuses and a direct call would drop."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
+    if forward_ad._current_level >= 0:  # inside dual_level
+        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
     return False
 
 
@@ -212,7 +217,7 @@ def fused_linear(
     the weight's gradient) and the pre-activation (for all of them) are kept until the backward
     pass: None for bf16, "e4m3" for 8 bits (``quantize_activation``'s form): half the bytes, and
     gradients made from what is kept. The forward result is the same. Gradients have their tensors'
-    types; what no gradient needs is neither kept nor computed. Differentiable once."""
+    types; what no gradient needs is neither kept nor computed. Differentiable once, in reverse mode."""
     host = _native.lin_host()
     act, kind = _ACTS.get(activation), _HELD.get(checkpoint)
     if act is None or kind is None or torch.is_autocast_enabled("cuda") or not x.is_cuda or not host.lin_plain(
@@ -228,7 +233,7 @@ def fused_linear(
             raise RuntimeError(f"{who}: weight of shape {tuple(weight.shape)} has no elements")
         if x.numel() == 0:
             return _no_rows(x, (weight, bias), residual, weight.shape[0])
-    if _wants_grad(x, weight, bias, residual):
+    if _wants_autograd(x, weight, bias, residual):
         return _FusedLinear.apply(x, weight, bias, residual, act, kind)
     with _current(x.device):
         return host.lin_forward(x, _bf16_source(weight), bias, residual, act, kind, False, False, False,
@@ -281,7 +286,7 @@ def swiglu_mlp(
     (``quantize_activation``'s form); the gated result is made from them again, where an
     ordinary module keeps it too. The backward pass applies the gate's gradient on the sums of its first
     product. Gradients have their tensors' types; what no gradient needs is neither kept nor computed.
-    Differentiable once."""
+    Differentiable once, in reverse mode."""
     host = _native.lin_host()
     kind = _HELD.get(checkpoint)
     shapes_fit = (w_gate.dim() == 2 and w_up.shape == w_gate.shape and w_down.dim() == 2 and x.dim() > 0
@@ -298,7 +303,7 @@ def swiglu_mlp(
             raise RuntimeError(f"{who}: weights of shapes {tuple(w_gate.shape)} and {tuple(w_down.shape)} have no elements")
         if x.numel() == 0:
             return _no_rows(x, (w_gate, w_up, w_down), residual, w_down.shape[0])
-    if _wants_grad(x, w_gate, w_up, w_down, residual):
+    if _wants_autograd(x, w_gate, w_up, w_down, residual):
         return _SwigluMlp.apply(x, w_gate, w_up, w_down, residual, kind)
     with _current(x.device):
         return host.mlp_forward(x, _bf16_source(w_gate), _bf16_source(w_up), _bf16_source(w_down), residual, kind, False,
