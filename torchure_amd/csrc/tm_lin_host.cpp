@@ -225,10 +225,17 @@ void set_residual(tm_lin_t& d, const Rows& r) {
   d.res_f32 = is_f32(r.t);
 }
 
-std::vector<i64> result_shape(const Tensor& x, i64 out) {
+// A call's result in x's leading dimensions, and the same memory as rows. (The result is no view, else torch would
+// refuse to change it in place.)
+struct Result {
+  Tensor y, rows;
+};
+
+Result result_for(const Tensor& x, i64 n, i64 out, const Rows& res) {
   std::vector<i64> s(x.sizes().begin(), x.sizes().end());
   s.back() = out;
-  return s;
+  const Tensor y = room(x, s, res.t.defined() ? res.t.scalar_type() : at::kBFloat16);
+  return {y, x.dim() == 2 ? y : y.view({n, out})};
 }
 
 // y = act(x w^T + bias) + residual. Returns (y, input kept, its exponents, z kept, its exponents, the weight's
@@ -246,7 +253,8 @@ py::tuple lin_forward(const Tensor& x, const Tensor& weight, const Opt& bias, co
     const Tensor b = bias ? bias->detach().contiguous() : Tensor();
     const i64 out = weight.size(0);
     const Rows o = c.input(xr, kind, keep_x, &kept);
-    y = room(x, {xr.n, out}, res.t.defined() ? res.t.scalar_type() : at::kBFloat16);
+    const Result result = result_for(x, xr.n, out, res);
+    y = result.y;
     tm_lin_t d = desc(TM_LIN_FORWARD, xr.n, xr.d, out);
     d.act = act;
     d.bias = ptr(b);
@@ -256,8 +264,7 @@ py::tuple lin_forward(const Tensor& x, const Tensor& weight, const Opt& bias, co
       z = room_for(kind, xr.n, out, x);
       hold(d, kind, z, {});
     }
-    c.product(d, o, wr, y);
-    if (x.dim() != 2) y = y.view(result_shape(x, out));
+    c.product(d, o, wr, result.rows);
     if (keep_w) w = wr.t;
   });
   return py::make_tuple(y, or_none(kept.values), or_none(kept.exps), or_none(z.values), or_none(z.exps), or_none(w));
@@ -338,11 +345,11 @@ py::tuple mlp_forward(const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
     }
     const Rows h = {room(x, {xr.n, up(ffn, 8)}, at::kBFloat16), xr.n, ffn, up(ffn, 8)};
     c.product(d, o, in.first, h.t);
-    y = room(x, {xr.n, out}, res.t.defined() ? res.t.scalar_type() : at::kBFloat16);
+    const Result result = result_for(x, xr.n, out, res);
+    y = result.y;
     tm_lin_t e = desc(TM_LIN_FORWARD, xr.n, ffn, out);
     set_residual(e, res);
-    c.product(e, h, dr, y);
-    if (x.dim() != 2) y = y.view(result_shape(x, out));
+    c.product(e, h, dr, result.rows);
     if (keep_in) {
       wg = in.first.t;
       wu = in.second.t;
