@@ -211,3 +211,12 @@ def test_a_quantized_activation_without_dimensions(no_device):
     one = torch.zeros(1, 32, dtype=torch.uint8)
     with pytest.raises(RuntimeError, match="not those"):
         ta.dequantize_activation(ta.QuantizedActivation(one, one[:, :1], torch.Size(()), BF16))
+
+
+@pytest.mark.parametrize("wide", [64, 128, 136])
+def test_act_grad_launches_of_2_to_the_31_workgroups_without_gpu(wide):
+    """2^25 bands of 32 rows by ``wide`` groups of 256 columns: 2^31 workgroups, 2^32, and more than that."""
+    lib = _native.lib()
+    rows, cols = 1 << 30, 256 * wide
+    assert lib.tm_act_grad(FAKE, cols, None, 0, FAKE, 0, cols, None, None, 0, 0, 0, rows, cols, None, 0, None) < 0
+    assert b"too large" in lib.tm_last_error()

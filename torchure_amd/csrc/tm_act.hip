@@ -10,6 +10,8 @@
 
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "torchure_amd.h"
 #include "tm_act.h"
 #include "tm_internal.h"
@@ -290,12 +292,12 @@ __global__ __launch_bounds__(256) void col_sum_kernel(void* __restrict__ out, in
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A launch has less than 2^32 work-items, 256 a workgroup.
 // bf16 matrices of more bytes than this go past the caches, which then keep the 8-bit values: nobody finds all of such a
 // matrix there afterwards. (Into 8 bits and back, us past / through them: 320 MB 150 / 180, 192 MB 93 / 115, 128 MB 65 / 70,
 // but 96 MB 50 / 47, 64 MB 34 / 33; fp32, whose lanes have 32 bytes each, 202 / 173 at 320 MB.)
 constexpr int64_t kStreamBytes = int64_t(160) << 20;
 
+// A launch has less than 2^32 work-items, 256 a workgroup.
 constexpr int64_t kMaxRows = int64_t(1) << 30, kMaxCols = int64_t(1) << 30, kMaxGroups = (int64_t(1) << 24) - 1;
 
 int check_shape(const char* who, int64_t rows, int64_t cols, int64_t groups) {
@@ -373,7 +375,7 @@ int tm_act_grad(uint16_t* d_dz, int64_t lddz, void* d_bias, int bias_f32, const 
   const int64_t wide = ceil_div(d_dz && lddz > cols ? lddz : cols, 256);
   const int band_rows = d_bias ? kBandRows : kPlainRows;
   const int64_t bands = rows > 0 ? ceil_div(rows, band_rows) : 0;
-  if (const int rc = check_shape(who, rows, cols, max(bands * wide, d_bias ? ceil_div(cols, 64) : 0))) return rc;
+  if (const int rc = check_shape(who, rows, cols, std::max<int64_t>(bands * wide, d_bias ? ceil_div(cols, 64) : 0))) return rc;
   if (rows == 0 || cols == 0) return act_fail(TM_EINVAL, "%s: no elements", who);
   if (!d_dy || (!d_dz && !d_bias)) return act_fail(TM_EINVAL, "%s: null pointer", who);
   if (act < 0 || act > TM_ACT_GELU_TANH) return act_fail(TM_EINVAL, "%s: unknown activation %d", who, act);
