@@ -529,6 +529,14 @@ int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_v
                        int64_t ldv, int64_t rows, int64_t cols, void* stream);
 
 /*
+ * d_dst (bf16, rows ldd apart, a multiple of 8 of at least cols, 16-byte aligned) = silu(g) u, g and u as held by
+ * TM_LIN_GATE (rows ldz apart, exponents with TM_HELD_E4M3), with the bits that TM_LIN_GATE_GRAD's o1 has; zeros from
+ * cols to the next multiple of 8. For a caller that wants the down projection's weight gradient alone.
+ */
+int tm_held_gate(uint16_t* d_dst, int64_t ldd, const void* d_g, const void* d_u, const uint8_t* d_g_exponents,
+                 const uint8_t* d_u_exponents, int64_t ldz, int held, int64_t rows, int64_t cols, void* stream);
+
+/*
  * The way back through an activation: d_dz (bf16, rows lddz apart, a multiple of 8 of at least cols, zeros
  * past cols, 16-byte aligned; or NULL) = dy act'(z), dy bf16 or (dy_f32) fp32 rows ldy apart, z as held
  * by tm_lin (rows ldz apart, exponents with TM_HELD_E4M3; not read when act is TM_ACT_NONE, which makes

@@ -1,5 +1,5 @@
 """The linear layers and the gated feed-forward among a program's other tensors: results that are changed in
-place afterwards. Bit for bit against the same calls without that."""
+place afterwards, and parts of the gradients. Bit for bit against the same calls without that."""
 
 from __future__ import annotations
 
@@ -34,3 +34,75 @@ def test_results_changed_in_place(lead, checkpoint):
         same(z, (y.detach() * 2).add_(dy))
         for a, b in zip(torch.autograd.grad(z, wanted, dy), want):
             same(a, b)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+@pytest.mark.parametrize("rows,dim,ffn,out", [(1, 8, 1, 8), (33, 24, 7, 16), (70, 40, 77, 24), (300, 64, 640, 40), (1001, 72, 1237, 33)])
+def test_the_down_projections_gradient_alone(rows, dim, ffn, out, checkpoint):
+    """The gated product made again from what is held: the bits of the call with all gradients."""
+    t, dy = T.mlp_case(rows, dim, ffn, out, None, seed=31)
+    d, dy = on_device(t), dy.to(DEV)
+    args = [d[k] for k in ("x", "w_gate", "w_up", "w_down")]
+    y = ta.swiglu_mlp(*args, None, checkpoint)
+    want = torch.autograd.grad(y, args, dy)[3]
+    z = ta.swiglu_mlp(*(v.detach() for v in args[:3]), args[3], None, checkpoint)
+    same(z, y)
+    got, = torch.autograd.grad(z, args[3], dy)
+    same(got, want)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_the_down_projections_gradient_alone_keeps_and_makes_nothing_else(checkpoint):
+    """Kept: gate and up. In the backward pass: their product and the gradient. (No operand of an fp32
+    w_down, no gradients of gate and up, which are three times as many bytes as that product.)"""
+    n, dim, ffn = 2048, 256, 1024
+    g = torch.Generator(device=DEV).manual_seed(32)
+    x, wg, wu = (torch.randn(s, device=DEV, generator=g).to(BF16) for s in ((n, dim), (ffn, dim), (ffn, dim)))
+    wd = torch.randn(dim, ffn, device=DEV, generator=g).requires_grad_()
+    dy = torch.ones(n, dim, dtype=BF16, device=DEV)
+
+    def step():
+        before = torch.cuda.memory_allocated()
+        y = ta.swiglu_mlp(x, wg, wu, wd, None, checkpoint)
+        kept = torch.cuda.memory_allocated() - before - y.numel() * 2
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        torch.autograd.grad(y, wd, dy)
+        return kept, torch.cuda.max_memory_allocated() - held
+
+    step()
+    torch.cuda.synchronize()
+    kept, more = step()
+    slack = 1 << 17
+    assert kept <= (2 * n * ffn * 2 if checkpoint is None else 2 * (n * ffn + n * ffn // 1024)) + slack
+    from torchure_amd import _native
+    split = _native.lib().tm_lin_workspace_bytes(_native.TM_LIN_GRAD_W, n, ffn, dim, 0)
+    assert more <= n * ffn * 2 + wd.numel() * 4 + split + slack
+
+
+@pytest.mark.parametrize("held", [1, 2])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (37, 29), (64, 64), (65, 300)])
+def test_the_gated_product_writes_its_rows_only(rows, cols, held):
+    from torchure_amd import _native
+
+    g = torch.Generator().manual_seed(33)
+    z = [T.grid_values(g, (rows, cols), 0.25, 12) for _ in range(2)]
+    if held == 1:
+        kept = [torch.zeros(rows, -(-cols // 8) * 8, dtype=BF16, device=DEV) for _ in z]
+        for k, v in zip(kept, z):
+            k[:, :cols] = v.to(DEV)
+        exps = [None, None]
+    else:
+        q = [ta.quantize_activation(v.to(DEV)) for v in z]
+        kept, exps = [v.values for v in q], [v.exponents for v in q]
+    width = -(-cols // 8) * 8
+    room = torch.full((rows + 4, width + 16), 7.0, dtype=BF16, device=DEV)
+    _native.check(_native.lib().tm_held_gate(
+        room[2:, 8:].data_ptr(), width + 16, kept[0].data_ptr(), kept[1].data_ptr(), *(None if e is None else e.data_ptr() for e in exps),
+        kept[0].shape[1], held, rows, cols, _native.stream_handle(torch.device(DEV, 0))), "tm_held_gate")
+    inside = torch.zeros(room.shape, dtype=torch.bool, device=DEV)
+    inside[2: 2 + rows, 8: 8 + width] = True
+    assert bool((room[~inside] == 7.0).all()) and not room[2: 2 + rows, 8 + cols: 8 + width].any()
+    gate, up = (T.held64("e4m3" if held == 2 else None, v.double()) for v in z)
+    want = T.act64("silu", gate) * up
+    T.close(room[2: 2 + rows, 8: 8 + cols], want, want.abs() * 2.0 ** -8 + up.abs() * gate.abs().clamp_min(1) * T.ACT_ERR, "silu(g) u")

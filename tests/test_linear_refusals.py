@@ -220,3 +220,19 @@ def test_act_grad_launches_of_2_to_the_31_workgroups_without_gpu(wide):
     rows, cols = 1 << 30, 256 * wide
     assert lib.tm_act_grad(FAKE, cols, None, 0, FAKE, 0, cols, None, None, 0, 0, 0, rows, cols, None, 0, None) < 0
     assert b"too large" in lib.tm_last_error()
+
+
+def test_held_gate_checks_without_gpu():
+    lib = _native.lib()
+    good = [FAKE, 40, FAKE, FAKE, FAKE, FAKE, 64, _native.TM_HELD_E4M3, 33, 40, None]
+    for at, bad in ((0, None), (0, 0x1008), (1, 44), (1, 32), (2, None), (2, 0x1004), (3, None), (3, 0x1008), (4, None), (5, None),
+                    (6, 40), (6, 96), (7, 0), (7, 1), (7, 3), (8, -1), (9, -1), (8, (1 << 30) + 1)):
+        args = list(good)
+        args[at] = bad
+        if (at, bad) == (7, 1):
+            args[6] = 36  # bf16 rows: whole groups of 8
+        assert lib.tm_held_gate(*args) < 0 and b"tm_held_gate" in lib.tm_last_error(), (at, bad)
+        assert b"launch" not in lib.tm_last_error(), (at, bad)
+    assert lib.tm_held_gate(None, 0, None, None, None, None, 0, 0, 0, 40, None) == 0  # nothing to do
+    assert lib.tm_held_gate(FAKE, 8, FAKE, FAKE, None, None, 8, _native.TM_HELD_BF16, 1 << 30, 1, None) < 0  # 2^25 bands
+    assert b"too large" in lib.tm_last_error()

@@ -142,6 +142,7 @@ _SIGNATURES = {
     "tm_lin": (ctypes.c_int, [ctypes.POINTER(TmLin), _vp, ctypes.c_size_t, _vp]),
     "tm_quantize_e4m3": (ctypes.c_int, [_vp, _vp, _i64, _vp, ctypes.c_int, _i64, _i64, _i64, _vp, _i64, _vp]),
     "tm_dequantize_e4m3": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _vp, _vp, _i64, _i64, _i64, _vp]),
+    "tm_held_gate": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, ctypes.c_int, _i64, _i64, _vp]),
     "tm_act_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "tm_act_grad": (
         ctypes.c_int,

@@ -1,5 +1,6 @@
 // tm_act.hip -- gfx950 element-wise kernels around the linear layers' products (tm_linear.hip):
 //   quantize_kernel, dequantize_kernel   activations into 8 bits and back (the format: tm_act.h)
+//   gate_kernel                          silu(g) u from g and u as held, where no other gradient makes it
 //   act_grad_kernel                      dz = dy act'(z) from z as held, with the column sums of dz, and
 //   col_sum_kernel                       the bias gradient from those sums
 // All are bound by memory: every element is read and written once, 16 bytes a lane.
@@ -194,6 +195,60 @@ __global__ __launch_bounds__(256) void dequantize_kernel(void* __restrict__ dst,
   }
 }
 
+// silu(g) u, a wave's elements as above, each by the operations of the gate's gradient (tm_linear.hip), so with its bits.
+// Columns from cols to the next multiple of 8 are held as zeros.
+template <bool kE4m3>
+__global__ __launch_bounds__(256) void gate_kernel(uint16_t* __restrict__ dst, int64_t ldd,
+                                                   const uint8_t* __restrict__ g, const uint8_t* __restrict__ u,
+                                                   const uint8_t* __restrict__ g_exps,
+                                                   const uint8_t* __restrict__ u_exps, int64_t ldz, int64_t rows,
+                                                   int cols, int wide) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t band = blockIdx.x / wide;
+  const int n = (static_cast<int>(blockIdx.x % wide) * 4 + wave) * 64 + 8 * (lane & 7);
+  if (n >= cols) return;
+  const int64_t m = band * 32 + (lane >> 3);
+  u32x4 a[4], b[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (m + 8 * i >= rows) continue;
+    const int64_t at = (m + 8 * i) * ldz + n;
+    if constexpr (kE4m3) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(g + at), y = *reinterpret_cast<const u32x2*>(u + at);
+      a[i] = u32x4{x.x, x.y, 0, 0};
+      b[i] = u32x4{y.x, y.y, 0, 0};
+    } else {
+      a[i] = *reinterpret_cast<const u32x4*>(g + 2 * at);
+      b[i] = *reinterpret_cast<const u32x4*>(u + 2 * at);
+    }
+  }
+  float sg = 1.0f, su = 1.0f;
+  if constexpr (kE4m3) {
+    const int64_t at = band * ((cols + 31) / 32) + (n >> 5);
+    sg = tm_act::two_to(static_cast<int>(g_exps[at]) - 127);
+    su = tm_act::two_to(static_cast<int>(u_exps[at]) - 127);
+  }
+  auto values = [](float (&x)[8], const u32x4& w, float scale) {
+    if constexpr (kE4m3) {
+      const f32x4 lo = tm_act::decode4(w.x, scale), hi = tm_act::decode4(w.y, scale);
+      x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
+      x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+    } else {
+      values8<false>(x, Raw8<false>{{w}});
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (m + 8 * i >= rows) continue;
+    float z[8], h[8];
+    values(z, a[i], sg);
+    values(h, b[i], su);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] *= z[e] * tm_act::sigmoid(z[e]);
+    put8<false>(dst, (m + 8 * i) * ldd + n, h, 8);
+  }
+}
+
 // Rows of a workgroup, and of one partial column sum where those are made. (8192 x 1024 fp32 dy cast to bf16: 19.8 us
 // with 128 rows, whose 256 workgroups leave a CU with four waves.)
 constexpr int kBandRows = 64, kPlainRows = 32;
@@ -360,6 +415,32 @@ int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_v
   if (dst_f32) launch(Int<1>{}, Int<0>{});
   else if (rows * cols * 2 > kStreamBytes) launch(Int<0>{}, Int<1>{});
   else launch(Int<0>{}, Int<0>{});
+  return launched(who);
+}
+
+int tm_held_gate(uint16_t* d_dst, int64_t ldd, const void* d_g, const void* d_u, const uint8_t* d_g_exponents,
+                 const uint8_t* d_u_exponents, int64_t ldz, int held, int64_t rows, int64_t cols, void* stream) {
+  const char* who = "tm_held_gate";
+  const int64_t wide = ceil_div(cols, 256), groups = rows > 0 && cols > 0 ? ceil_div(rows, 32) * wide : 0;
+  if (const int rc = check_shape(who, rows, cols, groups)) return rc;
+  if (groups == 0) return TM_OK;
+  if (!d_dst || !d_g || !d_u || (held == TM_HELD_E4M3 && (!d_g_exponents || !d_u_exponents)))
+    return act_fail(TM_EINVAL, "%s: null pointer", who);
+  if (ldd % 8 || ldd < cols || !aligned(d_dst, 16) || !aligned(d_g, 16) || !aligned(d_u, 16))
+    return act_fail(TM_EINVAL, "%s: output rows %lld apart for %lld columns: a multiple of 8; all 16-byte aligned", who,
+                    (long long)ldd, (long long)cols);
+  if (held == TM_HELD_BF16 ? ldz % 8 || ldz < cols : held != TM_HELD_E4M3 || ldz != ceil_div(cols, 32) * 32)
+    return act_fail(TM_EINVAL, "%s: held as %d in rows %lld apart for %lld columns", who, held, (long long)ldz,
+                    (long long)cols);
+  const dim3 grid(static_cast<uint32_t>(groups));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  auto launch = [&](auto e4m3) {
+    hipLaunchKernelGGL((gate_kernel<decltype(e4m3)::value != 0>), grid, dim3(256), 0, s, d_dst, ldd,
+                       static_cast<const uint8_t*>(d_g), static_cast<const uint8_t*>(d_u), d_g_exponents, d_u_exponents,
+                       ldz, rows, static_cast<int>(cols), static_cast<int>(wide));
+  };
+  if (held == TM_HELD_E4M3) launch(Int<1>{});
+  else launch(Int<0>{});
   return launched(who);
 }
 

@@ -28,6 +28,7 @@ struct Abi {
   decltype(&tm_lin) lin;
   decltype(&tm_quantize_e4m3) quantize;
   decltype(&tm_dequantize_e4m3) dequantize;
+  decltype(&tm_held_gate) held_gate;
   decltype(&tm_act_grad_workspace_bytes) act_bytes;
   decltype(&tm_act_grad) act_grad;
   decltype(&tm_last_error) last_error;
@@ -43,6 +44,7 @@ void lin_bind(const py::dict& addresses, const py::object& native_error) {
   a->lin = reinterpret_cast<decltype(a->lin)>(at("tm_lin"));
   a->quantize = reinterpret_cast<decltype(a->quantize)>(at("tm_quantize_e4m3"));
   a->dequantize = reinterpret_cast<decltype(a->dequantize)>(at("tm_dequantize_e4m3"));
+  a->held_gate = reinterpret_cast<decltype(a->held_gate)>(at("tm_held_gate"));
   a->act_bytes = reinterpret_cast<decltype(a->act_bytes)>(at("tm_act_grad_workspace_bytes"));
   a->act_grad = reinterpret_cast<decltype(a->act_grad)>(at("tm_act_grad"));
   a->last_error = reinterpret_cast<decltype(a->last_error)>(at("tm_last_error"));
@@ -156,6 +158,16 @@ struct Call {
     check(a.dequantize(ptr(out), is_f32(out), ld, bytes_of(h.values), bytes_of(h.exps), h.values.size(1), rows, cols,
                        stream),
           "tm_dequantize_e4m3");
+  }
+
+  // silu(g) u of what is held, as an operand.
+  Rows held_gate(const Held& g, const Held& u, int kind, i64 cols) const {
+    const i64 n = g.values.size(0), ld = up(cols, 8);
+    const Tensor h = room(g.values, {n, ld}, at::kBFloat16);
+    check(a.held_gate(bf16_of(h), ld, ptr(g.values), ptr(u.values), bytes_of(g.exps), bytes_of(u.exps), g.values.size(1),
+                      kind, n, cols, stream),
+          "tm_held_gate");
+    return {h, n, cols, ld};
   }
 
   // The first product's operand, and what is kept of it for the weight's gradient.
@@ -363,7 +375,7 @@ py::tuple mlp_forward(const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
 
 // (dx, dw_gate, dw_up, dw_down), each as asked for.
 py::tuple mlp_backward(const Tensor& dy, const Opt& xv, const Opt& xs, const Tensor& gv, const Opt& gs, const Tensor& uv,
-                       const Opt& us, const Opt& wg, const Opt& wu, const Tensor& wd, std::vector<i64> x_sizes, i64 ffn,
+                       const Opt& us, const Opt& wg, const Opt& wu, const Opt& wd, std::vector<i64> x_sizes, i64 ffn,
                        bool x_f32, bool g_f32, bool u_f32, bool d_f32, int kind, bool need_x, bool need_g, bool need_u,
                        bool need_d, uintptr_t stream) {
   HANDLE_TH_ERRORS
@@ -375,15 +387,20 @@ py::tuple mlp_backward(const Tensor& dy, const Opt& xv, const Opt& xs, const Ten
     auto weight = [](const Tensor& t, i64 rows, i64 cols) {
       return Rows{t, rows, cols, rows > 1 ? t.stride(0) : t.size(1)};
     };
-    // [d_gate | d_up], and the down projection's input again
-    const Rows both = {room(dy, {n, 2 * pad}, at::kBFloat16), n, ffn, 2 * pad};
-    Rows h = {Tensor(), n, ffn, pad};
-    if (need_d) h.t = room(dy, {n, pad}, at::kBFloat16);
-    tm_lin_t p = desc(TM_LIN_GATE_GRAD, n, ffn, out);
-    hold(p, kind, {gv, of(gs)}, {uv, of(us)});
-    p.o1 = ptr(h.t);
-    p.ldo1 = pad;
-    c.product(p, a, weight(wd, out, ffn), both.t);
+    const Held g = {gv, of(gs)}, u = {uv, of(us)};
+    // [d_gate | d_up], where a gradient behind them is wanted, and the down projection's input again
+    Rows both = {Tensor(), n, ffn, 2 * pad}, h = {Tensor(), n, ffn, pad};
+    if (need_x || need_g || need_u) {
+      both.t = room(dy, {n, 2 * pad}, at::kBFloat16);
+      if (need_d) h.t = room(dy, {n, pad}, at::kBFloat16);
+      tm_lin_t p = desc(TM_LIN_GATE_GRAD, n, ffn, out);
+      hold(p, kind, g, u);
+      p.o1 = ptr(h.t);
+      p.ldo1 = pad;
+      c.product(p, a, weight(*wd, out, ffn), both.t);
+    } else if (need_d) {
+      h = c.held_gate(g, u, kind, ffn);
+    }
     if (need_d) {
       dd = room(dy, {out, ffn}, type_of(d_f32));
       tm_lin_t q = desc(TM_LIN_GRAD_W, n, ffn, out);

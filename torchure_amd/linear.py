@@ -247,11 +247,11 @@ class _SwigluMlp(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, residual, kind):
         need_x, need_g, need_u, need_d, _ = ctx.needs_input_grad[:5]
-        any_of = need_x or need_g or need_u or need_d
+        behind_gate = need_x or need_g or need_u
         with _current(x.device):
             y, *kept = _native.lin_host().mlp_forward(
-                x, _bf16_source(w_gate), _bf16_source(w_up), _bf16_source(w_down), residual, kind, need_g or need_u, any_of,
-                need_x, any_of, _native.stream_handle(x.device))
+                x, _bf16_source(w_gate), _bf16_source(w_up), _bf16_source(w_down), residual, kind, need_g or need_u,
+                behind_gate or need_d, need_x, behind_gate, _native.stream_handle(x.device))
         ctx.meta = (x.shape, w_gate.shape[0], *(t.dtype == _F32 for t in (x, w_gate, w_up, w_down)), kind)
         ctx.save_for_backward(*kept)
         return y
@@ -285,7 +285,8 @@ def swiglu_mlp(
     pass are the input and the two products, in bf16 or, with ``checkpoint="e4m3"``, in 8 bits
     (``quantize_activation``'s form); the gated result is made from them again, where an
     ordinary module keeps it too. The backward pass applies the gate's gradient on the sums of its first
-    product. Gradients have their tensors' types; what no gradient needs is neither kept nor computed.
+    product, whose two results, of gate and up, are made together where either's weight or x wants a
+    gradient. Gradients have their tensors' types; what else no gradient needs is neither kept nor computed.
     Differentiable once, in reverse mode."""
     host = _native.lin_host()
     kind = _HELD.get(checkpoint)
