@@ -1,5 +1,6 @@
 """The linear layers and the gated feed-forward among a program's other tensors: results that are changed in
-place afterwards, and parts of the gradients. Bit for bit against the same calls without that."""
+place afterwards, operands that are negated views, and parts of the gradients. Bit for bit against the same calls
+without that."""
 
 from __future__ import annotations
 
@@ -106,3 +107,26 @@ def test_the_gated_product_writes_its_rows_only(rows, cols, held):
     gate, up = (T.held64("e4m3" if held == 2 else None, v.double()) for v in z)
     want = T.act64("silu", gate) * up
     T.close(room[2: 2 + rows, 8: 8 + cols], want, want.abs() * 2.0 ** -8 + up.abs() * gate.abs().clamp_min(1) * T.ACT_ERR, "silu(g) u")
+
+
+@pytest.mark.parametrize("out", [1, 48])
+def test_operands_that_are_negated_views(out):
+    """z.conj().imag is a view of z's memory with a flag for the sign."""
+    g = torch.Generator().manual_seed(34)
+
+    def negated(*shape):
+        v = torch.complex(torch.zeros(shape), torch.randn(shape, generator=g)).to(DEV).conj().imag
+        assert v.is_neg()
+        return v
+
+    x, w, m = (torch.randn(s, generator=g).to(BF16).to(DEV) for s in ((20, 40), (out, 40), (40, 40)))
+    b, r, n, h = negated(out), negated(20, out), torch._neg_view(w), torch._neg_view(x)
+    clones = [v.clone().resolve_neg() for v in (b, r, n, h)]
+    for act in (None, "silu"):
+        same(ta.fused_linear(h, n, b, r, act), ta.fused_linear(clones[3], clones[2], clones[0], clones[1], act))
+    same(ta.swiglu_mlp(h, m, m, n, r), ta.swiglu_mlp(clones[3], m, m, clones[2], clones[1]))
+    a, c = ta.quantize_activation(r), ta.quantize_activation(clones[1])
+    assert torch.equal(a.values, c.values) and torch.equal(a.exponents, c.exponents)
+    w = w.requires_grad_()
+    y = ta.fused_linear(x, w, None, clones[1])
+    same(torch.autograd.grad(y, w, r, retain_graph=True)[0], torch.autograd.grad(y, w, clones[1])[0])

@@ -262,7 +262,7 @@ py::tuple lin_forward(const Tensor& x, const Tensor& weight, const Opt& bias, co
     const Rows xr = rows_of(x), wr = c.operand(rows_of(weight));
     Rows res;
     if (residual) res = rows_of(*residual);
-    const Tensor b = bias ? bias->detach().contiguous() : Tensor();
+    const Tensor b = bias ? bias->detach().resolve_neg().contiguous() : Tensor();
     const i64 out = weight.size(0);
     const Rows o = c.input(xr, kind, keep_x, &kept);
     const Result result = result_for(x, xr.n, out, res);
