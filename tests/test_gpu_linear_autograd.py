@@ -1,6 +1,6 @@
 """The linear layers and the gated feed-forward among a program's other tensors: results that are changed in
-place afterwards, operands that are negated views, and parts of the gradients. Bit for bit against the same calls
-without that."""
+place afterwards, operands that are negated views, kept tensors that hooks move, and parts of the
+gradients. Bit for bit against the same calls without that."""
 
 from __future__ import annotations
 
@@ -130,3 +130,37 @@ def test_operands_that_are_negated_views(out):
     w = w.requires_grad_()
     y = ta.fused_linear(x, w, None, clones[1])
     same(torch.autograd.grad(y, w, r, retain_graph=True)[0], torch.autograd.grad(y, w, clones[1])[0])
+
+
+@pytest.mark.parametrize("checkpoint", [None, "e4m3"])
+def test_kept_tensors_that_come_back_in_other_strides(checkpoint):
+    """Hooks that give some of what is kept back in rows of their own, wider ones or columns."""
+    t, dy = T.linear_case(40, 64, 48, "silu", BF16, None, checkpoint, seed=35)
+    m, mdy = T.mlp_case(40, 64, 96, 48, None, seed=35)
+    d, dy, m, mdy = on_device(t), dy.to(DEV), on_device(m), mdy.to(DEV)
+    for name in ("w_gate", "w_up"):  # equal strides
+        room = torch.zeros(96, 192, dtype=BF16, device=DEV)
+        room[:, 64:128] = m[name].detach()
+        m[name] = room[:, 64:128].requires_grad_()
+
+    def wider(v):
+        return torch.empty(v.shape[0], v.shape[1] + 32, dtype=v.dtype, device=DEV)[:, : v.shape[1]].copy_(v)
+
+    ways = (torch.Tensor.contiguous, wider, lambda v: v.t().contiguous().t())
+    calls = ((lambda a: ta.fused_linear(*a, None, "silu", checkpoint), [d[k] for k in ("x", "weight", "bias")], dy),
+             (lambda a: ta.swiglu_mlp(*a, None, checkpoint), [m[k] for k in ("x", "w_gate", "w_up", "w_down")], mdy))
+    for call, args, g in calls:
+        want = torch.autograd.grad(call(args), args, g)
+        for way in ways:
+            for part in range(2):
+                count = [0]
+
+                def unpack(v):
+                    count[0] += 1
+                    return way(v.clone()) if count[0] % 2 == part else v
+
+                with torch.autograd.graph.saved_tensors_hooks(lambda v: v, unpack):
+                    y = call(args)
+                for a, b in zip(torch.autograd.grad(y, args, g), want):
+                    same(a, b)
+                assert count[0] > 1

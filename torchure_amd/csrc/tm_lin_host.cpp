@@ -83,7 +83,6 @@ bool is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
 char* ptr(const Tensor& t) { return t.defined() ? static_cast<char*>(t.data_ptr()) : nullptr; }
 uint8_t* bytes_of(const Tensor& t) { return reinterpret_cast<uint8_t*>(ptr(t)); }
 uint16_t* bf16_of(const Tensor& t) { return reinterpret_cast<uint16_t*>(ptr(t)); }
-Tensor of(const Opt& t) { return t ? *t : Tensor(); }
 py::object or_none(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
 Tensor room(const Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
@@ -116,6 +115,18 @@ bool fits(const Rows& r) {  // whole 16-byte groups, as the kernels read operand
 struct Held {
   Tensor values, exps;
 };
+
+// What the backward pass is given of it. (A saved tensor may come back in other strides than it was kept in: moved to
+// the host and back, say.)
+Held held_of(const Opt& values, const Opt& exps) {
+  return {values ? values->contiguous() : Tensor(), exps ? exps->contiguous() : Tensor()};
+}
+
+// A weight's kept operand, whole rows of it.
+Rows weight_of(const Tensor& kept, i64 rows, i64 cols) {
+  const Tensor t = kept.stride(1) == 1 ? kept : kept.contiguous();
+  return {t, rows, cols, rows > 1 ? t.stride(0) : t.size(1)};
+}
 
 Held room_for(int kind, i64 rows, i64 cols, const Tensor& like) {
   if (kind == TM_HELD_BF16) return {room(like, {rows, up(cols, 8)}, at::kBFloat16), {}};
@@ -187,9 +198,10 @@ struct Call {
   }
 
   // The bf16 operand of a kept input of `cols` columns.
-  Rows kept_operand(const Held& h, i64 cols) const {
-    const i64 n = h.values.size(0);
-    if (!h.exps.defined()) return {h.values, n, cols, n > 1 ? h.values.stride(0) : h.values.size(1)};
+  Rows kept_operand(const Tensor& values, const Opt& exps, i64 cols) const {
+    const i64 n = values.size(0);
+    if (!exps) return weight_of(values, n, cols);
+    const Held h = held_of(values, exps);
     const i64 ld = up(cols, 8);
     Tensor p = room(h.values, {n, ld}, at::kBFloat16);
     if (ld != cols) p.narrow(1, cols, ld - cols).zero_();
@@ -300,35 +312,33 @@ py::tuple lin_backward(const Tensor& dy, const Opt& xv, const Opt& xs, const Opt
     Rows dz = d;
     if (act || (products && !fits(d))) {
       if (products) dz = {room(dy, {d.n, up(d.d, 8)}, at::kBFloat16), d.n, d.d, up(d.d, 8)};
-      c.act_grad(products ? dz.t : Tensor(), db, d, act ? kind : TM_HELD_NOT, act ? Held{of(zv), of(zs)} : Held{}, act);
+      c.act_grad(products ? dz.t : Tensor(), db, d, act ? kind : TM_HELD_NOT, act ? held_of(zv, zs) : Held{}, act);
     } else if (need_b) {
       c.act_grad({}, db, d, TM_HELD_NOT, {}, TM_ACT_NONE);
     }
     if (need_x) {
       dx = room(dy, {d.n, inp}, type_of(x_f32));
       tm_lin_t p = desc(TM_LIN_GRAD_X, d.n, inp, d.d);
-      const Rows wr = {*w, d.d, inp, d.d > 1 ? w->stride(0) : w->size(1)};
-      c.product(p, dz, wr, dx);
+      c.product(p, dz, weight_of(*w, d.d, inp), dx);
       dx = dx.view(x_sizes);
     }
     if (need_w) {
       dw = room(dy, {d.d, inp}, type_of(w_f32));
       tm_lin_t p = desc(TM_LIN_GRAD_W, d.n, inp, d.d);
-      c.product(p, dz, c.kept_operand({of(xv), of(xs)}, inp), dw);
+      c.product(p, dz, c.kept_operand(*xv, xs, inp), dw);
     }
   });
   return py::make_tuple(or_none(dx), or_none(dw), or_none(db));
   END_HANDLE_TH_ERRORS_PYBIND
 }
 
-// The gate's and up's weights as operands with equal row strides.
-std::pair<Rows, Rows> pair_of(const Call& c, const Tensor& w_gate, const Tensor& w_up) {
-  Rows g = c.operand(rows_of(w_gate)), u = c.operand(rows_of(w_up));
+// The gate's and up's weights with equal row strides, which a product of both reads them in. (Operands of different
+// strides are rows of d, a multiple of 8, or d's next one.)
+std::pair<Rows, Rows> alike(Rows g, Rows u) {
   if (g.ld != u.ld) {  // one strided, one not: both into rows of their own
-    g = {g.t.narrow(1, 0, g.d).contiguous(), g.n, g.d, g.d};
-    u = {u.t.narrow(1, 0, u.d).contiguous(), u.n, u.d, u.d};
-    g = c.operand(g);
-    u = c.operand(u);
+    const i64 wide = up(g.d, 8);
+    g = {g.t.narrow(1, 0, wide).contiguous(), g.n, g.d, wide};
+    u = {u.t.narrow(1, 0, wide).contiguous(), u.n, u.d, wide};
   }
   return {g, u};
 }
@@ -343,7 +353,7 @@ py::tuple mlp_forward(const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
   without_gil([&] {
     const Call c{abi(), reinterpret_cast<void*>(stream)};
     const Rows xr = rows_of(x), dr = c.operand(rows_of(w_down));
-    const auto in = pair_of(c, w_gate, w_up);
+    const auto in = alike(c.operand(rows_of(w_gate)), c.operand(rows_of(w_up)));
     Rows res;
     if (residual) res = rows_of(*residual);
     const i64 ffn = w_gate.size(0), out = w_down.size(0);
@@ -384,10 +394,7 @@ py::tuple mlp_backward(const Tensor& dy, const Opt& xv, const Opt& xs, const Ten
     const Call c{abi(), reinterpret_cast<void*>(stream)};
     const Rows a = c.operand(rows_of(dy));
     const i64 n = a.n, out = a.d, dim = x_sizes.back(), pad = up(ffn, 64);
-    auto weight = [](const Tensor& t, i64 rows, i64 cols) {
-      return Rows{t, rows, cols, rows > 1 ? t.stride(0) : t.size(1)};
-    };
-    const Held g = {gv, of(gs)}, u = {uv, of(us)};
+    const Held g = held_of(gv, gs), u = held_of(uv, us);
     // [d_gate | d_up], where a gradient behind them is wanted, and the down projection's input again
     Rows both = {Tensor(), n, ffn, 2 * pad}, h = {Tensor(), n, ffn, pad};
     if (need_x || need_g || need_u) {
@@ -397,7 +404,7 @@ py::tuple mlp_backward(const Tensor& dy, const Opt& xv, const Opt& xs, const Ten
       hold(p, kind, g, u);
       p.o1 = ptr(h.t);
       p.ldo1 = pad;
-      c.product(p, a, weight(*wd, out, ffn), both.t);
+      c.product(p, a, weight_of(*wd, out, ffn), both.t);
     } else if (need_d) {
       h = c.held_gate(g, u, kind, ffn);
     }
@@ -410,12 +417,13 @@ py::tuple mlp_backward(const Tensor& dy, const Opt& xv, const Opt& xs, const Ten
     if (need_x) {
       dx = room(dy, {n, dim}, type_of(x_f32));
       tm_lin_t q = desc(TM_LIN_GRAD_X, n, dim, ffn);
-      q.b1 = bf16_of(*wu);
-      c.product(q, both, weight(*wg, ffn, dim), dx, true);
+      const auto in = alike(weight_of(*wg, ffn, dim), weight_of(*wu, ffn, dim));
+      q.b1 = bf16_of(in.second.t);
+      c.product(q, both, in.first, dx, true);
       dx = dx.view(x_sizes);
     }
     if (need_g || need_u) {
-      const Rows xb = c.kept_operand({of(xv), of(xs)}, dim);
+      const Rows xb = c.kept_operand(*xv, xs, dim);
       if (need_g) dg = room(dy, {ffn, dim}, type_of(g_f32));
       if (need_u) du = room(dy, {ffn, dim}, type_of(u_f32));
       if (need_g && need_u && g_f32 == u_f32) {
