@@ -521,8 +521,11 @@ int tm_lin(const tm_lin_t* h_desc, void* d_ws, size_t ws_bytes, void* stream);
  * 448 2^119 they are held as that, infinities and NaN as NaN. Reading back is exact in bf16 and fp32.
  *   tm_quantize_e4m3    from bf16 or (src_f32) fp32 rows lds apart. d_copy, when given: the values as bf16
  *                       too, rows ldc apart (cols' next multiple of 8; padding zero, 16-byte aligned).
- *   tm_dequantize_e4m3  to bf16 or fp32 rows ldd apart.
+ *   tm_dequantize_e4m3  to bf16 or (dst_f32) fp32 rows ldd apart.
+ * src_f32 and dst_f32 are 0 or 1, with TM_READ_NEXT added where the source, or the output, is read right
+ * after: else large bf16 matrices go past the caches.
  */
+#define TM_READ_NEXT 2
 int tm_quantize_e4m3(uint8_t* d_values, uint8_t* d_exponents, int64_t ldv, const void* d_src, int src_f32, int64_t lds,
                      int64_t rows, int64_t cols, uint16_t* d_copy, int64_t ldc, void* stream);
 int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_values, const uint8_t* d_exponents,

@@ -164,3 +164,27 @@ def test_kept_tensors_that_come_back_in_other_strides(checkpoint):
                 for a, b in zip(torch.autograd.grad(y, args, g), want):
                     same(a, b)
                 assert count[0] > 1
+
+
+def test_large_matrices_that_a_product_reads_next():
+    """On either side of the size from which bf16 matrices may go past the caches: the same bits."""
+    from torchure_amd import _native
+
+    g = torch.Generator(device=DEV).manual_seed(36)
+    for rows in (10_000, 10_300):
+        x, w = torch.randn(rows, 8192, generator=g, device=DEV).to(BF16), torch.randn(40, 8192, generator=g, device=DEV).to(BF16)
+        dy = torch.randn(rows, 40, generator=g, device=DEV).to(BF16)
+        w.requires_grad_()
+        q = ta.quantize_activation(x)
+        y = ta.fused_linear(x, w, checkpoint="e4m3")
+        same(y, ta.fused_linear(x, w))
+        held = ta.dequantize_activation(q)
+        same(torch.autograd.grad(y, w, dy)[0], torch.autograd.grad(ta.fused_linear(held, w), w, dy)[0])
+        lib, stream = _native.lib(), _native.stream_handle(torch.device(DEV, 0))
+        values, exps, back = torch.empty_like(q.values), torch.empty_like(q.exponents), torch.empty_like(x)
+        _native.check(lib.tm_quantize_e4m3(values.data_ptr(), exps.data_ptr(), 8192, x.data_ptr(), _native.TM_READ_NEXT, 8192, rows,
+                                           8192, None, 0, stream), "tm_quantize_e4m3")
+        _native.check(lib.tm_dequantize_e4m3(back.data_ptr(), _native.TM_READ_NEXT, 8192, values.data_ptr(), exps.data_ptr(), 8192,
+                                             rows, 8192, stream), "tm_dequantize_e4m3")
+        assert torch.equal(values, q.values) and torch.equal(exps, q.exponents)
+        same(back, held)

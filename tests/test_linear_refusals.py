@@ -236,3 +236,12 @@ def test_held_gate_checks_without_gpu():
     assert lib.tm_held_gate(None, 0, None, None, None, None, 0, 0, 0, 40, None) == 0  # nothing to do
     assert lib.tm_held_gate(FAKE, 8, FAKE, FAKE, None, None, 8, _native.TM_HELD_BF16, 1 << 30, 1, None) < 0  # 2^25 bands
     assert b"too large" in lib.tm_last_error()
+
+
+def test_unknown_flags_without_gpu():
+    lib = _native.lib()
+    for flags in (4, 5, -1, 1 << 30):
+        assert lib.tm_quantize_e4m3(FAKE, FAKE, 64, FAKE, flags, 40, 33, 40, None, 0, None) < 0
+        assert b"flags" in lib.tm_last_error()
+        assert lib.tm_dequantize_e4m3(FAKE, flags, 40, FAKE, FAKE, 64, 33, 40, None) < 0
+        assert b"flags" in lib.tm_last_error()

@@ -35,6 +35,7 @@ TM_NOALLOC_MAX_TENSORS = 16384
 TM_LIN_FORWARD, TM_LIN_GATE, TM_LIN_GRAD_X, TM_LIN_GATE_GRAD, TM_LIN_GRAD_W = range(5)
 TM_ACTS = ("none", "relu", "silu", "gelu", "gelu_tanh")  # TM_ACT_*, in order
 TM_HELD_NOT, TM_HELD_BF16, TM_HELD_E4M3 = range(3)
+TM_READ_NEXT = 2
 
 # tm_tensor_t (include/torchure_amd.h), 64 bytes.
 TENSOR_DTYPE = np.dtype(

@@ -347,9 +347,11 @@ __global__ __launch_bounds__(256) void col_sum_kernel(void* __restrict__ out, in
 bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// bf16 matrices of more bytes than this go past the caches, which then keep the 8-bit values: nobody finds all of such a
-// matrix there afterwards. (Into 8 bits and back, us past / through them: 320 MB 150 / 180, 192 MB 93 / 115, 128 MB 65 / 70,
-// but 96 MB 50 / 47, 64 MB 34 / 33; fp32, whose lanes have 32 bytes each, 202 / 173 at 320 MB.)
+// bf16 matrices of more bytes than this go past the caches, which then keep the 8-bit values, unless the caller says that
+// they are read next. (Into 8 bits and back, us past / through them: 320 MB 150 / 180, 192 MB 93 / 115, 128 MB 65 / 70,
+// but 96 MB 50 / 47, 64 MB 34 / 33; fp32, whose lanes have 32 bytes each, 202 / 173 at 320 MB. Into 8 bits and through a
+// product of 128 columns, which finds part of the matrix in the caches: 175 MB 99 / 94, back and through the weight's
+// gradient 102 / 91; of 1024 columns, 169 MB, 195 / 190 and 197 / 197; at 320 MB no difference.)
 constexpr int64_t kStreamBytes = int64_t(160) << 20;
 
 // A launch has less than 2^32 work-items, 256 a workgroup.
@@ -373,25 +375,28 @@ extern "C" {
 int tm_quantize_e4m3(uint8_t* d_values, uint8_t* d_exponents, int64_t ldv, const void* d_src, int src_f32, int64_t lds,
                      int64_t rows, int64_t cols, uint16_t* d_copy, int64_t ldc, void* stream) {
   const char* who = "tm_quantize_e4m3";
+  if (src_f32 & ~(1 | TM_READ_NEXT)) return act_fail(TM_EINVAL, "%s: unknown flags %d", who, src_f32);
+  const bool f32 = src_f32 & 1;
   const int64_t wide = ceil_div(cols, 256), groups = rows > 0 && cols > 0 ? ceil_div(rows, 32) * wide : 0;
   if (const int rc = check_shape(who, rows, cols, groups)) return rc;
   if (groups == 0) return TM_OK;
   if (!d_values || !d_exponents || !d_src) return act_fail(TM_EINVAL, "%s: null pointer", who);
-  if (ldv != ceil_div(cols, 32) * 32 || !aligned(d_values, 16) || lds < cols || !aligned(d_src, src_f32 ? 4 : 2))
+  if (ldv != ceil_div(cols, 32) * 32 || !aligned(d_values, 16) || lds < cols || !aligned(d_src, f32 ? 4 : 2))
     return act_fail(TM_EINVAL, "%s: values (rows %lld apart) need rows of the next multiple of 32 to %lld, 16-byte "
                     "aligned; source rows are %lld apart", who, (long long)ldv, (long long)cols, (long long)lds);
   if (d_copy && (ldc != ceil_div(cols, 8) * 8 || !aligned(d_copy, 16)))
     return act_fail(TM_EINVAL, "%s: copy rows %lld apart for %lld columns: the next multiple of 8, 16-byte aligned", who,
                     (long long)ldc, (long long)cols);
+  const bool past = !f32 && !(src_f32 & TM_READ_NEXT) && rows * cols * 2 > kStreamBytes;
   const dim3 grid(static_cast<uint32_t>(groups));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  auto launch = [&](auto f32, auto stream8) {
-    hipLaunchKernelGGL((quantize_kernel<decltype(f32)::value != 0, decltype(stream8)::value != 0>), grid, dim3(256), 0, s,
+  auto launch = [&](auto kind, auto stream8) {
+    hipLaunchKernelGGL((quantize_kernel<decltype(kind)::value != 0, decltype(stream8)::value != 0>), grid, dim3(256), 0, s,
                        d_values, d_exponents, ldv, d_src, lds, rows, static_cast<int>(cols), static_cast<int>(wide),
                        d_copy, ldc);
   };
-  if (src_f32) launch(Int<1>{}, Int<0>{});
-  else if (rows * cols * 2 > kStreamBytes) launch(Int<0>{}, Int<1>{});
+  if (f32) launch(Int<1>{}, Int<0>{});
+  else if (past) launch(Int<0>{}, Int<1>{});
   else launch(Int<0>{}, Int<0>{});
   return launched(who);
 }
@@ -399,21 +404,24 @@ int tm_quantize_e4m3(uint8_t* d_values, uint8_t* d_exponents, int64_t ldv, const
 int tm_dequantize_e4m3(void* d_dst, int dst_f32, int64_t ldd, const uint8_t* d_values, const uint8_t* d_exponents,
                        int64_t ldv, int64_t rows, int64_t cols, void* stream) {
   const char* who = "tm_dequantize_e4m3";
+  if (dst_f32 & ~(1 | TM_READ_NEXT)) return act_fail(TM_EINVAL, "%s: unknown flags %d", who, dst_f32);
+  const bool f32 = dst_f32 & 1;
   const int64_t wide = ceil_div(cols, 256), groups = rows > 0 && cols > 0 ? ceil_div(rows, 32) * wide : 0;
   if (const int rc = check_shape(who, rows, cols, groups)) return rc;
   if (groups == 0) return TM_OK;
   if (!d_values || !d_exponents || !d_dst) return act_fail(TM_EINVAL, "%s: null pointer", who);
-  if (ldv != ceil_div(cols, 32) * 32 || !aligned(d_values, 16) || ldd < cols || !aligned(d_dst, dst_f32 ? 4 : 2))
+  if (ldv != ceil_div(cols, 32) * 32 || !aligned(d_values, 16) || ldd < cols || !aligned(d_dst, f32 ? 4 : 2))
     return act_fail(TM_EINVAL, "%s: values (rows %lld apart) need rows of the next multiple of 32 to %lld, 16-byte "
                     "aligned; output rows are %lld apart", who, (long long)ldv, (long long)cols, (long long)ldd);
+  const bool past = !f32 && !(dst_f32 & TM_READ_NEXT) && rows * cols * 2 > kStreamBytes;
   const dim3 grid(static_cast<uint32_t>(groups));
   hipStream_t s = static_cast<hipStream_t>(stream);
-  auto launch = [&](auto f32, auto stream8) {
-    hipLaunchKernelGGL((dequantize_kernel<decltype(f32)::value != 0, decltype(stream8)::value != 0>), grid, dim3(256), 0, s,
+  auto launch = [&](auto kind, auto stream8) {
+    hipLaunchKernelGGL((dequantize_kernel<decltype(kind)::value != 0, decltype(stream8)::value != 0>), grid, dim3(256), 0, s,
                        d_dst, ldd, d_values, d_exponents, ldv, rows, static_cast<int>(cols), static_cast<int>(wide));
   };
-  if (dst_f32) launch(Int<1>{}, Int<0>{});
-  else if (rows * cols * 2 > kStreamBytes) launch(Int<0>{}, Int<1>{});
+  if (f32) launch(Int<1>{}, Int<0>{});
+  else if (past) launch(Int<0>{}, Int<1>{});
   else launch(Int<0>{}, Int<0>{});
   return launched(who);
 }

@@ -157,16 +157,17 @@ struct Call {
     return {p, r.n, r.d, p.size(1)};
   }
 
-  Held quantize(const Rows& x, const Tensor& copy) const {
+  // next: 0, or TM_READ_NEXT where x is read again by what follows.
+  Held quantize(const Rows& x, const Tensor& copy, int next) const {
     const Held h = room_for(TM_HELD_E4M3, x.n, x.d, x.t);
-    check(a.quantize(bytes_of(h.values), bytes_of(h.exps), h.values.size(1), ptr(x.t), is_f32(x.t), x.ld, x.n, x.d,
+    check(a.quantize(bytes_of(h.values), bytes_of(h.exps), h.values.size(1), ptr(x.t), is_f32(x.t) | next, x.ld, x.n, x.d,
                      bf16_of(copy), copy.defined() ? copy.size(1) : 0, stream),
           "tm_quantize_e4m3");
     return h;
   }
 
-  void dequantize(const Tensor& out, i64 ld, const Held& h, i64 rows, i64 cols) const {
-    check(a.dequantize(ptr(out), is_f32(out), ld, bytes_of(h.values), bytes_of(h.exps), h.values.size(1), rows, cols,
+  void dequantize(const Tensor& out, i64 ld, const Held& h, i64 rows, i64 cols, int next) const {
+    check(a.dequantize(ptr(out), is_f32(out) | next, ld, bytes_of(h.values), bytes_of(h.exps), h.values.size(1), rows, cols,
                        stream),
           "tm_dequantize_e4m3");
   }
@@ -189,11 +190,11 @@ struct Call {
       return o;
     }
     if (fits(x)) {
-      *kept = quantize(x, {});
+      *kept = quantize(x, {}, TM_READ_NEXT);
       return x;
     }
     const Tensor copy = room(x.t, {x.n, up(x.d, 8)}, at::kBFloat16);
-    *kept = quantize(x, copy);
+    *kept = quantize(x, copy, 0);
     return {copy, x.n, x.d, copy.size(1)};
   }
 
@@ -205,7 +206,7 @@ struct Call {
     const i64 ld = up(cols, 8);
     Tensor p = room(h.values, {n, ld}, at::kBFloat16);
     if (ld != cols) p.narrow(1, cols, ld - cols).zero_();
-    dequantize(p, ld, h, n, cols);
+    dequantize(p, ld, h, n, cols, TM_READ_NEXT);
     return {p, n, cols, ld};
   }
 
@@ -451,7 +452,7 @@ py::tuple act_quantize(const Tensor& x, uintptr_t stream) {
   Held h;
   without_gil([&] {
     const Call c{abi(), reinterpret_cast<void*>(stream)};
-    h = c.quantize(rows_of(x), {});
+    h = c.quantize(rows_of(x), {}, 0);
   });
   return py::make_tuple(h.values, h.exps);
   END_HANDLE_TH_ERRORS_PYBIND
@@ -464,7 +465,7 @@ Tensor act_dequantize(const Tensor& values, const Tensor& exps, std::vector<i64>
     const Call c{abi(), reinterpret_cast<void*>(stream)};
     out = room(values, sizes, type_of(f32));
     const i64 cols = sizes.back();
-    if (out.numel()) c.dequantize(out, cols, {values, exps}, out.numel() / cols, cols);
+    if (out.numel()) c.dequantize(out, cols, {values, exps}, out.numel() / cols, cols, 0);
   });
   return out;
   END_HANDLE_TH_ERRORS_PYBIND
