@@ -77,3 +77,21 @@ def test_values_and_slopes(act, rows):
         bad = ~((got - want).abs() <= bound)
         assert not bad.any(), [(float(a), float(b), float(c), float(d)) for a, b, c, d in
                                zip(z[bad].double(), got[bad], want[bad], bound[bad])][:8]
+
+
+@pytest.mark.parametrize("largest", [448.0, 225.0, 224.5, 300.0])
+@pytest.mark.parametrize("e", [0, -30, 60])
+def test_8_bits_are_off_by_no_more_than_stated(largest, e):
+    """At most 2^-4 of the value, or 2^-10 of the block's power of two; zero from there down; and 2^-4 alone
+    is too little from 2^-13.8 of the block's largest on."""
+    x = torch.exp2(torch.linspace(-24, 0, 32 * 32).double()) * largest * torch.tensor([1.0, -1.0]).double().repeat(512)
+    x = (x * 2.0 ** e).float().reshape(32, 32)
+    assert float(x.abs().max()) == largest * 2.0 ** e
+    q = ta.quantize_activation(x.to(DEV))
+    assert int(q.exponents) == e + 127
+    off = (ta.dequantize_activation(q).cpu().double() - x.double()).abs()
+    size, power = x.double().abs(), 2.0 ** e
+    assert bool((off <= torch.maximum(2.0 ** -4 * size, torch.full_like(size, 2.0 ** -10 * power))).all())
+    assert bool((off == size)[size <= 2.0 ** -10 * power].all())
+    fine = size >= 2.0 ** -6 * power
+    assert bool((off <= 2.0 ** -4 * size)[fine].all()) and not bool((off <= 2.0 ** -4 * size)[~fine].all())

@@ -3,9 +3,9 @@
 //
 // The 8-bit format: e4m3 values (4 exponent bits, 3 of mantissa, largest 448, no infinities) and one
 // exponent byte e + 127 for each block of 32 rows x 32 columns. e is the least exponent with which
-// the block's largest finite magnitude is at most 448 2^e, clamped to [-117, 119], so that a value's
-// relative error is at most 2^-4 down to 2^-15 of the block's largest and every held value, v 2^e,
-// is a normal bf16 number or zero: reading back rounds nothing. (e4m3 is itself a floating format:
+// the block's largest finite magnitude is at most 448 2^e, clamped to [-117, 119]. A value is off by at most 2^-4
+// of itself where it is at least 2^-6 2^e (2^-13.8 of the block's largest, or less), else by at most 2^-10 2^e;
+// every held value, v 2^e, is a normal bf16 number or zero: reading back rounds nothing. (e4m3 is itself a floating format:
 // a block's scale sets its range, not its step. A square block keeps that scale the same along rows
 // and columns, so a product may contract either, and costs 1 byte in 1024.) Values past 448 2^119
 // (over 2.98e38) are held as that, infinities and NaN as NaN.
