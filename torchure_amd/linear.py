@@ -7,7 +7,9 @@
   the two above keep what they need for the backward pass when called with ``checkpoint="e4m3"``.
 
 The products are this package's bf16 MFMA GEMMs (``tm_lin``) with fp32 accumulation; bias, activation,
-residual, the gate and its gradient, and the 8-bit form of what is kept are done on the accumulators.
+residual, the gate and its gradient, and the 8-bit form of what is kept are done on the accumulators. What
+a product reads is rounded to bf16 first, as autocast and a bf16 module's autograd do: fp32 operands, the
+gated result, and in the backward pass the gradients of the pre-activation, gate and up.
 As in the trainer (torchure/train/trainer.py:374), hidden states are bf16, or fp32 under bf16 autocast;
 weights are bf16, or fp32 masters of which the bf16 working copy is read where it is current.
 """
@@ -216,8 +218,11 @@ def fused_linear(
     ``activation``: None or "none", "relu", "silu", "gelu" or "gelu_tanh". ``checkpoint``: how the input (for
     the weight's gradient) and the pre-activation (for all of them) are kept until the backward
     pass: None for bf16, "e4m3" for 8 bits (``quantize_activation``'s form): half the bytes, and
-    gradients made from what is kept. The forward result is the same. Gradients have their tensors'
-    types; what no gradient needs is neither kept nor computed. Differentiable once, in reverse mode."""
+    gradients made from what is kept (of an fp32 x its fp32 values in 8 bits). The forward result is the same.
+
+    The gradient of the pre-activation (without an activation an fp32 result's gradient itself) is rounded to
+    bf16 for the products that make x's and the weight's gradients from it, whatever their types, and not for
+    the bias's. Gradients have their tensors' types; what no gradient needs is neither kept nor computed. Differentiable once, in reverse mode."""
     host = _native.lin_host()
     act, kind = _ACTS.get(activation), _HELD.get(checkpoint)
     if act is None or kind is None or torch.is_autocast_enabled("cuda") or not x.is_cuda or not host.lin_plain(
@@ -286,7 +291,8 @@ def swiglu_mlp(
     (``quantize_activation``'s form); the gated result is made from them again, where an
     ordinary module keeps it too. The backward pass applies the gate's gradient on the sums of its first
     product, whose two results, of gate and up, are made together where either's weight or x wants a
-    gradient. Gradients have their tensors' types; what else no gradient needs is neither kept nor computed.
+    gradient; both are rounded to bf16 for the products behind them, as is an fp32 result's gradient for
+    the first. Gradients have their tensors' types; what else no gradient needs is neither kept nor computed.
     Differentiable once, in reverse mode."""
     host = _native.lin_host()
     kind = _HELD.get(checkpoint)
