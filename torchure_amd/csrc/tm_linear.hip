@@ -32,7 +32,7 @@
 // split over K: fp32 partial tiles in the workspace, added in order by lin_finish_kernel, which then does what
 // the unsplit tiles' end does.
 //
-// Measured (one MI355X, 8192 rows): 8192 -> 8192 805-840 us, 1.31-1.37 PFLOP/s; 9728 -> 2560 with residual 350 us, 1.17;
+// Measured (one MI355X, 8192 rows): 8192 -> 8192 805-840 us, 1.31-1.37 PFLOP/s; 9728 -> 2560 with residual 323-335 us, 1.22-1.26;
 // 2560 -> 9728 with silu, bias and 8-bit z 386 us, 1.06; the gate 2560 -> 9728 690-720 us, 1.13-1.18; its gradient 540 us
 // from bf16, 480 from 8 bits; grad_x of both its products 647 us, 1.26; their grad_w 666 us, 1.23. MFMA busy
 // is 62-71% of a launch (39% of the gate's gradient); the rest is ends and first loads.
@@ -1165,9 +1165,9 @@ constexpr int64_t kPad = 64;  // [d0 | d1]: each half is padded to a multiple of
 constexpr int64_t kMaxPartialBytes = int64_t(2) << 30;
 // Measured on MI355X: microseconds of a slice and of a tile's end, by tile, fitted to a sweep of 15 tilings and
 // splits of 22 products (the block's forward, gradient and weight-gradient products at 8192 rows and some of
-// 1999 rows; 8192 x 9728 -> 2560, 320 tiles of 256 x 256: 366 us with 256 of them whole and the others in
-// four parts, 417 unsplit, 390 in tiles of 192 x 256). With them the choice took at most 3% more time than
-// the best of the 15. The ends of a round of tiles come together and are bound by memory: the gate's, by
+// 1999 rows), before the ends got their present form: of 8192 x 9728 -> 2560's 320 tiles of 256 x 256, 256 whole and the
+// others in four parts took 366 us then, 417 unsplit, 390 in tiles of 192 x 256. The choice takes at most 2-3%
+// more time than the best of the 15, then and on 28 products with the present ends. The ends of a round of tiles come together and are bound by memory: the gate's, by
 // what they read and write more.
 struct Cost {
   int mb, nb;

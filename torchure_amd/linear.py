@@ -222,7 +222,8 @@ def fused_linear(
 
     The gradient of the pre-activation (without an activation an fp32 result's gradient itself) is rounded to
     bf16 for the products that make x's and the weight's gradients from it, whatever their types, and not for
-    the bias's. Gradients have their tensors' types; what no gradient needs is neither kept nor computed. Differentiable once, in reverse mode."""
+    the bias's. Gradients have their tensors' types; what no gradient needs is neither kept nor computed.
+    Differentiable once, in reverse mode."""
     host = _native.lin_host()
     act, kind = _ACTS.get(activation), _HELD.get(checkpoint)
     if act is None or kind is None or torch.is_autocast_enabled("cuda") or not x.is_cuda or not host.lin_plain(
