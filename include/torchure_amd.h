@@ -514,6 +514,28 @@ size_t tm_lin_workspace_bytes(int op, int64_t rows, int64_t inp, int64_t out, in
 int tm_lin(const tm_lin_t* h_desc, void* d_ws, size_t ws_bytes, void* stream);
 
 /*
+ * The AdamW step on moments held in 8 bits. A record's exp_avg and exp_avg_sq then point to bytes, tm_moments8_bytes(numel)
+ * of them each, at any alignment: a code for each element up to numel's next multiple of 256 (zero past numel), then a byte for each block of
+ * 64 elements. exp_avg: e4m3 values times 2^(byte - 127). exp_avg_sq: its root, n(c) 2^(byte - 145), n(c) = c below 16, else
+ * (16 + c % 16) 2^(c / 16 - 1), 255 NaN. All bytes zero but for 10 and 40 in the blocks' bytes is a fresh state of zeros
+ * (all zero is too). The other fields, tables, groups and the workspace (tm_workspace_bytes) are tm_adamw_step's;
+ * masters, grads and copies need their elements' alignment only.
+ *   tm_adamw8_step     step += 1, the update in fp32 from what is held, and the new moments held again: rounded up or down by a
+ *                      hash of seed, step and element, so that the mean is kept. Infinite and NaN moments are held as NaN.
+ *   tm_moments8_read   master[] = exp_avg's values and grad[] = the root's, as bf16 (exact), or, with TM_GRAD_F32 in a record's
+ *                      flags, exp_avg's and exp_avg_sq's (the root's square) as fp32.
+ *   tm_moments8_write  holds the fp32 values at master (exp_avg) and grad (exp_avg_sq), to the nearest.
+ */
+int64_t tm_moments8_bytes(int64_t numel);
+int tm_adamw8_step(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk_t* d_chunks, int64_t n_chunks,
+                   int64_t chunk_elems, const tm_hyper_t* h_groups, int32_t n_groups, const float* d_coef, uint64_t seed,
+                   void* d_ws, void* stream);
+int tm_moments8_read(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk_t* d_chunks, int64_t n_chunks,
+                     int64_t chunk_elems, void* stream);
+int tm_moments8_write(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk_t* d_chunks, int64_t n_chunks,
+                      int64_t chunk_elems, void* stream);
+
+/*
  * Activations held in 8 bits between forward and backward: e4m3 values (rows ldv apart, ldv = cols' next
  * multiple of 32, padding zero, 16-byte aligned) and for each block of 32 rows x 32 columns the byte
  * e + 127 (ceil(rows / 32) x ceil(cols / 32)): e the least exponent with which the block's largest

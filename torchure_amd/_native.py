@@ -109,6 +109,13 @@ _SIGNATURES = {
         ctypes.c_int,
         [_vp, _i64, _vp, _i64, _i64, ctypes.POINTER(TmHyper), ctypes.c_int32, _vp, _vp],
     ),
+    "tm_moments8_bytes": (_i64, [_i64]),
+    "tm_adamw8_step": (
+        ctypes.c_int,
+        [_vp, _i64, _vp, _i64, _i64, ctypes.POINTER(TmHyper), ctypes.c_int32, _vp, ctypes.c_uint64, _vp, _vp],
+    ),
+    "tm_moments8_read": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _vp]),
+    "tm_moments8_write": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _vp]),
     "tm_accum_norm_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "tm_grad_accumulate_list": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, ctypes.c_int, _vp, ctypes.c_size_t, _vp, _vp]),
     "tm_clip_coef": (ctypes.c_int, [_vp, ctypes.c_float, _vp, _vp]),

@@ -55,6 +55,22 @@ int tm_internal_fail(int code, const char* fmt, ...) {
   return code;
 }
 
+int tm_internal_check_table(const void* d_tensors, int64_t n_tensors, const void* d_chunks, int64_t n_chunks,
+                            int64_t chunk_elems, const char* who) {
+  if (n_tensors < 0 || n_chunks < 0) return tm_internal_fail(TM_EINVAL, "%s: negative size", who);
+  if (n_tensors > 0 && !d_tensors) return tm_internal_fail(TM_EINVAL, "%s: null tensor table", who);
+  if (n_chunks > 0 && !d_chunks) return tm_internal_fail(TM_EINVAL, "%s: null chunk table", who);
+  if (n_tensors > 0xFFFFFFFFll) return tm_internal_fail(TM_EINVAL, "%s: too many tensors", who);
+  // Chunk indices are 32-bit; launches are split to stay under 2^32 work-items each.
+  if (n_chunks > 0xFFFFFFFFll)
+    return tm_internal_fail(TM_EINVAL, "%s: %lld chunks, at most %lld (use larger chunks)", who,
+                            (long long)n_chunks, 0xFFFFFFFFll);
+  if (chunk_elems <= 0 || chunk_elems % TM_CHUNK_ALIGN != 0 || chunk_elems > (int64_t(1) << 30))
+    return tm_internal_fail(TM_EINVAL, "%s: chunk_elems %lld must be a positive multiple of %d, <= 2^30", who,
+                            (long long)chunk_elems, TM_CHUNK_ALIGN);
+  return TM_OK;
+}
+
 namespace {
 
 constexpr int kThreads = 256;  // 4 wave64 per block
@@ -1012,26 +1028,10 @@ int launch_chunk_slices(int64_t n_chunks, int64_t chunk_elems, const char* what,
   return TM_OK;
 }
 
-int check_table(const void* d_tensors, int64_t n_tensors, const void* d_chunks, int64_t n_chunks,
-                int64_t chunk_elems, const char* who) {
-  if (n_tensors < 0 || n_chunks < 0) return fail(TM_EINVAL, "%s: negative size", who);
-  if (n_tensors > 0 && !d_tensors) return fail(TM_EINVAL, "%s: null tensor table", who);
-  if (n_chunks > 0 && !d_chunks) return fail(TM_EINVAL, "%s: null chunk table", who);
-  if (n_tensors > 0xFFFFFFFFll) return fail(TM_EINVAL, "%s: too many tensors", who);
-  // Chunk indices are 32-bit; launches are split to stay under 2^32 work-items each.
-  if (n_chunks > 0xFFFFFFFFll)
-    return fail(TM_EINVAL, "%s: %lld chunks, at most %lld (use larger chunks)", who,
-                (long long)n_chunks, 0xFFFFFFFFll);
-  if (chunk_elems <= 0 || chunk_elems % TM_CHUNK_ALIGN != 0 || chunk_elems > (int64_t(1) << 30))
-    return fail(TM_EINVAL, "%s: chunk_elems %lld must be a positive multiple of %d, <= 2^30", who,
-                (long long)chunk_elems, TM_CHUNK_ALIGN);
-  return TM_OK;
-}
-
 int check_step_args(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk_t* d_chunks,
                     int64_t n_chunks, int64_t chunk_elems, const tm_hyper_t* h_groups, int32_t n_groups,
                     const char* who) {
-  int rc = check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, who);
+  int rc = tm_internal_check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, who);
   if (rc) return rc;
   if (n_groups < 1 || n_groups > TM_MAX_GROUPS || !h_groups)
     return fail(TM_EINVAL, "%s: n_groups %d outside 1..%d", who, n_groups, TM_MAX_GROUPS);
@@ -1163,7 +1163,7 @@ int64_t tm_fill_chunks(const int64_t* h_numels, int64_t n_tensors, int64_t chunk
 int tm_grad_norm(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk_t* d_chunks,
                  int64_t n_chunks, int64_t chunk_elems, float max_norm, int clip, void* d_ws,
                  float* d_norm, float* d_coef, void* stream) {
-  int rc = check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, "tm_grad_norm");
+  int rc = tm_internal_check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, "tm_grad_norm");
   if (rc) return rc;
   if (!d_ws || !d_norm) return fail(TM_EINVAL, "tm_grad_norm: null workspace or norm output");
   if (clip && !d_coef) return fail(TM_EINVAL, "tm_grad_norm: clip requested with null coef output");
@@ -1179,7 +1179,7 @@ int tm_grad_norm(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk
 
 int tm_grad_scale(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk_t* d_chunks,
                   int64_t n_chunks, int64_t chunk_elems, const float* d_coef, void* stream) {
-  int rc = check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, "tm_grad_scale");
+  int rc = tm_internal_check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, "tm_grad_scale");
   if (rc) return rc;
   if (!d_coef) return fail(TM_EINVAL, "tm_grad_scale: null coef");
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -1232,7 +1232,7 @@ size_t tm_accum_norm_workspace_bytes(int64_t n_chunks, int64_t chunk_elems) {
 int tm_grad_accumulate_list(const tm_accum_t* d_list, int64_t n_list, const tm_chunk_t* d_chunks,
                             int64_t n_chunks, int64_t chunk_elems, int with_norm, void* d_ws, size_t ws_bytes,
                             float* d_norm, void* stream) {
-  int rc = check_table(d_list, n_list, d_chunks, n_chunks, chunk_elems, "tm_grad_accumulate_list");
+  int rc = tm_internal_check_table(d_list, n_list, d_chunks, n_chunks, chunk_elems, "tm_grad_accumulate_list");
   if (rc) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (with_norm) {
@@ -1310,7 +1310,7 @@ int tm_stream_copy(void* d_dst, const void* d_src, int64_t nbytes, void* stream)
 
 int tm_cast_bf16_list(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk_t* d_chunks,
                       int64_t n_chunks, int64_t chunk_elems, void* stream) {
-  int rc = check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, "tm_cast_bf16_list");
+  int rc = tm_internal_check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, "tm_cast_bf16_list");
   if (rc) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return launch_chunk_slices(n_chunks, chunk_elems, "cast_bf16_list_kernel",

@@ -28,6 +28,13 @@ Mixed precision: masters are the fp32 ``nn.Parameter``s, as in the reference
 (``torchure_amd.optimizer.working``); when its own ``.grad`` is None the bf16
 grad of the working copy is consumed, and the working copy is refreshed with
 RNE(master) after the update.
+
+With ``state_bits=8`` the two moments are held in 8 bits (``tm_adamw8_step``: e4m3 for exp_avg, the
+root of exp_avg_sq in 4 + 4 bits, a power of two for each 64 elements, rounded by random bits so
+that the mean is kept): 2.03 instead of 8 bytes of state a param, 16.06 instead of 28 bytes moved by
+a step. Everything else is as above; ``exp_avg`` and ``exp_avg_sq`` are then byte tensors, which
+only this class reads (``flat_moments`` gives their values), and checkpoints of either width load
+into both.
 """
 
 from __future__ import annotations
@@ -109,7 +116,13 @@ class AdamW(torch.optim.Optimizer):
         fused: bool | None = None,
         chunk_elems: int = tables.DEFAULT_CHUNK_ELEMS,
         defer_clip: bool = True,
+        state_bits: int = 32,
+        seed: int = 0,
     ) -> None:
+        """torch.optim.AdamW's parameters; ``chunk_elems`` and ``defer_clip`` as in the module's text.
+        ``state_bits``: 32 or 8, how the moments are held. ``seed`` (0 to 2^64 - 1) sets the random bits that
+        8-bit moments are rounded by; it is the program's to keep, as are lr and betas: a run that goes on from a
+        checkpoint with the same seed goes on as it would have."""
         if isinstance(lr, torch.Tensor) or any(isinstance(b, torch.Tensor) for b in betas):
             raise NotImplementedError("torchure_amd.AdamW: tensor lr/betas are not supported")
         if not 0.0 <= lr:
@@ -147,10 +160,17 @@ class AdamW(torch.optim.Optimizer):
             "fused": True,
             "decoupled_weight_decay": True,
         }
+        if state_bits not in (8, 32):
+            raise ValueError(f"torchure_amd.AdamW: state_bits must be 32 or 8, got {state_bits!r}")
+        if not 0 <= int(seed) < 1 << 64:
+            raise ValueError(f"torchure_amd.AdamW: seed must be in [0, 2^64), got {seed}")
         self.chunk_elems = tables.check_chunk_elems(chunk_elems)
         self.defer_clip = bool(defer_clip)
+        self.state_bits = int(state_bits)
+        self.seed = int(seed)
         self._pending = None  # (coef device tensor, _ClipRecord)
         self._uploader = tables.TableUploader()
+        self._uploader_read = tables.TableUploader()  # flat_moments' tables
         self._verified: dict = {}  # id(param) -> _ParamEntry
         self._plan = None  # _Plan of the last full step, reused while nothing changes
         super().__init__(params, defaults)
@@ -177,6 +197,8 @@ class AdamW(torch.optim.Optimizer):
         state = super().__getstate__()
         state["chunk_elems"] = self.chunk_elems
         state["defer_clip"] = self.defer_clip
+        state["state_bits"] = self.state_bits
+        state["seed"] = self.seed
         return state
 
     def __setstate__(self, state):
@@ -186,8 +208,11 @@ class AdamW(torch.optim.Optimizer):
             self._mark_owned(group["params"])
         self.__dict__.setdefault("chunk_elems", tables.DEFAULT_CHUNK_ELEMS)
         self.__dict__.setdefault("defer_clip", True)
+        self.__dict__.setdefault("state_bits", 32)
+        self.__dict__.setdefault("seed", 0)
         self.__dict__.setdefault("_pending", None)
         self.__dict__.setdefault("_uploader", tables.TableUploader())
+        self.__dict__.setdefault("_uploader_read", tables.TableUploader())
         self.__dict__.setdefault("_verified", {})
         self.__dict__.setdefault("_plan", None)
 
@@ -396,7 +421,11 @@ class AdamW(torch.optim.Optimizer):
         tables.make_ready(plan.chunks, device)
         return [StepLaunch(device, self._uploader(rows, device), plan.n, plan.chunks, plan.n_chunks,
                            self.chunk_elems, _native.hyper_array(hyper), len(hyper), coef,
-                           plan.written, (plan.wparams, plan.wworks))]
+                           plan.written, (plan.wparams, plan.wworks), self._held_seed())]
+
+    def _held_seed(self):
+        """The seed of a step on 8-bit moments, None with 32 bits."""
+        return self.seed if self.state_bits == 8 else None
 
     @torch.no_grad()
     def init_state(self) -> None:
@@ -425,7 +454,8 @@ class AdamW(torch.optim.Optimizer):
                     fresh.append(p)  # anything else is refused, precisely, by _verify_param
         if fresh:
             with torch.no_grad():
-                for p, m, v in pooled_moments(fresh, zero=True):
+                pooled = pooled_held_moments if self.state_bits == 8 else pooled_moments
+                for p, m, v in pooled(fresh, zero=True):
                     state_map[p] = {"step": torch.zeros((), dtype=torch.float32, device=p.device),
                                     "exp_avg": m, "exp_avg_sq": v}
 
@@ -443,12 +473,18 @@ class AdamW(torch.optim.Optimizer):
                 raise RuntimeError(f"{who}: working copy must be bf16 of the param's size and device")
         if len(state) == 0:
             state["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
-            state["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
-            state["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+            if self.state_bits == 8:
+                (_, state["exp_avg"], state["exp_avg_sq"]), = pooled_held_moments([p])
+            else:
+                state["exp_avg"] = torch.zeros_like(p, memory_format=torch.preserve_format)
+                state["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
         else:
             st = state["step"]
             if st.device != p.device or st.dtype != torch.float32:
                 state["step"] = st.to(dtype=torch.float32, device=p.device)
+            if self.state_bits == 8 or state["exp_avg"].dtype == torch.uint8:
+                state["exp_avg"], state["exp_avg_sq"] = self._as_held(p, state["exp_avg"], state["exp_avg_sq"])
+                return _ParamEntry(p, work, state["step"], state["exp_avg"], state["exp_avg_sq"])
             for k in ("exp_avg", "exp_avg_sq"):
                 t = state[k]
                 if t.numel() != p.numel():
@@ -472,9 +508,30 @@ class AdamW(torch.optim.Optimizer):
             group["foreach"] = None
         self._repack_states()
 
+    def _as_held(self, p: torch.Tensor, m: torch.Tensor, v: torch.Tensor):
+        """``p``'s moments as this optimizer holds them, from either width."""
+        who, size = "torchure_amd.AdamW", held_bytes(p.numel())
+        both = (m, v)
+        held = all(t.numel() == size and t.dtype == torch.uint8 for t in both)
+        if not held and not all(t.numel() == p.numel() and t.is_floating_point() for t in both):
+            raise RuntimeError(f"{who}: the moments of a param of {p.numel()} elements have {m.numel()} and {v.numel()} "
+                               f"elements of {m.dtype} and {v.dtype}")
+        if held == (self.state_bits == 8):
+            return tuple(t.to(dtype=torch.uint8 if held else torch.float32, device=p.device).contiguous() for t in both)
+        if held:
+            out = [torch.empty_like(p, memory_format=torch.contiguous_format).detach() for _ in both]
+            _convert_moments("tm_moments8_read", [(t.to(p.device).contiguous(), o) for t, o in zip(both, out)], p)
+            return tuple(out)
+        (_, *out), = pooled_held_moments([p])
+        wide = [t.to(dtype=torch.float32, device=p.device).contiguous() for t in both]
+        _convert_moments("tm_moments8_write", list(zip(out, wide)), p)
+        return tuple(out)
+
     def _repack_states(self) -> None:
         """Moments loaded from a checkpoint (separate tensors, or views of a loaded storage)
-        are copied into this optimizer's pooled layout, as if created by its first step."""
+        are copied into this optimizer's pooled layout, as if created by its first step; those of the other width
+        are converted. (torch's loader casts byte moments to the param's fp32: whole numbers up to 255,
+        cast back here.)"""
         held = []
         for group in self.param_groups:
             for p in group["params"]:
@@ -482,17 +539,54 @@ class AdamW(torch.optim.Optimizer):
                 if not st or not (p.is_cuda and p.dtype == torch.float32 and p.is_contiguous()):
                     continue
                 m, v = st.get("exp_avg"), st.get("exp_avg_sq")
-                if (isinstance(m, torch.Tensor) and isinstance(v, torch.Tensor) and m.numel() == p.numel()
-                        and v.numel() == p.numel() and m.dtype == v.dtype == torch.float32
-                        and m.device == v.device == p.device):
-                    held.append((p, st, m, v))
+                if not (isinstance(m, torch.Tensor) and isinstance(v, torch.Tensor)):
+                    continue
+                size = held_bytes(p.numel())
+                if p.numel() and m.numel() == size and v.numel() == size:
+                    m, v = (t.to(dtype=torch.uint8, device=p.device) for t in (m, v))
+                elif not (m.numel() == p.numel() and v.numel() == p.numel() and m.dtype == v.dtype == torch.float32
+                          and m.device == v.device == p.device):
+                    continue
+                if self.state_bits == 8 or m.dtype == torch.uint8:
+                    m, v = self._as_held(p, m, v)
+                held.append((p, st, m, v))
         if not held:
             return
+        pooled = pooled_held_moments if self.state_bits == 8 else pooled_moments
         with torch.no_grad():
-            for (p, st, m, v), (_, pm, pv) in zip(held, pooled_moments([h[0] for h in held], zero=False)):
+            for (p, st, m, v), (_, pm, pv) in zip(held, pooled([h[0] for h in held], zero=False)):
                 pm.copy_(m.reshape(pm.shape))
                 pv.copy_(v.reshape(pv.shape))
                 st["exp_avg"], st["exp_avg_sq"] = pm, pv
+
+    @torch.no_grad()
+    def flat_moments(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """What 8-bit moments stand for: exp_avg and the root of exp_avg_sq (which is what is held of it) of
+        all params that have state, one after the other in the groups' order, as two bf16 vectors, exactly."""
+        who = "torchure_amd.AdamW.flat_moments"
+        if self.state_bits != 8:
+            raise RuntimeError(f"{who}: the moments of an optimizer with state_bits=32 are its state's own tensors")
+        params = [p for group in self.param_groups for p in group["params"] if self.state.get(p)]
+        if not params:
+            raise RuntimeError(f"{who}: no param has state yet")
+        device = params[0].device
+        if any(p.device != device for p in params):
+            raise RuntimeError(f"{who}: params on several devices")
+        for p in params:
+            st = self.state[p]
+            if st["exp_avg"].dtype != torch.uint8 or st["exp_avg"].device != device or not st["exp_avg"].is_contiguous():
+                self._verify_param(p, st, getattr(p, "_tm_working", None))
+        numels = np.array([p.numel() for p in params], dtype=np.int64)
+        total = int(numels.sum())
+        m, r = (torch.empty(total, dtype=torch.bfloat16, device=device) for _ in range(2))
+        rows = np.zeros(len(params), dtype=_native.TENSOR_DTYPE)
+        at = 2 * (np.cumsum(numels) - numels).astype(np.uint64)
+        rows["master"], rows["grad"] = at + np.uint64(m.data_ptr()), at + np.uint64(r.data_ptr())
+        rows["numel"] = numels
+        for k in ("exp_avg", "exp_avg_sq"):
+            rows[k] = [self.state[p][k].data_ptr() for p in params]
+        _launch_moments("tm_moments8_read", rows, device, self._uploader_read)
+        return m, r
 
     def _plan_launches(self, per_dev, hyper, coef) -> list["StepLaunch"]:
         groups_c = _native.hyper_array(hyper)
@@ -505,7 +599,7 @@ class AdamW(torch.optim.Optimizer):
             chunks, n_chunks = tables.CHUNKS.get(rows["numel"], self.chunk_elems, device)
             launch = StepLaunch(device, self._uploader(rows, device), n, chunks, n_chunks,
                                 self.chunk_elems, groups_c, len(hyper), coef, written,
-                                ([e.param for e in pairs], [e.work for e in pairs]))
+                                ([e.param for e in pairs], [e.work for e in pairs]), self._held_seed())
             launch.host_rows = rows.tobytes()
             out.append(launch)
         return out
@@ -619,7 +713,8 @@ class _Plan:
 
 
 class StepLaunch:
-    """One ``tm_adamw_step`` call with its device tables kept alive.
+    """One ``tm_adamw_step`` call (with a ``seed``: ``tm_adamw8_step``, on 8-bit moments) with its device tables
+    kept alive.
 
     Calling it enqueues the prep + update kernels on the device's current
     stream. Calling it again re-applies one more AdamW step to the same
@@ -629,7 +724,8 @@ class StepLaunch:
     """
 
     def __init__(self, device, d_rows, n, chunks, n_chunks, chunk_elems, groups_c, n_groups, coef,
-                 written=(), pairs=((), ())):
+                 written=(), pairs=((), ()), seed=None):
+        self.seed = seed
         self.written = written if isinstance(written, list) else list(written)
         # the masters with a working copy, and those copies
         self.pair_params, self.pair_works = (x if isinstance(x, list) else list(x) for x in pairs)
@@ -648,7 +744,8 @@ class StepLaunch:
 
     def __call__(self) -> None:
         tables.follow_home_stream(self.home, self.device, (self.d_rows, self.chunks, self.ws))
-        rc = _native.lib().tm_adamw_step(
+        name = "tm_adamw_step" if self.seed is None else "tm_adamw8_step"
+        rc = getattr(_native.lib(), name)(
             self.d_rows.data_ptr(),
             self.n,
             self.chunks.data_ptr(),
@@ -657,10 +754,11 @@ class StepLaunch:
             self.groups_c,
             self.n_groups,
             self.coef.data_ptr() if self.coef is not None else None,
+            *(() if self.seed is None else (self.seed,)),
             self.ws.data_ptr(),
             _native.stream_handle(self.device),
         )
-        _native.check(rc, "tm_adamw_step")
+        _native.check(rc, name)
         if self.written:
             _native.host().bump(self.written)
         if self.pair_params:  # the copies now hold RNE(master) as of the versions after the bump
@@ -755,8 +853,52 @@ def pooled_moments(params, zero: bool = True):
     return [(p, *out[id(p)]) for p in params]
 
 
+def held_bytes(numel: int) -> int:
+    """Bytes of one 8-bit moment of ``numel`` elements: a code each up to the next multiple of 256, and an exponent
+    for each 64 of those."""
+    codes = -(-numel // 256) * 256
+    return codes + codes // 64
+
+
+def pooled_held_moments(params, zero: bool = True):
+    """``pooled_moments`` for 8-bit moments: (param, exp_avg, exp_avg_sq), byte vectors in one pool per role and device,
+    each from a multiple of 256 bytes."""
+    per_dev: dict = {}
+    for p in params:
+        per_dev.setdefault(p.device, []).append(p)
+    out = {}
+    for device, ps in per_dev.items():
+        sizes = [held_bytes(p.numel()) for p in ps]
+        offs = np.cumsum([0] + [-(-n // 256) * 256 for n in sizes]).tolist()
+        make = torch.zeros if zero else torch.empty
+        pools = [make(max(offs[-1], 1), dtype=torch.uint8, device=device) for _ in range(2)]
+        for p, o, n in zip(ps, offs, sizes):
+            out[id(p)] = tuple(pool[o: o + n] for pool in pools)
+    return [(p, *out[id(p)]) for p in params]
+
+
+def _launch_moments(name: str, rows, device, upload) -> None:
+    if not int(rows["numel"].sum()):
+        return
+    with torch.cuda.device(device):
+        chunks, n_chunks = tables.CHUNKS.get(rows["numel"], tables.DEFAULT_CHUNK_ELEMS, device)
+        d_rows = upload(rows, device)
+        rc = getattr(_native.lib(), name)(d_rows.data_ptr(), len(rows), chunks.data_ptr(), n_chunks,
+                                          tables.DEFAULT_CHUNK_ELEMS, _native.stream_handle(device))
+    _native.check(rc, name)
+
+
+def _convert_moments(name: str, pairs, p: torch.Tensor) -> None:
+    """One param's moments between their bytes and fp32: ``pairs`` is ((bytes, values) of exp_avg, of exp_avg_sq)."""
+    (mb, mv), (vb, vv) = pairs
+    rows = np.zeros(1, dtype=_native.TENSOR_DTYPE)
+    rows["exp_avg"], rows["exp_avg_sq"], rows["master"], rows["grad"] = (t.data_ptr() for t in (mb, vb, mv, vv))
+    rows["numel"], rows["flags"] = p.numel(), _native.TM_GRAD_F32
+    _launch_moments(name, rows, p.device, tables.upload)
+
+
 def step_bytes_per_param(grad_bytes: int, with_norm: bool = True, with_bf16_out: bool = True) -> int:
-    """Algorithmic HBM bytes per parameter of one step (norm pass + update)."""
+    """Algorithmic HBM bytes per parameter of one step (norm pass + update) on 32-bit moments."""
     upd = grad_bytes + 3 * 4 + 3 * 4 + (2 if with_bf16_out else 0)
     return upd + (grad_bytes if with_norm else 0)
 
