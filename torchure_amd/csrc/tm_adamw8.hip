@@ -12,8 +12,13 @@
 // 5e-4 of itself). Rounded up with the probability of the part that lies above, what is held has the right mean.
 // The random bits are a hash of (seed, step, element): the same run gives the same bits, on any launch shape.
 //
-// Arithmetic is fp32 (the 32-bit step's is fp64, to the bit of torch's): errors of 1e-7 beside a held moment's 2^-4. The step uses the
-// moments before they are rounded.
+// The new moments are summed in fp64 as in the 32-bit step and rounded to fp32 once (fp64 costs the step nothing, 5.95 TB/s
+// either way; sums in fp32 turned three times as many of the roundings the other way); the rest is fp32. The step uses the moments
+// before they are held again.
+//
+// Bound by memory: 16.06 bytes a param with bf16 grads and copies (28 with 32-bit moments). The codes were computed with per-value
+// tests, selects and e4m3 conversions first, 300 vector instructions a wave, which bound the step at 5.5 TB/s; as float's own denormals
+// (below) it runs at 5.95, in-order streams of 256 to 1024 bytes a wave.
 
 #include <hip/hip_runtime.h>
 
@@ -48,13 +53,20 @@ constexpr int kThreads = 256;
 constexpr int kWave = 64;
 constexpr int kSlice = kWave * 4;  // elements a wave takes at a time: four blocks, 16 lanes each
 constexpr int kBlock = 64;
+// Slices to a wave: the step's eight streams are fastest with one (5.95 TB/s over 2e9 elements, 5.75 with two, 5.95
+// with four and twice the registers; a cap on the waves of a CU, as the 32-bit step has, only loses), reading
+// the moments' two streams in and two out with two (6.16 TB/s, one 5.6, four 5.6).
+constexpr int kStepSlices = 1, kReadSlices = 2;
+static_assert(TM_CHUNK_ALIGN % (kSlice * kStepSlices) == 0 && TM_CHUNK_ALIGN % (kSlice * kReadSlices) == 0, "whole pieces to a chunk");
 constexpr int kRootLow = 40;  // the least byte of a root's exponent
 
-// Global-address-space accesses, past the caches: every byte is touched once.
+// Global-address-space accesses, past the caches: every byte is touched once. (Cached loads or stores in the step: 5.5 TB/s;
+// the codes that moments8_kernel reads alone are faster through them, 6.16 TB/s for 5.85.)
 #define TM_GLOBAL __attribute__((address_space(1)))
-template <typename T>
+template <typename T, bool kCached = false>
 __device__ __forceinline__ T ld(const void* p) {
-  return __builtin_nontemporal_load((const TM_GLOBAL T*)p);
+  if constexpr (kCached) return *(const TM_GLOBAL T*)p;
+  else return __builtin_nontemporal_load((const TM_GLOBAL T*)p);
 }
 template <typename T, typename V>
 __device__ __forceinline__ void st(void* p, V v) {
@@ -80,32 +92,35 @@ __device__ __forceinline__ uint32_t element_bits(uint32_t z) {
 }
 
 // ---------------------------------------------------------------- the two formats
+//
+// Both are the top bits of a float that is scaled so that the format's smallest normal number is float's own, 2^-126:
+// below, float's denormals have the format's constant step. A code is then (bits + random bits below the last place) >> the
+// places left out, and a value the float of the shifted code, scaled back. (ldexp: the scales pass 2^127.)
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7FFFFFFFu) < 0x7F800000u; }
 
-// m / 2^e to a whole number of e4m3 steps, up where the part above the lower one plus u is at least 1, u = (low 16
-// of `bits` + 1/2) / 2^16. Below 2^-6 the step is 2^-9: adding 2^-6 puts the value into the binade of that step.
-__device__ __forceinline__ float hold_m(float m, float inv, uint32_t bits) {
-  const float y = m * inv, size = fminf(fabsf(y), 448.0f), base = size < 0x1p-6f ? 0x1p-6f : 0.0f;
-  const uint32_t up = __float_as_uint(size + base) + ((bits & 0xFFFFu) * 16u + 8u);
-  const float held = __uint_as_float(up & 0xFFF00000u) - base;
-  return finite(m) ? copysignf(held, y) : __uint_as_float(0x7FC00000u);
-}
+// e4m3: 2^-6 2^e -> 2^-126. Root: 16 2^x -> 2^-126, x = byte - 145.
+__device__ __forceinline__ float scale_m(float m, uint32_t me) { return ldexpf(m, 7 - static_cast<int>(me)); }
+__device__ __forceinline__ float scale_root(float r, uint32_t re) { return ldexpf(r, 15 - static_cast<int>(re)); }
 
-// `k`: the exponent's byte. Numbers from 16 2^x on are floats whose top bits are the code; below, adding 16 2^x makes
-// them so.
-__device__ __forceinline__ uint32_t root_base(uint32_t k) { return (k - 15u) << 23; }
-__device__ __forceinline__ uint32_t hold_root(float r, uint32_t k, uint32_t bits) {
-  const uint32_t high = root_base(k), low = high + (1u << 23);
-  const bool small = r < __uint_as_float(low);
-  const uint32_t up = __float_as_uint(small ? r + __uint_as_float(low) : r) + ((bits >> 16) * 8u + 4u);
-  const uint32_t c = (up >> 19) - ((small ? low : high) >> 19);
-  return !finite(r) ? 255u : max(c, r > 0.0f ? 1u : 0u);
+// Up where the part above the lower code plus u is at least 1, u = (16 random bits + 1/2) / 2^16; m's are the low
+// ones of `bits`, a root's the high ones. kAny: values that are infinite, NaN or past what can be held.
+template <bool kAny>
+__device__ __forceinline__ uint32_t hold_m(float m, uint32_t me, uint32_t bits) {
+  float y = scale_m(m, me);
+  if constexpr (kAny) y = __builtin_amdgcn_fmed3f(y, -0x1.cp-112f, 0x1.cp-112f);  // 448 2^-120
+  const uint32_t up = __float_as_uint(y) + ((bits & 0xFFFFu) << 4 | 8u);
+  const uint32_t c = (up >> 24 & 0x80u) | (up >> 20 & 0x7Fu);
+  return kAny && !finite(m) ? 0x7Fu : c;
 }
-__device__ __forceinline__ float read_root(uint32_t c, uint32_t k) {
-  const uint32_t high = root_base(k) + (c << 19), low = root_base(k) + (1u << 23);
-  const float f = c < 16u ? __uint_as_float(high + (1u << 23)) - __uint_as_float(low) : __uint_as_float(high);
-  return c == 255u ? __uint_as_float(0x7FC00000u) : f;
+template <bool kAny>
+__device__ __forceinline__ uint32_t hold_root(float r, uint32_t re, uint32_t bits) {
+  const uint32_t up = __float_as_uint(scale_root(r, re)) + ((bits >> 13 & ~7u) | 4u);
+  const uint32_t c = max(up >> 19, min(__float_as_uint(r), 1u));
+  return kAny && !finite(r) ? 255u : c;
+}
+__device__ __forceinline__ float read_root(uint32_t c, uint32_t re) {
+  return ldexpf(__uint_as_float(c << 19), static_cast<int>(re) - 15);
 }
 
 // Four elements of a lane, its block's exponents in all 16 lanes of a row.
@@ -114,23 +129,36 @@ struct Codes {
   uint32_t me, re;   // the exponents' bytes
 };
 
-__device__ __forceinline__ Codes hold4(const float* m, const float* r, const uint32_t* bits) {
-  Codes c;
-  const uint32_t most_m = tm_act::row_max(tm_act::largest_finite<4>(m));
-  const uint32_t most_r = tm_act::row_max(tm_act::largest_finite<4>(r));
-  const int e = tm_act::block_exponent(most_m);
-  const float inv = tm_act::two_to(-e);
-  c.me = static_cast<uint32_t>(e + 127);
-  c.re = max((most_r + 0x000FFFFFu) >> 23, static_cast<uint32_t>(kRootLow));
-  float h[4];
-  c.r = 0;
+template <bool kAny>
+__device__ __forceinline__ void codes4(Codes& c, const float* m, const float* r, const uint32_t* bits) {
+  c.m = c.r = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    h[j] = hold_m(m[j], inv, bits[j]);
-    c.r |= hold_root(r[j], c.re, bits[j]) << (8 * j);
+    c.m |= hold_m<kAny>(m[j], c.me, bits[j]) << (8 * j);
+    c.r |= hold_root<kAny>(r[j], c.re, bits[j]) << (8 * j);
   }
-  c.m = __builtin_amdgcn_cvt_pk_fp8_f32(h[0], h[1], 0, false);
-  c.m = __builtin_amdgcn_cvt_pk_fp8_f32(h[2], h[3], c.m, true);
+}
+
+__device__ __forceinline__ uint32_t most4(const float* x) {
+  return max(max(__float_as_uint(x[0]) & 0x7FFFFFFFu, __float_as_uint(x[1]) & 0x7FFFFFFFu),
+             max(__float_as_uint(x[2]) & 0x7FFFFFFFu, __float_as_uint(x[3]) & 0x7FFFFFFFu));
+}
+
+__device__ __forceinline__ Codes hold4(const float* m, const float* r, const uint32_t* bits) {
+  Codes c;
+  uint32_t most_m = most4(m), most_r = most4(r);
+  // a wave with an m past all blocks' range, an infinity or a NaN looks at each value
+  const bool any = __any(max(most_m, most_r) > tm_act::kPlainMost);
+  if (any) {
+    most_m = tm_act::largest_finite<4>(m);
+    most_r = tm_act::largest_finite<4>(r);
+  }
+  most_m = tm_act::row_max(most_m);
+  most_r = tm_act::row_max(most_r);
+  c.me = static_cast<uint32_t>(tm_act::block_exponent(most_m) + 127);
+  c.re = max((most_r + 0x000FFFFFu) >> 23, static_cast<uint32_t>(kRootLow));
+  if (any) codes4<true>(c, m, r, bits);
+  else codes4<false>(c, m, r, bits);
   return c;
 }
 
@@ -139,15 +167,21 @@ __device__ __forceinline__ void read4(const Codes& c, float* m, float* r) {
   m[0] = d.x; m[1] = d.y; m[2] = d.z; m[3] = d.w;
 #pragma unroll
   for (int j = 0; j < 4; ++j) r[j] = read_root((c.r >> (8 * j)) & 0xFFu, c.re);
+  if (__any(((~c.r - 0x01010101u) & c.r & 0x80808080u) != 0)) {  // a byte of 255
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (((c.r >> (8 * j)) & 0xFFu) == 255u) r[j] = __uint_as_float(0x7FC00000u);
+  }
 }
 
 // A tensor's held moment: codes of all elements up to the next multiple of 256, then the blocks' exponents.
 __device__ __host__ __forceinline__ int64_t held_codes(int64_t n) { return (n + kSlice - 1) / kSlice * kSlice; }
 
+template <bool kCached = false>
 __device__ __forceinline__ Codes load_codes(const tm_tensor_t& d, int64_t codes, int64_t e) {
   const uint8_t* m = reinterpret_cast<const uint8_t*>(d.exp_avg);
   const uint8_t* r = reinterpret_cast<const uint8_t*>(d.exp_avg_sq);
-  return {ld<u32_at1>(m + e), ld<u32_at1>(r + e), m[codes + e / kBlock], r[codes + e / kBlock]};
+  return {ld<u32_at1, kCached>(m + e), ld<u32_at1, kCached>(r + e), m[codes + e / kBlock], r[codes + e / kBlock]};
 }
 __device__ __forceinline__ void store_codes(const tm_tensor_t& d, int64_t codes, int64_t e, const Codes& c) {
   uint8_t* m = reinterpret_cast<uint8_t*>(d.exp_avg);
@@ -161,9 +195,11 @@ __device__ __forceinline__ void store_codes(const tm_tensor_t& d, int64_t codes,
 }
 
 // Four values from element e on, `left` of them there (0 to 4; zeros after): whole vectors at any element's alignment.
+// kWhole: all are.
+template <bool kWhole>
 __device__ __forceinline__ void load_f32(float* v, uint64_t base, int64_t e, int left) {
   const float* p = reinterpret_cast<const float*>(base) + e;
-  if (left == 4) {
+  if (kWhole || left == 4) {
     const f32x4 a = ld<f32x4_at4>(p);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   } else {
@@ -171,9 +207,10 @@ __device__ __forceinline__ void load_f32(float* v, uint64_t base, int64_t e, int
     for (int j = 0; j < 4; ++j) v[j] = j < left ? p[j] : 0.0f;
   }
 }
+template <bool kWhole>
 __device__ __forceinline__ void store_f32(uint64_t base, int64_t e, int left, const float* v) {
   float* p = reinterpret_cast<float*>(base) + e;
-  if (left == 4) {
+  if (kWhole || left == 4) {
     st<f32x4_at4>(p, (f32x4{v[0], v[1], v[2], v[3]}));
   } else {
 #pragma unroll
@@ -181,9 +218,10 @@ __device__ __forceinline__ void store_f32(uint64_t base, int64_t e, int left, co
       if (j < left) p[j] = v[j];
   }
 }
+template <bool kWhole>
 __device__ __forceinline__ void load_bf16(float* v, uint64_t base, int64_t e, int left) {
   const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + e;
-  if (left == 4) {
+  if (kWhole || left == 4) {
     const u32x2 w = ld<u32x2_at2>(p);
     v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
   } else {
@@ -191,10 +229,11 @@ __device__ __forceinline__ void load_bf16(float* v, uint64_t base, int64_t e, in
     for (int j = 0; j < 4; ++j) v[j] = j < left ? bf16_lo(p[j]) : 0.0f;
   }
 }
+template <bool kWhole>
 __device__ __forceinline__ void store_bf16(uint64_t base, int64_t e, int left, const float* v) {
   uint16_t* p = reinterpret_cast<uint16_t*>(base) + e;
   const u32x2 w = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-  if (left == 4) {
+  if (kWhole || left == 4) {
     st<u32x2_at2>(p, w);
   } else {
 #pragma unroll
@@ -203,22 +242,31 @@ __device__ __forceinline__ void store_bf16(uint64_t base, int64_t e, int left, c
   }
 }
 
-// This workgroup's chunk, and the first element of its slice. (A power of two takes a shift for the division's 25
-// instructions.)
-__device__ __forceinline__ int64_t slice_of(const tm_chunk_t* __restrict__ chunks, uint32_t first_chunk,
-                                            uint32_t slices_per_chunk, int64_t chunk_elems, tm_chunk_t& ck) {
-  const bool pow2 = (slices_per_chunk & (slices_per_chunk - 1)) == 0;
-  const uint32_t local = pow2 ? blockIdx.x >> __builtin_ctz(slices_per_chunk) : blockIdx.x / slices_per_chunk;
+// This workgroup's chunk, and the first element of its kSlices slices, in the table's order. (A power of two takes a shift for the
+// division's 25 instructions. Neighbouring slices run on different XCDs, each of which reads and writes part of
+// an exponents' line: 1.028 times the bytes. 32 slices in a row to an XCD had whole lines and were 9% slower.)
+template <int kSlices>
+__device__ __forceinline__ int64_t piece_of(const tm_chunk_t* __restrict__ chunks, uint32_t first_chunk,
+                                            uint32_t pieces_per_chunk, int64_t chunk_elems, tm_chunk_t& ck) {
+  const bool pow2 = (pieces_per_chunk & (pieces_per_chunk - 1)) == 0;
+  const uint32_t local = pow2 ? blockIdx.x >> __builtin_ctz(pieces_per_chunk) : blockIdx.x / pieces_per_chunk;
   ck = chunks[first_chunk + local];
-  return static_cast<int64_t>(ck.chunk) * chunk_elems + static_cast<int64_t>(blockIdx.x - local * slices_per_chunk) * kSlice;
+  return static_cast<int64_t>(ck.chunk) * chunk_elems +
+         static_cast<int64_t>(blockIdx.x - local * pieces_per_chunk) * (kSlices * kSlice);
+}
+
+// How many of the four elements from e on there are.
+__device__ __forceinline__ int left_of(int64_t numel, int64_t e) {
+  return static_cast<int>(max(int64_t(0), min(int64_t(4), numel - e)));
 }
 
 // ---------------------------------------------------------------- the step
 
 // What the update needs of a tensor, made once for it (64 bytes, in the workspace).
 struct alignas(16) Scal {
-  float neg_lrwd, beta1, omb1, beta2, omb2, eps, step_size, inv_bc2s;
-  uint32_t key, flags, pad[6];
+  double beta1, omb1, beta2, omb2;
+  float neg_lrwd, eps, step_size, inv_bc2s;
+  uint32_t key, flags, pad[2];
 };
 constexpr uint32_t kDecay = 1u, kF32 = 2u, kOut = 4u, kClip = 8u;
 
@@ -240,7 +288,8 @@ __global__ __launch_bounds__(kThreads) void adamw8_prep_kernel(const tm_tensor_t
     // as in the 32-bit step: a record naming a group that the call does not have is poisoned
     const float nan = __builtin_nanf("");
     *step_p = nan;
-    s.neg_lrwd = s.beta1 = s.omb1 = s.beta2 = s.omb2 = s.eps = s.step_size = s.inv_bc2s = nan;
+    s.beta1 = s.omb1 = s.beta2 = s.omb2 = nan;
+    s.neg_lrwd = s.eps = s.step_size = s.inv_bc2s = nan;
     s.flags |= kDecay;
     scal[t] = s;
     return;
@@ -251,10 +300,10 @@ __global__ __launch_bounds__(kThreads) void adamw8_prep_kernel(const tm_tensor_t
   const double bc1 = 1.0 - pow(h.beta1, static_cast<double>(step));
   const double bc2 = 1.0 - pow(h.beta2, static_cast<double>(step));
   s.neg_lrwd = static_cast<float>(-(h.lr * h.weight_decay));
-  s.beta1 = static_cast<float>(h.beta1);
-  s.omb1 = static_cast<float>(1.0 - h.beta1);
-  s.beta2 = static_cast<float>(h.beta2);
-  s.omb2 = static_cast<float>(1.0 - h.beta2);
+  s.beta1 = h.beta1;
+  s.omb1 = 1.0 - h.beta1;
+  s.beta2 = h.beta2;
+  s.omb2 = 1.0 - h.beta2;
   s.eps = static_cast<float>(h.eps);
   s.step_size = static_cast<float>(h.lr / bc1);
   s.inv_bc2s = static_cast<float>(1.0 / sqrt(bc2));
@@ -263,87 +312,130 @@ __global__ __launch_bounds__(kThreads) void adamw8_prep_kernel(const tm_tensor_t
   scal[t] = s;
 }
 
-// One wave to a slice of 256 elements: 4 a lane, a block of 64 to 16 lanes, whose largest moments meet by DPP moves.
+// A wave's kStepSlices slices from `start` on: 4 elements a lane of each, a block of 64 to 16 lanes, whose largest moments meet
+// by DPP moves.
+template <bool kF32, bool kWhole>
+__device__ __forceinline__ void update(const tm_tensor_t& d, const Scal& s, float coef, int64_t start) {
+  const int64_t e0 = start + static_cast<int64_t>(threadIdx.x) * 4, codes = held_codes(d.numel);
+  float p[kStepSlices][4], g[kStepSlices][4];
+  Codes was[kStepSlices];
+#pragma unroll
+  for (int k = 0; k < kStepSlices; ++k) {
+    const int64_t e = e0 + k * kSlice;
+    if (!kWhole && start + k * kSlice >= d.numel) continue;  // else the slice's codes are there, all of them
+    const int left = kWhole ? 4 : left_of(d.numel, e);
+    if constexpr (kF32) load_f32<kWhole>(g[k], d.grad, e, left);
+    else load_bf16<kWhole>(g[k], d.grad, e, left);
+    load_f32<kWhole>(p[k], d.master, e, left);
+    was[k] = load_codes(d, codes, e);
+  }
+#pragma unroll
+  for (int k = 0; k < kStepSlices; ++k) {
+    const int64_t e = e0 + k * kSlice;
+    if (!kWhole && start + k * kSlice >= d.numel) continue;
+    float m[4], r[4];
+    read4(was[k], m, r);
+    uint32_t bits[4];
+    const uint32_t z = static_cast<uint32_t>(e) * kHashA + s.key;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float gj = g[k][j] * coef;
+      const float pj = (s.flags & kDecay) ? fmaf(s.neg_lrwd, p[k][j], p[k][j]) : p[k][j];
+      const double gd = gj;
+      m[j] = static_cast<float>(fma(s.beta1, static_cast<double>(m[j]), s.omb1 * gd));
+      r[j] = sqrtf(static_cast<float>(fma(s.beta2, static_cast<double>(r[j] * r[j]), s.omb2 * gd * gd)));
+      p[k][j] = pj - s.step_size * m[j] / fmaf(r[j], s.inv_bc2s, s.eps);
+      bits[j] = element_bits(z + j * kHashA);
+    }
+    const Codes now = hold4(m, r, bits);
+    const int left = kWhole ? 4 : left_of(d.numel, e);
+    store_f32<kWhole>(d.master, e, left, p[k]);
+    store_codes(d, codes, e, now);
+    if (s.flags & kOut) store_bf16<kWhole>(d.param_bf16, e, left, p[k]);
+  }
+}
+
 __global__ __launch_bounds__(kWave) void adamw8_update_kernel(const tm_tensor_t* __restrict__ tensors, int64_t n_tensors,
                                                               const tm_chunk_t* __restrict__ chunks, uint32_t first_chunk,
-                                                              uint32_t slices_per_chunk, int64_t chunk_elems,
+                                                              uint32_t pieces_per_chunk, int64_t chunk_elems,
                                                               const Scal* __restrict__ scal,
                                                               const float* __restrict__ coef_p) {
   tm_chunk_t ck;
-  const int64_t start = slice_of(chunks, first_chunk, slices_per_chunk, chunk_elems, ck);
+  const int64_t start = piece_of<kStepSlices>(chunks, first_chunk, pieces_per_chunk, chunk_elems, ck);
   if (ck.tensor >= n_tensors) return;
   const tm_tensor_t d = tensors[ck.tensor];
-  if (start >= d.numel) return;  // else the slice's codes are there, whole
+  if (start >= d.numel) return;
   const Scal s = scal[ck.tensor];
-  const int64_t e = start + static_cast<int64_t>(threadIdx.x) * 4, codes = held_codes(d.numel);
-  const int left = static_cast<int>(max(int64_t(0), min(int64_t(4), d.numel - e)));
-  float p[4], g[4], m[4], r[4];
-  if (s.flags & kF32) load_f32(g, d.grad, e, left);
-  else load_bf16(g, d.grad, e, left);
-  load_f32(p, d.master, e, left);
-  const Codes was = load_codes(d, codes, e);
   const float coef = (s.flags & kClip) && coef_p ? *coef_p : 1.0f;
-  read4(was, m, r);
-  uint32_t bits[4];
-  const uint32_t z = static_cast<uint32_t>(e) * kHashA + s.key;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float gj = g[j] * coef;
-    const float pj = (s.flags & kDecay) ? fmaf(s.neg_lrwd, p[j], p[j]) : p[j];
-    m[j] = fmaf(s.beta1, m[j], s.omb1 * gj);
-    const float v = fmaf(s.beta2, r[j] * r[j], s.omb2 * gj * gj);
-    r[j] = sqrtf(v);
-    p[j] = pj - s.step_size * m[j] / fmaf(r[j], s.inv_bc2s, s.eps);
-    bits[j] = element_bits(z + j * kHashA);
+  const bool whole = start + kStepSlices * kSlice <= d.numel;
+  if (s.flags & kF32) {
+    if (whole) update<true, true>(d, s, coef, start);
+    else update<true, false>(d, s, coef, start);
+  } else {
+    if (whole) update<false, true>(d, s, coef, start);
+    else update<false, false>(d, s, coef, start);
   }
-  const Codes now = hold4(m, r, bits);
-  store_f32(d.master, e, left, p);
-  store_codes(d, codes, e, now);
-  if (s.flags & kOut) store_bf16(d.param_bf16, e, left, p);
 }
 
 // ---------------------------------------------------------------- moments as values
 
 // kRead: master = exp_avg's values and grad = the root's, in bf16, or with TM_GRAD_F32 exp_avg's and exp_avg_sq's
 // (the root's square) in fp32. Else the fp32 exp_avg and exp_avg_sq there are held, to the nearest.
-template <bool kRead>
-__global__ __launch_bounds__(kWave) void moments8_kernel(const tm_tensor_t* __restrict__ tensors, int64_t n_tensors,
-                                                         const tm_chunk_t* __restrict__ chunks, uint32_t first_chunk,
-                                                         uint32_t slices_per_chunk, int64_t chunk_elems) {
-  tm_chunk_t ck;
-  const int64_t start = slice_of(chunks, first_chunk, slices_per_chunk, chunk_elems, ck);
-  if (ck.tensor >= n_tensors) return;
-  const tm_tensor_t d = tensors[ck.tensor];
-  if (start >= d.numel) return;
-  const int64_t e = start + static_cast<int64_t>(threadIdx.x) * 4, codes = held_codes(d.numel);
-  const int left = static_cast<int>(max(int64_t(0), min(int64_t(4), d.numel - e)));
-  float m[4], r[4];
+template <bool kRead, bool kWhole>
+__device__ __forceinline__ void move_moments(const tm_tensor_t& d, int64_t start) {
+  const int64_t e0 = start + static_cast<int64_t>(threadIdx.x) * 4, codes = held_codes(d.numel);
+  Codes was[kReadSlices];
   if constexpr (kRead) {
-    read4(load_codes(d, codes, e), m, r);
-    if (d.flags & TM_GRAD_F32) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] *= r[j];
-      store_f32(d.master, e, left, m);
-      store_f32(d.grad, e, left, r);
+    for (int k = 0; k < kReadSlices; ++k)
+      if (kWhole || start + k * kSlice < d.numel) was[k] = load_codes<true>(d, codes, e0 + k * kSlice);
+  }
+#pragma unroll
+  for (int k = 0; k < kReadSlices; ++k) {
+    const int64_t e = e0 + k * kSlice;
+    if (!kWhole && start + k * kSlice >= d.numel) continue;
+    const int left = kWhole ? 4 : left_of(d.numel, e);
+    float m[4], r[4];
+    if constexpr (kRead) {
+      read4(was[k], m, r);
+      if (d.flags & TM_GRAD_F32) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[j] *= r[j];
+        store_f32<kWhole>(d.master, e, left, m);
+        store_f32<kWhole>(d.grad, e, left, r);
+      } else {
+        store_bf16<kWhole>(d.master, e, left, m);
+        store_bf16<kWhole>(d.grad, e, left, r);
+      }
     } else {
-      store_bf16(d.master, e, left, m);
-      store_bf16(d.grad, e, left, r);
-    }
-  } else {
-    load_f32(m, d.master, e, left);
-    load_f32(r, d.grad, e, left);
+      load_f32<kWhole>(m, d.master, e, left);
+      load_f32<kWhole>(r, d.grad, e, left);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) r[j] = sqrtf(r[j]);
-    const uint32_t half[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-    store_codes(d, codes, e, hold4(m, r, half));
+      for (int j = 0; j < 4; ++j) r[j] = sqrtf(r[j]);
+      const uint32_t half[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+      store_codes(d, codes, e, hold4(m, r, half));
+    }
   }
 }
 
-// kernel(first_chunk, slices_per_chunk, blocks) over a chunk table: launches of less than 2^32 work-items, of
-// whole chunks.
+template <bool kRead>
+__global__ __launch_bounds__(kWave) void moments8_kernel(const tm_tensor_t* __restrict__ tensors, int64_t n_tensors,
+                                                         const tm_chunk_t* __restrict__ chunks, uint32_t first_chunk,
+                                                         uint32_t pieces_per_chunk, int64_t chunk_elems) {
+  tm_chunk_t ck;
+  const int64_t start = piece_of<kReadSlices>(chunks, first_chunk, pieces_per_chunk, chunk_elems, ck);
+  if (ck.tensor >= n_tensors) return;
+  const tm_tensor_t d = tensors[ck.tensor];
+  if (start >= d.numel) return;
+  if (start + kReadSlices * kSlice <= d.numel) move_moments<kRead, true>(d, start);
+  else move_moments<kRead, false>(d, start);
+}
+
+// kernel(first_chunk, pieces_per_chunk, blocks) over a chunk table, a piece of `slices` slices to a workgroup: launches of
+// less than 2^32 work-items, of whole chunks.
 template <class F>
-int launch_chunks(int64_t n_chunks, int64_t chunk_elems, const char* what, F&& launch) {
-  const int64_t spc = chunk_elems / kSlice, per = 0xFFFFFFFFll / kWave / spc;
+int launch_chunks(int64_t n_chunks, int64_t chunk_elems, int slices, const char* what, F&& launch) {
+  const int64_t spc = chunk_elems / (kSlice * slices), per = 0xFFFFFFFFll / kWave / spc;
   for (int64_t first = 0; first < n_chunks; first += per) {
     const int64_t cnt = std::min(per, n_chunks - first);
     launch(static_cast<uint32_t>(first), static_cast<uint32_t>(spc), dim3(static_cast<uint32_t>(cnt * spc)));
@@ -358,7 +450,7 @@ int moments8(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chunk_t* 
              int64_t chunk_elems, void* stream, const char* who) {
   const int rc = tm_internal_check_table(d_tensors, n_tensors, d_chunks, n_chunks, chunk_elems, who);
   if (rc) return rc;
-  return launch_chunks(n_chunks, chunk_elems, who, [&](uint32_t first, uint32_t spc, dim3 grid) {
+  return launch_chunks(n_chunks, chunk_elems, kReadSlices, who, [&](uint32_t first, uint32_t spc, dim3 grid) {
     hipLaunchKernelGGL(moments8_kernel<kRead>, grid, dim3(kWave), 0, static_cast<hipStream_t>(stream), d_tensors, n_tensors,
                        d_chunks, first, spc, chunk_elems);
   });
@@ -392,7 +484,7 @@ int tm_adamw8_step(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_chu
                      s, d_tensors, n_tensors, hyper, static_cast<uint32_t>(seed), static_cast<uint32_t>(seed >> 32), scal);
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return fail(TM_ELAUNCH, "adamw8_prep_kernel: launch failed: %s", hipGetErrorString(err));
-  return launch_chunks(n_chunks, chunk_elems, "adamw8_update_kernel", [&](uint32_t first, uint32_t spc, dim3 grid) {
+  return launch_chunks(n_chunks, chunk_elems, kStepSlices, "adamw8_update_kernel", [&](uint32_t first, uint32_t spc, dim3 grid) {
     hipLaunchKernelGGL(adamw8_update_kernel, grid, dim3(kWave), 0, s, d_tensors, n_tensors, d_chunks, first, spc, chunk_elems,
                        scal, d_coef);
   });

@@ -171,6 +171,7 @@ class AdamW(torch.optim.Optimizer):
         self._pending = None  # (coef device tensor, _ClipRecord)
         self._uploader = tables.TableUploader()
         self._uploader_read = tables.TableUploader()  # flat_moments' tables
+        self._held = None  # flat_moments' _Held of the last call, used again while nothing changes
         self._verified: dict = {}  # id(param) -> _ParamEntry
         self._plan = None  # _Plan of the last full step, reused while nothing changes
         super().__init__(params, defaults)
@@ -213,6 +214,7 @@ class AdamW(torch.optim.Optimizer):
         self.__dict__.setdefault("_pending", None)
         self.__dict__.setdefault("_uploader", tables.TableUploader())
         self.__dict__.setdefault("_uploader_read", tables.TableUploader())
+        self.__dict__.setdefault("_held", None)
         self.__dict__.setdefault("_verified", {})
         self.__dict__.setdefault("_plan", None)
 
@@ -566,26 +568,28 @@ class AdamW(torch.optim.Optimizer):
         who = "torchure_amd.AdamW.flat_moments"
         if self.state_bits != 8:
             raise RuntimeError(f"{who}: the moments of an optimizer with state_bits=32 are its state's own tensors")
-        params = [p for group in self.param_groups for p in group["params"] if self.state.get(p)]
-        if not params:
-            raise RuntimeError(f"{who}: no param has state yet")
-        device = params[0].device
-        if any(p.device != device for p in params):
-            raise RuntimeError(f"{who}: params on several devices")
-        for p in params:
-            st = self.state[p]
-            if st["exp_avg"].dtype != torch.uint8 or st["exp_avg"].device != device or not st["exp_avg"].is_contiguous():
-                self._verify_param(p, st, getattr(p, "_tm_working", None))
-        numels = np.array([p.numel() for p in params], dtype=np.int64)
-        total = int(numels.sum())
-        m, r = (torch.empty(total, dtype=torch.bfloat16, device=device) for _ in range(2))
-        rows = np.zeros(len(params), dtype=_native.TENSOR_DTYPE)
-        at = 2 * (np.cumsum(numels) - numels).astype(np.uint64)
-        rows["master"], rows["grad"] = at + np.uint64(m.data_ptr()), at + np.uint64(r.data_ptr())
-        rows["numel"] = numels
-        for k in ("exp_avg", "exp_avg_sq"):
-            rows[k] = [self.state[p][k].data_ptr() for p in params]
-        _launch_moments("tm_moments8_read", rows, device, self._uploader_read)
+        host, state, held = _native.host(), self.state, self._held
+        # the params, their states and the states' tensors, compared as objects (a tensor's hash is a Python call)
+        every, keys, values = [p for group in self.param_groups for p in group["params"]], list(state), list(state.values())
+        if held is None or not all(map(host.same, (every, keys, values), held.given)):
+            held = None
+        else:
+            tensors = [st[k] for k in ("exp_avg", "exp_avg_sq") for st in held.states]
+            if not host.same(tensors, held.tensors) or not np.array_equal(host.ptrs(tensors), held.ptrs):
+                held = None
+        if held is None:
+            params = [p for p in every if state.get(p)]
+            if not params:
+                raise RuntimeError(f"{who}: no param has state yet")
+            if any(p.device != params[0].device for p in params):
+                raise RuntimeError(f"{who}: params on several devices")
+            for p in params:
+                self._verify_param(p, state[p], getattr(p, "_tm_working", None))
+            held = self._held = _Held((every, keys, values), params, [state[p] for p in params])
+        m, r = (torch.empty(held.total, dtype=torch.bfloat16, device=held.device) for _ in range(2))
+        rows = held.rows
+        rows["master"], rows["grad"] = held.starts + np.uint64(m.data_ptr()), held.starts + np.uint64(r.data_ptr())
+        _launch_moments("tm_moments8_read", rows, held.device, self._uploader_read)
         return m, r
 
     def _plan_launches(self, per_dev, hyper, coef) -> list["StepLaunch"]:
@@ -653,6 +657,22 @@ class _ParamEntry:
         self.numel = p.numel()
         self.device = p.device
         self.dev_index = p.get_device()
+
+
+class _Held:
+    """``flat_moments``' table, and the objects it was built from."""
+
+    __slots__ = ("given", "states", "tensors", "ptrs", "device", "rows", "starts", "total")
+
+    def __init__(self, given, params: list, states: list):
+        self.given, self.states, self.device = given, states, params[0].device
+        self.tensors = [st[k] for k in ("exp_avg", "exp_avg_sq") for st in states]
+        self.ptrs = _native.host().ptrs(self.tensors)
+        self.rows = np.zeros(len(params), dtype=_native.TENSOR_DTYPE)
+        self.rows["numel"] = [p.numel() for p in params]
+        self.rows["exp_avg"], self.rows["exp_avg_sq"] = self.ptrs[: len(params)], self.ptrs[len(params):]
+        ends = np.cumsum(self.rows["numel"])
+        self.starts, self.total = (2 * (ends - self.rows["numel"])).astype(np.uint64), int(ends[-1])
 
 
 class _ClipRecord:
