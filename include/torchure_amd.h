@@ -536,6 +536,24 @@ int tm_moments8_write(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_
                       int64_t chunk_elems, void* stream);
 
 /*
+ * Layer norm (layer = 1) and RMS norm (0) of a matrix's rows (torchure/models/qwen3/qwen3.py:86-217,243-274: the block's and the heads'
+ * RMS norms): y = (x - mean) rstd w + b, rstd = 1 / sqrt(mean((x - mean)^2) + eps), mean = 0 for RMS; fp32 inside, rounded once.
+ * x (rows ldx apart), y (rows cols apart), w and b (cols; or NULL) bf16 or, with their flag, fp32, at their elements' alignment.
+ *   tm_norm_forward    d_rstd and d_mean (rows values each, mean for layer norm only): written where given, for the backward pass.
+ *   tm_norm_backward   d_dx (x's type, rows cols apart), d_dw (dw_f32) and d_db (b_f32, layer norm only), each or NULL, from dy
+ *                      (y's type, rows lddy apart). With d_dw or d_db, d_ws holds tm_norm_workspace_bytes bytes. Sums over
+ *                      rows are made in a fixed order.
+ * Limits: cols <= 16384, rows <= 2^40.
+ */
+int tm_norm_forward(void* d_y, int y_f32, float* d_rstd, float* d_mean, const void* d_x, int x_f32, int64_t ldx,
+                    const void* d_w, int w_f32, const void* d_b, int b_f32, int layer, double eps, int64_t rows, int64_t cols,
+                    void* stream);
+size_t tm_norm_workspace_bytes(int64_t rows, int64_t cols, int x_f32, int y_f32, int layer);
+int tm_norm_backward(void* d_dx, void* d_dw, void* d_db, int b_f32, const void* d_dy, int y_f32, int64_t lddy, const void* d_x,
+                     int x_f32, int64_t ldx, const float* d_rstd, const float* d_mean, const void* d_w, int w_f32, int dw_f32,
+                     int layer, int64_t rows, int64_t cols, void* d_ws, size_t ws_bytes, void* stream);
+
+/*
  * Activations held in 8 bits between forward and backward: e4m3 values (rows ldv apart, ldv = cols' next
  * multiple of 32, padding zero, 16-byte aligned) and for each block of 32 rows x 32 columns the byte
  * e + 127 (ceil(rows / 32) x ceil(cols / 32)): e the least exponent with which the block's largest

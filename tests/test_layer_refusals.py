@@ -1,0 +1,90 @@
+"""What the norms and the embedding refuse, without a GPU: the Python checks (the one of the device left out to reach the
+others) and the C ABI's, which all come before any HIP call."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import torchure_amd as ta
+from torchure_amd import _native, norm
+
+BF16, F32, F16 = torch.bfloat16, torch.float32, torch.float16
+FAKE = 0x1000
+
+
+def ones(*shape, dtype=BF16):
+    return torch.ones(shape, dtype=dtype)
+
+
+@pytest.fixture
+def no_device(monkeypatch):
+    monkeypatch.setattr(norm, "_on_gpu", lambda t, who, what: None)
+
+
+def test_cpu_tensors():
+    for call in (lambda: ta.rms_norm(ones(3, 4)), lambda: ta.layer_norm(ones(3, 4), ones(4), ones(4))):
+        with pytest.raises(RuntimeError, match="ROCm GPU"):
+            call()
+
+
+@pytest.mark.parametrize("args,error,match", [
+    (dict(x=ones(3, 4, dtype=F16)), NotImplementedError, "x must be"),
+    (dict(x=ones()), ValueError, "dimension"),
+    (dict(x=ones(3, 0), weight=None, bias=None), RuntimeError, "0 features"),
+    (dict(x=ones(2, 16385), weight=None, bias=None), RuntimeError, "16385 features"),
+    (dict(weight=ones(4, dtype=F16)), NotImplementedError, "weight must be"),
+    (dict(bias=ones(4, dtype=torch.float64)), NotImplementedError, "bias must be"),
+    (dict(weight=ones(3)), RuntimeError, "weight of shape"),
+    (dict(weight=ones(1, 4)), RuntimeError, "weight of shape"),
+    (dict(bias=ones(5)), RuntimeError, "bias of shape"),
+    (dict(dtype=F16), NotImplementedError, "dtype"),
+    (dict(dtype=torch.int32), NotImplementedError, "dtype"),
+    (dict(eps=-1e-6), ValueError, "eps"),
+    (dict(eps=float("nan")), ValueError, "eps"),
+    (dict(x=torch.eye(4).to_sparse()), NotImplementedError, "dense"),
+])
+def test_layer_norm(no_device, args, error, match):
+    with pytest.raises(error, match=match):
+        ta.layer_norm(**{"x": ones(3, 4), "weight": ones(4), "bias": ones(4), **args})
+
+
+def test_rms_norm(no_device):
+    with pytest.raises(RuntimeError, match="weight of shape"):
+        ta.rms_norm(ones(3, 4), ones(5))
+    with pytest.raises(TypeError):
+        ta.rms_norm(ones(3, 4), ones(4), bias=ones(4))
+
+
+def test_no_rows(no_device):
+    y = ta.layer_norm(ones(0, 4).requires_grad_(), ones(4), dtype=F32)
+    assert y.shape == (0, 4) and y.dtype == F32 and y.grad_fn is not None
+
+
+def test_norm_checks_without_gpu():
+    lib = _native.lib()
+    #       y     f  rstd  mean  x     f  ldx w     f  b     f  layer eps   rows cols
+    good = [FAKE, 0, FAKE, FAKE, FAKE, 0, 40, FAKE, 0, FAKE, 0, 1, 1e-5, 33, 40, None]
+    for at, bad in ((0, None), (0, 0x1001), (2, 0x1002), (3, None), (3, 0x1002), (4, None), (4, 0x1001), (6, 39), (7, 0x1001),
+                    (9, 0x1001), (13, -1), (13, (1 << 40) + 1), (14, 0), (14, -1), (14, 16385)):
+        args = list(good)
+        args[at] = bad
+        assert lib.tm_norm_forward(*args) < 0 and b"tm_norm_forward" in lib.tm_last_error(), (at, bad)
+        assert b"launch" not in lib.tm_last_error(), (at, bad)
+    assert lib.tm_norm_forward(*good[:13], 0, 40, None) == 0  # nothing to do
+    args = list(good)
+    args[1], args[0] = 1, 0x1002
+    assert lib.tm_norm_forward(*args) < 0
+    need = lib.tm_norm_workspace_bytes(33, 40, 0, 0, 1)
+    assert need > 0 and need % 320 == 0 and lib.tm_norm_workspace_bytes(33, 40, 0, 0, 0) == need // 2
+    assert lib.tm_norm_workspace_bytes(0, 40, 0, 0, 1) == 0 and lib.tm_norm_workspace_bytes(1, 16385, 0, 0, 1) == 0
+    #       dx    dw    db    bf dy    yf lddy x    xf ldx rstd  mean  w     wf dwf layer rows cols ws
+    good = [FAKE, FAKE, FAKE, 0, FAKE, 0, 40, FAKE, 0, 40, FAKE, FAKE, FAKE, 0, 0, 1, 33, 40, FAKE, need, None]
+    for at, bad in ((0, 0x1001), (1, 0x1001), (2, 0x1001), (4, None), (4, 0x1001), (6, 39), (7, None), (7, 0x1001), (9, 39), (10, None),
+                    (11, None), (12, 0x1001), (15, 0), (16, 0), (16, -1), (17, 0), (17, 16385), (18, None), (18, 0x1002),
+                    (19, need - 1)):
+        args = list(good)
+        args[at] = bad
+        assert lib.tm_norm_backward(*args) < 0 and b"tm_norm_backward" in lib.tm_last_error(), (at, bad)
+        assert b"launch" not in lib.tm_last_error(), (at, bad)
+    assert lib.tm_norm_backward(None, None, None, *good[3:18], None, 0, None) == 0  # nothing wanted

@@ -14,6 +14,7 @@ from torchure_amd.linear import (
     quantize_activation,
     swiglu_mlp,
 )
+from torchure_amd.norm import layer_norm, rms_norm
 from torchure_amd.optimizer import (
     AdamW,
     WarmupStableDecaySchedulder,
@@ -28,6 +29,8 @@ __all__ = [
     "clip_grad_norm",
     "fused_linear",
     "swiglu_mlp",
+    "layer_norm",
+    "rms_norm",
     "quantize_activation",
     "dequantize_activation",
     "QuantizedActivation",

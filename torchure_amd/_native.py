@@ -148,6 +148,17 @@ _SIGNATURES = {
     "tm_ce_grad_w_ld_bf16": (ctypes.c_int, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
     "tm_lin_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, _i64, _i64, _i64, ctypes.c_int]),
     "tm_lin": (ctypes.c_int, [ctypes.POINTER(TmLin), _vp, ctypes.c_size_t, _vp]),
+    "tm_norm_forward": (
+        ctypes.c_int,
+        [_vp, ctypes.c_int, _vp, _vp, _vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _vp, ctypes.c_int, ctypes.c_int,
+         ctypes.c_double, _i64, _i64, _vp],
+    ),
+    "tm_norm_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "tm_norm_backward": (
+        ctypes.c_int,
+        [_vp, _vp, _vp, ctypes.c_int, _vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _vp, _vp, _vp, ctypes.c_int,
+         ctypes.c_int, ctypes.c_int, _i64, _i64, _vp, ctypes.c_size_t, _vp],
+    ),
     "tm_quantize_e4m3": (ctypes.c_int, [_vp, _vp, _i64, _vp, ctypes.c_int, _i64, _i64, _i64, _vp, _i64, _vp]),
     "tm_dequantize_e4m3": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _vp, _vp, _i64, _i64, _i64, _vp]),
     "tm_held_gate": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, ctypes.c_int, _i64, _i64, _vp]),
@@ -233,6 +244,20 @@ def lin_host():
         h.lin_bind({n: ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _SIGNATURES}, NativeError)
         _LIN_HOST = h
     return _LIN_HOST
+
+
+_LAYER_HOST = None
+
+
+def layer_host():
+    """``host()`` with the norms' C entry points bound."""
+    global _LAYER_HOST
+    if _LAYER_HOST is None:
+        handle = lib()
+        h = host()
+        h.layer_bind({n: ctypes.cast(getattr(handle, n), ctypes.c_void_p).value for n in _SIGNATURES}, NativeError)
+        _LAYER_HOST = h
+    return _LAYER_HOST
 
 
 def check(rc: int, what: str) -> None:

@@ -19,7 +19,7 @@ import subprocess
 _HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(_HERE)
 SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("tm_optim.hip", "tm_ce.hip", "tm_ce_gemm.hip", "tm_linear.hip", "tm_act.hip",
-                                                  "tm_adamw8.hip")]
+                                                  "tm_adamw8.hip", "tm_norm.hip")]
 INCLUDE = os.path.join(ROOT, "include")
 OUTPUT = os.path.join(_HERE, "libtorchure_amd.so")
 ARCH = "gfx950"
@@ -48,7 +48,7 @@ def command(output: str = OUTPUT, extra: list[str] | None = None) -> list[str]:
     ]
 
 
-HOST_SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("tm_host.cpp", "tm_ce_host.cpp", "tm_lin_host.cpp")]
+HOST_SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("tm_host.cpp", "tm_ce_host.cpp", "tm_lin_host.cpp", "tm_layer_host.cpp")]
 
 
 def host_output() -> str:

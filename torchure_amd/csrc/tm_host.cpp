@@ -524,11 +524,13 @@ struct Stamp {
 
 void tm_ce_host_bind(py::module_& m);   // tm_ce_host.cpp
 void tm_lin_host_bind(py::module_& m);  // tm_lin_host.cpp
+void tm_layer_host_bind(py::module_& m);  // tm_layer_host.cpp
 
 PYBIND11_MODULE(_tm_host, m) {
   m.doc() = "torchure_amd host-side list primitives (CPU only)";
   tm_ce_host_bind(m);
   tm_lin_host_bind(m);
+  tm_layer_host_bind(m);
   m.def("collect", &collect, "(grads, their params, distinct owner marks) of a list of params");
   m.def("grad_rows", &grad_rows, "tensor table of a grad-only call");
   m.def("plan_match", &plan_match, "the steady-state step's checks: (grads, pointers) or None");

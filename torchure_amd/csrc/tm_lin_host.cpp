@@ -13,15 +13,14 @@
 #include <string>
 #include <tuple>
 
+#include "tm_rows.h"
 #include "torchure_amd.h"
 
 namespace py = pybind11;
 
 namespace {
 
-using i64 = int64_t;
-using at::Tensor;
-using Opt = c10::optional<Tensor>;
+using namespace tm_rows;
 
 struct Abi {
   decltype(&tm_lin_workspace_bytes) lin_bytes;
@@ -57,10 +56,6 @@ const Abi& abi() {
   return *g_abi;
 }
 
-struct EntryFailed : std::runtime_error {
-  using std::runtime_error::runtime_error;
-};
-
 void check(int rc, const char* what) {
   if (rc != 0)
     throw EntryFailed(std::string(what) + " failed (" + std::to_string(rc) + "): " + abi().last_error());
@@ -76,34 +71,6 @@ auto without_gil(Body&& body) -> decltype(body()) {
     PyErr_SetString(abi().native_error.ptr(), e.what());
     throw py::error_already_set();
   }
-}
-
-i64 up(i64 n, i64 to) { return (n + to - 1) / to * to; }
-bool is_f32(const Tensor& t) { return t.scalar_type() == at::kFloat; }
-char* ptr(const Tensor& t) { return t.defined() ? static_cast<char*>(t.data_ptr()) : nullptr; }
-uint8_t* bytes_of(const Tensor& t) { return reinterpret_cast<uint8_t*>(ptr(t)); }
-uint16_t* bf16_of(const Tensor& t) { return reinterpret_cast<uint16_t*>(ptr(t)); }
-py::object or_none(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
-
-Tensor room(const Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
-  return at::empty(sizes, like.options().dtype(type).requires_grad(false).memory_format(c10::nullopt));
-}
-
-// A tensor as rows of its last dimension, the elements of a row next to each other, rows apart by at least their
-// length and less than 2^23 elements. (The tensor is kept alive by its own storage where no copy is made.)
-struct Rows {
-  Tensor t;
-  i64 n = 0, d = 0, ld = 0;
-};
-
-Rows rows_of(const Tensor& given) {
-  Tensor t = given.detach();
-  if (t.is_neg()) t = t.resolve_neg();
-  const i64 d = t.size(-1), n = d ? t.numel() / d : 0;
-  if (t.dim() != 2) t = t.reshape({n, d});
-  if ((d > 1 && t.stride(1) != 1) || (n > 1 && (t.stride(0) < d || t.stride(0) >= (1 << 23))))
-    t = t.contiguous();
-  return {t, n, d, n > 1 ? t.stride(0) : d};
 }
 
 bool fits(const Rows& r) {  // whole 16-byte groups, as the kernels read operands

@@ -1,0 +1,97 @@
+// tm_units.h -- units of 4 or 8 neighbouring elements of a bf16 or fp32 row, as the row kernels read and write them: one
+// access of 8 or 16 bytes at any element's alignment, element by element at a row's end.
+#ifndef TM_UNITS_H
+#define TM_UNITS_H
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "tm_act.h"
+
+namespace tm_units {
+
+using tm_act::u32x2;
+using tm_act::u32x4;
+using tm_act::u32x4_at2;
+using tm_act::u32x4_at4;
+typedef u32x2 u32x2_at2 __attribute__((aligned(2)));
+
+template <bool kStream, typename T>
+__device__ __forceinline__ T load(const T* p) {
+  if constexpr (kStream) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool kStream, typename T, typename V>
+__device__ __forceinline__ void store(T* p, V v) {
+  if constexpr (kStream) __builtin_nontemporal_store(static_cast<T>(v), p);
+  else *p = v;
+}
+
+// `left` of them exist; zeros after. kStream: past the caches.
+template <bool kF32, int kU, bool kStream = false>
+__device__ __forceinline__ void get(float (&v)[kU], const void* base, int64_t at, int left) {
+  if constexpr (kF32) {
+    static_assert(kU == 4, "16 bytes");
+    const float* p = static_cast<const float*>(base) + at;
+    if (left >= 4) {
+      const u32x4 w = load<kStream>(reinterpret_cast<const u32x4_at4*>(p));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = i < left ? p[i] : 0.0f;
+    }
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if (left >= kU) {
+      uint32_t w[kU / 2];
+      if constexpr (kU == 8) {
+        const u32x4 a = load<kStream>(reinterpret_cast<const u32x4_at2*>(p));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = a[i];
+      } else {
+        const u32x2 a = load<kStream>(reinterpret_cast<const u32x2_at2*>(p));
+        w[0] = a.x;
+        w[1] = a.y;
+      }
+#pragma unroll
+      for (int i = 0; i < kU; ++i) v[i] = i % 2 ? tm_act::bf16_hi(w[i / 2]) : tm_act::bf16_lo(w[i / 2]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kU; ++i) v[i] = i < left ? tm_act::bf16_lo(p[i]) : 0.0f;
+    }
+  }
+}
+
+template <bool kF32, int kU, bool kStream = false>
+__device__ __forceinline__ void put(void* base, int64_t at, const float (&v)[kU], int left) {
+  if constexpr (kF32) {
+    float* p = static_cast<float*>(base) + at;
+    if (left >= 4) {
+      store<kStream>(reinterpret_cast<u32x4_at4*>(p), (u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]),
+                                                             __float_as_uint(v[2]), __float_as_uint(v[3])}));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) p[i] = v[i];
+    }
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(base) + at;
+    uint32_t w[kU / 2];
+#pragma unroll
+    for (int i = 0; i < kU / 2; ++i) w[i] = tm_act::pack_bf16(v[2 * i], v[2 * i + 1]);
+    if (left >= kU) {
+      if constexpr (kU == 8) store<kStream>(reinterpret_cast<u32x4_at2*>(p), (u32x4{w[0], w[1], w[2], w[3]}));
+      else store<kStream>(reinterpret_cast<u32x2_at2*>(p), (u32x2{w[0], w[1]}));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kU; ++i)
+        if (i < left) p[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+
+}  // namespace tm_units
+
+#endif
