@@ -28,40 +28,61 @@ __device__ __forceinline__ void store(T* p, V v) {
   else *p = v;
 }
 
-// `left` of them exist; zeros after. kStream: past the caches.
+// A unit as it was read.
+template <bool kF32, int kU>
+struct Raw {
+  static_assert(!kF32 || kU == 4, "at most 16 bytes");
+  uint32_t w[kF32 ? kU : kU / 2];
+};
+
+// `left` of its elements exist; zeros after. kStream: past the caches.
 template <bool kF32, int kU, bool kStream = false>
-__device__ __forceinline__ void get(float (&v)[kU], const void* base, int64_t at, int left) {
+__device__ __forceinline__ Raw<kF32, kU> read(const void* base, int64_t at, int left) {
+  Raw<kF32, kU> r = {};
   if constexpr (kF32) {
-    static_assert(kU == 4, "16 bytes");
-    const float* p = static_cast<const float*>(base) + at;
+    const uint32_t* p = static_cast<const uint32_t*>(base) + at;
     if (left >= 4) {
-      const u32x4 w = load<kStream>(reinterpret_cast<const u32x4_at4*>(p));
+      const u32x4 a = load<kStream>(reinterpret_cast<const u32x4_at4*>(p));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(w[i]);
+      for (int i = 0; i < 4; ++i) r.w[i] = a[i];
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = i < left ? p[i] : 0.0f;
+      for (int i = 0; i < 3; ++i)
+        if (i < left) r.w[i] = p[i];
     }
   } else {
     const uint16_t* p = static_cast<const uint16_t*>(base) + at;
     if (left >= kU) {
-      uint32_t w[kU / 2];
       if constexpr (kU == 8) {
         const u32x4 a = load<kStream>(reinterpret_cast<const u32x4_at2*>(p));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = a[i];
+        for (int i = 0; i < 4; ++i) r.w[i] = a[i];
       } else {
         const u32x2 a = load<kStream>(reinterpret_cast<const u32x2_at2*>(p));
-        w[0] = a.x;
-        w[1] = a.y;
+        r.w[0] = a.x;
+        r.w[1] = a.y;
       }
-#pragma unroll
-      for (int i = 0; i < kU; ++i) v[i] = i % 2 ? tm_act::bf16_hi(w[i / 2]) : tm_act::bf16_lo(w[i / 2]);
     } else {
 #pragma unroll
-      for (int i = 0; i < kU; ++i) v[i] = i < left ? tm_act::bf16_lo(p[i]) : 0.0f;
+      for (int i = 0; i < kU - 1; ++i)
+        if (i < left) r.w[i / 2] |= static_cast<uint32_t>(p[i]) << (16 * (i & 1));
     }
   }
+  return r;
+}
+
+template <bool kF32, int kU>
+__device__ __forceinline__ void values(float (&v)[kU], const Raw<kF32, kU>& r) {
+#pragma unroll
+  for (int i = 0; i < kU; ++i) {
+    if constexpr (kF32) v[i] = __uint_as_float(r.w[i]);
+    else v[i] = i % 2 ? tm_act::bf16_hi(r.w[i / 2]) : tm_act::bf16_lo(r.w[i / 2]);
+  }
+}
+
+template <bool kF32, int kU, bool kStream = false>
+__device__ __forceinline__ void get(float (&v)[kU], const void* base, int64_t at, int left) {
+  values(v, read<kF32, kU, kStream>(base, at, left));
 }
 
 template <bool kF32, int kU, bool kStream = false>

@@ -10,35 +10,13 @@ can be the bf16 operand of the product behind it.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
+from torch.autograd import forward_ad
 
 from torchure_amd import _native
-from torchure_amd.linear import _current, _NoRows, _on_gpu, _wants_autograd
+from torchure_amd.linear import _NoRows, _on_gpu
 
 _BF16, _F32 = torch.bfloat16, torch.float32
 MAX_FEATURES = 16384
-
-
-class _Norm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, layer, eps, y_f32):
-        with _current(x.device):
-            y, *kept = _native.layer_host().norm_forward(x, weight, bias, layer, eps, y_f32, any(ctx.needs_input_grad[:3]),
-                                                         _native.stream_handle(x.device))
-        ctx.meta = (x.shape, layer, weight is not None and weight.dtype == _F32, bias is not None and bias.dtype == _F32)
-        ctx.save_for_backward(*kept)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        need = ctx.needs_input_grad[:3]
-        grads = (None,) * 3
-        if any(need):
-            with _current(dy.device):
-                grads = _native.layer_host().norm_backward(dy, *ctx.saved_tensors, *ctx.meta, *need,
-                                                           _native.stream_handle(dy.device))
-        return *grads, None, None, None
 
 
 def _checked(who, x, weight, bias, dtype):
@@ -62,6 +40,13 @@ def _checked(who, x, weight, bias, dtype):
             raise RuntimeError(f"{who}: {what} of shape {tuple(t.shape)} for {features} features")
 
 
+def _refuse_tangents(who, *tensors):
+    """A forward-mode tangent is refused: the kernels would drop it."""
+    if forward_ad._current_level >= 0:  # inside dual_level
+        if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+            raise NotImplementedError(f"{who}: forward-mode derivatives are not supported")
+
+
 def _norm(who, x, weight, bias, layer, eps, dtype):
     host = _native.layer_host()
     if dtype is None:
@@ -74,11 +59,10 @@ def _norm(who, x, weight, bias, layer, eps, dtype):
     if not x.is_cuda or not host.norm_plain(x, weight, bias, torch.cuda.current_device()):
         _checked(who, x, weight, bias, dtype)
         if x.numel() == 0:
+            _refuse_tangents(who, x, weight, bias)
             return _NoRows.apply(x.shape, dtype, x, *(t for t in (weight, bias) if t is not None))
-    if _wants_autograd(x, weight, bias):
-        return _Norm.apply(x, weight, bias, layer, eps, dtype == _F32)
-    with _current(x.device):
-        return host.norm_forward(x, weight, bias, layer, eps, dtype == _F32, False, _native.stream_handle(x.device))[0]
+    _refuse_tangents(who, x, weight, bias)
+    return host.norm(x, weight, bias, layer, eps, dtype == _F32, _native.stream_handle(x.device))
 
 
 def rms_norm(
