@@ -554,6 +554,23 @@ int tm_norm_backward(void* d_dx, void* d_dw, void* d_db, int b_f32, const void* 
                      int layer, int64_t rows, int64_t cols, void* d_ws, size_t ws_bytes, void* stream);
 
 /*
+ * Token embedding (torchure/models/qwen3/qwen3.py:285-286: the table that the head is tied to). Ids are int64 (ids64) or int32; tables bf16
+ * or fp32 (w_f32), rows ldw apart; y and dy bf16 or fp32 (y_f32), at their elements' alignment.
+ *   tm_embed_lookup   y (tokens x cols) = scale * w[ids], rounded once. An id outside 0..vocab-1 gives a row of NaN.
+ *   tm_embed_grad     dw (vocab x cols) = scale * the sums of dy's rows (lddy apart) by id, in fp32 and in the tokens' order, rounded
+ *                     once, and zeros where no token is; or, with add, dw += those sums, rows without tokens untouched. Ids
+ *                     outside 0..vocab-1 and `padding` (-1: none) take no part. d_ws, 16-byte aligned, holds
+ *                     tm_embed_grad_workspace_bytes bytes.
+ * Limits: 2^30 tokens and ids, 2^20 columns, a gradient of tokens x cols up to about 2^32 x 8 elements (refused past its launches).
+ */
+int tm_embed_lookup(void* d_y, int y_f32, const void* d_w, int w_f32, int64_t ldw, const void* d_ids, int ids64, int64_t tokens,
+                    int64_t vocab, int64_t cols, float scale, void* stream);
+size_t tm_embed_grad_workspace_bytes(int64_t tokens, int64_t vocab, int64_t cols);
+int tm_embed_grad(void* d_dw, int w_f32, int64_t ldw, const void* d_dy, int y_f32, int64_t lddy, const void* d_ids, int ids64,
+                  int64_t tokens, int64_t vocab, int64_t cols, float scale, int64_t padding, int add, void* d_ws,
+                  size_t ws_bytes, void* stream);
+
+/*
  * Activations held in 8 bits between forward and backward: e4m3 values (rows ldv apart, ldv = cols' next
  * multiple of 32, padding zero, 16-byte aligned) and for each block of 32 rows x 32 columns the byte
  * e + 127 (ceil(rows / 32) x ceil(cols / 32)): e the least exponent with which the block's largest

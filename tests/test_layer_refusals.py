@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import torchure_amd as ta
-from torchure_amd import _native, norm
+from torchure_amd import _native, embed, norm
 
 BF16, F32, F16 = torch.bfloat16, torch.float32, torch.float16
 FAKE = 0x1000
@@ -20,10 +20,13 @@ def ones(*shape, dtype=BF16):
 @pytest.fixture
 def no_device(monkeypatch):
     monkeypatch.setattr(norm, "_on_gpu", lambda t, who, what: None)
+    monkeypatch.setattr(embed, "_on_gpu", lambda t, who, what: None)
 
 
 def test_cpu_tensors():
-    for call in (lambda: ta.rms_norm(ones(3, 4)), lambda: ta.layer_norm(ones(3, 4), ones(4), ones(4))):
+    for call in (lambda: ta.rms_norm(ones(3, 4)), lambda: ta.layer_norm(ones(3, 4), ones(4), ones(4)),
+                 lambda: ta.embedding(torch.arange(3), ones(4, 5)),
+                 lambda: ta.embedding_grad_(ones(4, 5), torch.arange(3), ones(3, 5))):
         with pytest.raises(RuntimeError, match="ROCm GPU"):
             call()
 
@@ -88,3 +91,84 @@ def test_norm_checks_without_gpu():
         assert lib.tm_norm_backward(*args) < 0 and b"tm_norm_backward" in lib.tm_last_error(), (at, bad)
         assert b"launch" not in lib.tm_last_error(), (at, bad)
     assert lib.tm_norm_backward(None, None, None, *good[3:18], None, 0, None) == 0  # nothing wanted
+
+
+IDS = torch.arange(3)
+
+
+@pytest.mark.parametrize("args,error,match", [
+    (dict(ids=IDS.float()), NotImplementedError, "ids must be"),
+    (dict(ids=IDS.to(torch.int16)), NotImplementedError, "ids must be"),
+    (dict(weight=ones(4, 5, dtype=F16)), NotImplementedError, "weight must be"),
+    (dict(weight=ones(4)), RuntimeError, "weight of shape"),
+    (dict(weight=ones(2, 4, 5)), RuntimeError, "weight of shape"),
+    (dict(weight=ones(0, 5)), RuntimeError, "weight of shape"),
+    (dict(weight=ones(4, 0)), RuntimeError, "weight of shape"),
+    (dict(weight=torch.eye(4).to_sparse()), NotImplementedError, "dense"),
+    (dict(padding_idx=4), ValueError, "padding_idx"),
+    (dict(padding_idx=-5), ValueError, "padding_idx"),
+    (dict(dtype=F16), NotImplementedError, "dtype"),
+])
+def test_embedding(no_device, args, error, match):
+    with pytest.raises(error, match=match):
+        ta.embedding(**{"ids": IDS, "weight": ones(4, 5), **args})
+
+
+@pytest.mark.parametrize("args,error,match", [
+    (dict(grad=ones(4, 5, dtype=F16)), NotImplementedError, "grad must be"),
+    (dict(dy=ones(3, 5, dtype=F16)), NotImplementedError, "dy must be"),
+    (dict(dy=ones(3, 4)), RuntimeError, "dy of shape"),
+    (dict(dy=ones(5)), RuntimeError, "dy of shape"),
+    (dict(dy=ones(1, 3, 5)), RuntimeError, "dy of shape"),
+    (dict(grad=ones(5, 4).t()), RuntimeError, "strides"),
+    (dict(grad=ones(1, 5).expand(4, 5)), RuntimeError, "strides"),
+    (dict(grad=ones(4, 10)[:, ::2]), RuntimeError, "strides"),
+    (dict(grad=ones(4, 5).requires_grad_()), RuntimeError, "requires a gradient"),
+    (dict(padding_idx=7), ValueError, "padding_idx"),
+])
+def test_embedding_grad(no_device, args, error, match):
+    with pytest.raises(error, match=match):
+        ta.embedding_grad_(**{"grad": ones(4, 5), "ids": IDS, "dy": ones(3, 5), **args})
+
+
+def test_embedding_grad_into_its_own_input(no_device):
+    table = ones(8, 5)
+    with pytest.raises(RuntimeError, match="share memory"):
+        ta.embedding_grad_(table, IDS, table[5:])
+    with pytest.raises(RuntimeError, match="share memory"):
+        ta.embedding_grad_(table[:6], IDS, table[5:])
+
+
+def test_no_tokens(no_device):
+    y = ta.embedding(IDS[:0].view(0, 1), ones(4, 5).requires_grad_(), dtype=F32)
+    assert y.shape == (0, 1, 5) and y.dtype == F32 and y.grad_fn is not None
+    table = ones(4, 5)
+    assert ta.embedding_grad_(table, IDS[:0], ones(0, 5)) is table
+
+
+def test_embedding_checks_without_gpu():
+    lib = _native.lib()
+    #       y     f  w     f  ldw ids   64 tokens vocab cols scale
+    good = [FAKE, 0, FAKE, 0, 40, FAKE, 1, 33, 100, 40, 1.0, None]
+    for at, bad in ((0, None), (0, 0x1001), (2, None), (2, 0x1001), (4, 39), (5, None), (5, 0x1004), (7, -1), (7, (1 << 30) + 1), (8, 0),
+                    (8, (1 << 30) + 1), (9, 0), (9, (1 << 20) + 1)):
+        args = list(good)
+        args[at] = bad
+        assert lib.tm_embed_lookup(*args) < 0 and b"tm_embed_lookup" in lib.tm_last_error(), (at, bad)
+        assert b"launch" not in lib.tm_last_error(), (at, bad)
+    assert lib.tm_embed_lookup(*good[:7], 0, 100, 40, 1.0, None) == 0  # nothing to do
+    need = lib.tm_embed_grad_workspace_bytes(33, 100, 40)
+    assert need == 16 + 2 * 144 + 8 * 256 + 8 * 2 * 40
+    for bad in ((0, 100, 40), (33, 0, 40), (33, 100, 0), ((1 << 30) + 1, 100, 40)):
+        assert lib.tm_embed_grad_workspace_bytes(*bad) == 0
+    #       dw    f  ldw dy    f  lddy ids  64 tokens vocab cols scale pad add ws
+    good = [FAKE, 0, 40, FAKE, 0, 40, FAKE, 1, 33, 100, 40, 1.0, -1, 0, FAKE, need, None]
+    for at, bad in ((0, None), (0, 0x1001), (2, 39), (3, None), (3, 0x1001), (5, 39), (6, None), (6, 0x1004), (8, 0), (8, -1), (9, 0), (10, 0),
+                    (14, None), (14, 0x1008), (15, need - 1)):
+        args = list(good)
+        args[at] = bad
+        assert lib.tm_embed_grad(*args) < 0 and b"tm_embed_grad" in lib.tm_last_error(), (at, bad)
+        assert b"launch" not in lib.tm_last_error(), (at, bad)
+    big = (1 << 30, 100, 1 << 12)
+    args = [FAKE, 0, 1 << 12, FAKE, 0, 1 << 12, FAKE, 1, *big, 1.0, -1, 0, FAKE, lib.tm_embed_grad_workspace_bytes(*big), None]
+    assert lib.tm_embed_grad(*args) < 0 and b"too large" in lib.tm_last_error()

@@ -7,6 +7,7 @@ through a C ABI (include/torchure_amd.h, libtorchure_amd.so).
 
 from torchure_amd import _native
 from torchure_amd.core.grad_helper import clip_grad_norm
+from torchure_amd.embed import embedding, embedding_grad_
 from torchure_amd.linear import (
     QuantizedActivation,
     dequantize_activation,
@@ -29,6 +30,8 @@ __all__ = [
     "clip_grad_norm",
     "fused_linear",
     "swiglu_mlp",
+    "embedding",
+    "embedding_grad_",
     "layer_norm",
     "rms_norm",
     "quantize_activation",

@@ -159,6 +159,16 @@ _SIGNATURES = {
         [_vp, _vp, _vp, ctypes.c_int, _vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _vp, _vp, _vp, ctypes.c_int,
          ctypes.c_int, ctypes.c_int, _i64, _i64, _vp, ctypes.c_size_t, _vp],
     ),
+    "tm_embed_lookup": (
+        ctypes.c_int,
+        [_vp, ctypes.c_int, _vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _i64, _i64, ctypes.c_float, _vp],
+    ),
+    "tm_embed_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "tm_embed_grad": (
+        ctypes.c_int,
+        [_vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _vp, ctypes.c_int, _i64, _i64, _i64, ctypes.c_float, _i64,
+         ctypes.c_int, _vp, ctypes.c_size_t, _vp],
+    ),
     "tm_quantize_e4m3": (ctypes.c_int, [_vp, _vp, _i64, _vp, ctypes.c_int, _i64, _i64, _i64, _vp, _i64, _vp]),
     "tm_dequantize_e4m3": (ctypes.c_int, [_vp, ctypes.c_int, _i64, _vp, _vp, _i64, _i64, _i64, _vp]),
     "tm_held_gate": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, ctypes.c_int, _i64, _i64, _vp]),
@@ -250,7 +260,7 @@ _LAYER_HOST = None
 
 
 def layer_host():
-    """``host()`` with the norms' C entry points bound."""
+    """``host()`` with the norms' and the embedding's C entry points bound."""
     global _LAYER_HOST
     if _LAYER_HOST is None:
         handle = lib()

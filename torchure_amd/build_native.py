@@ -7,7 +7,7 @@
 - _tm_host.<ext>.so: host-side list primitives and the host side of the fused CE and of the linear
   layers (CPU code) as a Python extension, with g++ against torch's headers and libraries.
 
-Both are compiled in parallel.
+All sources are compiled in parallel.
 """
 
 from __future__ import annotations
@@ -15,11 +15,12 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import tempfile
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(_HERE)
 SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("tm_optim.hip", "tm_ce.hip", "tm_ce_gemm.hip", "tm_linear.hip", "tm_act.hip",
-                                                  "tm_adamw8.hip", "tm_norm.hip")]
+                                                  "tm_adamw8.hip", "tm_norm.hip", "tm_embed.hip")]
 INCLUDE = os.path.join(ROOT, "include")
 OUTPUT = os.path.join(_HERE, "libtorchure_amd.so")
 ARCH = "gfx950"
@@ -32,20 +33,17 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found")
 
 
-def command(output: str = OUTPUT, extra: list[str] | None = None) -> list[str]:
-    return [
-        hipcc(),
-        f"--offload-arch={ARCH}",
-        "-O3",
-        "-std=c++17",
-        "-fPIC",
-        "-shared",
-        "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-        f"-I{INCLUDE}",
-        *(extra or []),
-        "-o", output,
-        *SOURCES,
-    ]
+FLAGS = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+         f"-I{INCLUDE}"]
+
+
+def command(output: str, source: str, extra: list[str] | None = None) -> list[str]:
+    """One source's object."""
+    return [hipcc(), *FLAGS, *(extra or []), "-c", source, "-o", output]
+
+
+def link_command(output: str, objects: list[str]) -> list[str]:
+    return [hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", "-o", output, *objects]
 
 
 HOST_SOURCES = [os.path.join(_HERE, "csrc", f) for f in ("tm_host.cpp", "tm_ce_host.cpp", "tm_lin_host.cpp", "tm_layer_host.cpp")]
@@ -80,23 +78,30 @@ def _start(cmd: list[str]) -> subprocess.Popen:
 
 
 def build(verbose: bool = False) -> str:
-    """Always recompiles both libraries; each is written to a temporary name and renamed
-    into place. Returns the kernel library's path."""
-    jobs = []
-    for out, cmd_of, what in ((OUTPUT, command, "hipcc"), (host_output(), host_command, "g++")):
-        tmp = out + ".tmp"
-        jobs.append((out, tmp, what, _start(cmd_of(tmp))))
+    """Always recompiles both libraries, all sources at once; each is written to a temporary name and renamed into place. Returns the
+    kernel library's path."""
     errors = []
-    for out, tmp, what, proc in jobs:
+
+    def finish(what: str, proc: subprocess.Popen) -> None:
         stdout, stderr = proc.communicate()
         if proc.returncode != 0:
             errors.append(f"{what} failed:\n{stdout}\n{stderr}")
-            continue
-        if verbose and stderr:
+        elif verbose and stderr:
             print(stderr)
-        os.replace(tmp, out)
+
+    with tempfile.TemporaryDirectory(prefix="tm_build_") as room:
+        objects = [os.path.join(room, os.path.basename(src) + ".o") for src in SOURCES]
+        tmp, host_tmp = OUTPUT + ".tmp", host_output() + ".tmp"
+        jobs = [("g++", _start(host_command(host_tmp)))]
+        jobs += [(f"hipcc {os.path.basename(src)}", _start(command(obj, src))) for obj, src in zip(objects, SOURCES)]
+        for what, proc in jobs:
+            finish(what, proc)
+        if not errors:
+            finish("hipcc (link)", _start(link_command(tmp, objects)))
     if errors:
         raise RuntimeError("\n".join(errors))
+    os.replace(tmp, OUTPUT)
+    os.replace(host_tmp, host_output())
     return OUTPUT
 
 

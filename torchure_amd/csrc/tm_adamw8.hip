@@ -63,14 +63,14 @@ constexpr int kRootLow = 40;  // the least byte of a root's exponent
 // Global-address-space accesses, past the caches: every byte is touched once. (Cached loads or stores in the step: 5.5 TB/s;
 // the codes that moments8_kernel reads alone are faster through them, 6.16 TB/s for 5.85.)
 #define TM_GLOBAL __attribute__((address_space(1)))
-template <typename T, bool kCached = false>
-__device__ __forceinline__ T ld(const void* p) {
-  if constexpr (kCached) return *(const TM_GLOBAL T*)p;
-  else return __builtin_nontemporal_load((const TM_GLOBAL T*)p);
+// (Types of their elements' alignment; a template's argument would lose it.)
+template <bool kCached>
+__device__ __forceinline__ uint32_t load_bytes(const uint8_t* p) {
+  const auto* q = (const TM_GLOBAL u32_at1*)p;
+  return kCached ? *q : __builtin_nontemporal_load(q);
 }
-template <typename T, typename V>
-__device__ __forceinline__ void st(void* p, V v) {
-  __builtin_nontemporal_store(static_cast<T>(v), (TM_GLOBAL T*)p);
+__device__ __forceinline__ void store_bytes(uint8_t* p, uint32_t v) {
+  __builtin_nontemporal_store(static_cast<u32_at1>(v), (TM_GLOBAL u32_at1*)p);
 }
 
 // ---------------------------------------------------------------- random bits
@@ -181,13 +181,13 @@ template <bool kCached = false>
 __device__ __forceinline__ Codes load_codes(const tm_tensor_t& d, int64_t codes, int64_t e) {
   const uint8_t* m = reinterpret_cast<const uint8_t*>(d.exp_avg);
   const uint8_t* r = reinterpret_cast<const uint8_t*>(d.exp_avg_sq);
-  return {ld<u32_at1, kCached>(m + e), ld<u32_at1, kCached>(r + e), m[codes + e / kBlock], r[codes + e / kBlock]};
+  return {load_bytes<kCached>(m + e), load_bytes<kCached>(r + e), m[codes + e / kBlock], r[codes + e / kBlock]};
 }
 __device__ __forceinline__ void store_codes(const tm_tensor_t& d, int64_t codes, int64_t e, const Codes& c) {
   uint8_t* m = reinterpret_cast<uint8_t*>(d.exp_avg);
   uint8_t* r = reinterpret_cast<uint8_t*>(d.exp_avg_sq);
-  st<u32_at1>(m + e, c.m);
-  st<u32_at1>(r + e, c.r);
+  store_bytes(m + e, c.m);
+  store_bytes(r + e, c.r);
   if ((threadIdx.x & 15) == 0) {
     m[codes + e / kBlock] = static_cast<uint8_t>(c.me);
     r[codes + e / kBlock] = static_cast<uint8_t>(c.re);
@@ -200,7 +200,7 @@ template <bool kWhole>
 __device__ __forceinline__ void load_f32(float* v, uint64_t base, int64_t e, int left) {
   const float* p = reinterpret_cast<const float*>(base) + e;
   if (kWhole || left == 4) {
-    const f32x4 a = ld<f32x4_at4>(p);
+    const f32x4 a = __builtin_nontemporal_load((const TM_GLOBAL f32x4_at4*)p);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
   } else {
 #pragma unroll
@@ -211,7 +211,8 @@ template <bool kWhole>
 __device__ __forceinline__ void store_f32(uint64_t base, int64_t e, int left, const float* v) {
   float* p = reinterpret_cast<float*>(base) + e;
   if (kWhole || left == 4) {
-    st<f32x4_at4>(p, (f32x4{v[0], v[1], v[2], v[3]}));
+    const f32x4_at4 a = f32x4{v[0], v[1], v[2], v[3]};
+    __builtin_nontemporal_store(a, (TM_GLOBAL f32x4_at4*)p);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -222,7 +223,7 @@ template <bool kWhole>
 __device__ __forceinline__ void load_bf16(float* v, uint64_t base, int64_t e, int left) {
   const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + e;
   if (kWhole || left == 4) {
-    const u32x2 w = ld<u32x2_at2>(p);
+    const u32x2 w = __builtin_nontemporal_load((const TM_GLOBAL u32x2_at2*)p);
     v[0] = bf16_lo(w.x); v[1] = bf16_hi(w.x); v[2] = bf16_lo(w.y); v[3] = bf16_hi(w.y);
   } else {
 #pragma unroll
@@ -232,9 +233,9 @@ __device__ __forceinline__ void load_bf16(float* v, uint64_t base, int64_t e, in
 template <bool kWhole>
 __device__ __forceinline__ void store_bf16(uint64_t base, int64_t e, int left, const float* v) {
   uint16_t* p = reinterpret_cast<uint16_t*>(base) + e;
-  const u32x2 w = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+  const u32x2_at2 w = u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
   if (kWhole || left == 4) {
-    st<u32x2_at2>(p, w);
+    __builtin_nontemporal_store(w, (TM_GLOBAL u32x2_at2*)p);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)

@@ -1,7 +1,7 @@
-// tm_layer_host.cpp -- host side of the norms (CPU code only): makes the results and workspaces and reaches the kernels
+// tm_layer_host.cpp -- host side of the norms and the embedding (CPU code only): makes the results and workspaces and reaches the kernels
 // through the C ABI (include/torchure_amd.h). The autograd functions are C++ too: a norm's kernels take 10 to 100 us, and a
 // function in Python, with the lock that its backward pass takes on the engine's thread, as much again on the host. Arguments come checked
-// from norm.py.
+// from norm.py and embed.py.
 
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -24,6 +24,9 @@ struct Abi {
   decltype(&tm_norm_forward) norm_forward;
   decltype(&tm_norm_workspace_bytes) norm_bytes;
   decltype(&tm_norm_backward) norm_backward;
+  decltype(&tm_embed_lookup) lookup;
+  decltype(&tm_embed_grad_workspace_bytes) embed_bytes;
+  decltype(&tm_embed_grad) embed_grad;
   decltype(&tm_last_error) last_error;
   py::object native_error;
 };
@@ -36,6 +39,9 @@ void layer_bind(const py::dict& addresses, const py::object& native_error) {
   a->norm_forward = reinterpret_cast<decltype(a->norm_forward)>(at("tm_norm_forward"));
   a->norm_bytes = reinterpret_cast<decltype(a->norm_bytes)>(at("tm_norm_workspace_bytes"));
   a->norm_backward = reinterpret_cast<decltype(a->norm_backward)>(at("tm_norm_backward"));
+  a->lookup = reinterpret_cast<decltype(a->lookup)>(at("tm_embed_lookup"));
+  a->embed_bytes = reinterpret_cast<decltype(a->embed_bytes)>(at("tm_embed_grad_workspace_bytes"));
+  a->embed_grad = reinterpret_cast<decltype(a->embed_grad)>(at("tm_embed_grad"));
   a->last_error = reinterpret_cast<decltype(a->last_error)>(at("tm_last_error"));
   a->native_error = native_error;
   g_abi = a;
@@ -181,10 +187,99 @@ bool norm_plain(const Tensor& x, const Opt& weight, const Opt& bias, int device)
   return true;
 }
 
+// ---------------------------------------------------------------- embedding
+
+struct Embed {
+  double scale;
+  i64 padding;
+  bool y_f32;
+  void* stream;
+};
+
+bool wide(const Tensor& ids) { return ids.scalar_type() == at::kLong; }
+
+Tensor lookup(const Tensor& ids, const Tensor& weight, const Embed& e) {
+  const OnDevice on(weight);
+  const Rows w = rows_of(weight);
+  std::vector<i64> sizes(ids.sizes().begin(), ids.sizes().end());
+  sizes.push_back(w.d);
+  const Tensor y = room(weight, sizes, type_of(e.y_f32));
+  check(abi().lookup(ptr(y), e.y_f32, ptr(w.t), is_f32(w.t), w.ld, ptr(ids), wide(ids), ids.numel(), w.n, w.d,
+                     static_cast<float>(e.scale), e.stream),
+        "tm_embed_lookup");
+  return y;
+}
+
+// dw = the gradient, or, with `add`, dw += it.
+void table_grad(const Tensor& dw, i64 ldw, const Tensor& dy, const Tensor& ids, double scale, i64 padding, bool add, void* stream) {
+  const OnDevice on(dy);
+  const Rows d = rows_of(dy);
+  const size_t need = abi().embed_bytes(ids.numel(), dw.size(0), dw.size(1));
+  const Tensor ws = room(dy, {static_cast<i64>(need)}, at::kByte);
+  check(abi().embed_grad(ptr(dw), is_f32(dw), ldw, ptr(d.t), is_f32(d.t), d.ld, ptr(ids), wide(ids), ids.numel(), dw.size(0),
+                         dw.size(1), static_cast<float>(scale), padding, add, ptr(ws), need, stream),
+        "tm_embed_grad");
+}
+
+struct EmbedFunction : torch::autograd::Function<EmbedFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, const Embed& e) {
+    const Tensor kept = ids.contiguous();
+    ctx->save_for_backward({kept});
+    ctx->saved_data["vocab"] = weight.size(0);
+    ctx->saved_data["f32"] = is_f32(weight);
+    ctx->saved_data["scale"] = e.scale;
+    ctx->saved_data["padding"] = e.padding;
+    ctx->saved_data["stream"] = reinterpret_cast<i64>(e.stream);
+    return lookup(kept, weight, e);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor& dy = grads[0];
+    const Tensor ids = ctx->get_saved_variables()[0].contiguous();
+    Tensor dw;
+    {
+      const at::AutoGradMode no_grad(false);
+      dw = room(dy, {ctx->saved_data["vocab"].toInt(), dy.size(-1)}, type_of(ctx->saved_data["f32"].toBool()));
+      table_grad(dw, dw.size(1), dy, ids, ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), false,
+                 reinterpret_cast<void*>(ctx->saved_data["stream"].toInt()));
+    }
+    return once({Tensor(), dw, Tensor()});
+  }
+};
+
+Tensor embedding(const Tensor& ids, const Tensor& weight, double scale, i64 padding, bool y_f32, uintptr_t stream) {
+  HANDLE_TH_ERRORS
+  return without_gil([&] {
+    const Embed e = {scale, padding, y_f32, reinterpret_cast<void*>(stream)};
+    const bool record = at::GradMode::is_enabled() && wants_grad(weight);
+    return record ? EmbedFunction::apply(ids, weight, e) : lookup(ids.contiguous(), weight, e);
+  });
+  END_HANDLE_TH_ERRORS_PYBIND
+}
+
+void embedding_grad(const Tensor& grad, const Tensor& ids, const Tensor& dy, double scale, i64 padding, uintptr_t stream) {
+  HANDLE_TH_ERRORS
+  without_gil([&] {
+    const at::AutoGradMode no_grad(false);
+    table_grad(grad, grad.size(0) > 1 ? grad.stride(0) : grad.size(1), dy, ids.contiguous(), scale, padding, true,
+               reinterpret_cast<void*>(stream));
+  });
+  END_HANDLE_TH_ERRORS_PYBIND
+}
+
+// As norm_plain, for a lookup.
+bool embedding_plain(const Tensor& ids, const Tensor& weight, int device) {
+  return plain(weight, device) && weight.dim() == 2 && weight.numel() > 0 && ids.is_cuda() && ids.layout() == at::kStrided &&
+         ids.device().index() == device && (wide(ids) || ids.scalar_type() == at::kInt) && ids.numel() > 0;
+}
+
 }  // namespace
 
 void tm_layer_host_bind(py::module_& m) {
-  m.def("layer_bind", &layer_bind, "addresses of the C ABI's norm entry points, and the exception of a failed call");
+  m.def("layer_bind", &layer_bind, "addresses of the C ABI's norm and embedding entry points, and the exception of a failed call");
   m.def("norm", &norm, "a norm, with its gradients where they are wanted");
+  m.def("embedding", &embedding, "rows of a table by id, with the table's gradient where it is wanted");
+  m.def("embedding_grad", &embedding_grad, "the table's gradient, added to one that is there");
+  m.def("embedding_plain", &embedding_plain, "whether a lookup needs none of the other checks");
   m.def("norm_plain", &norm_plain, "whether a call needs none of the other checks");
 }

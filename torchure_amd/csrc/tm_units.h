@@ -17,17 +17,6 @@ using tm_act::u32x4_at2;
 using tm_act::u32x4_at4;
 typedef u32x2 u32x2_at2 __attribute__((aligned(2)));
 
-template <bool kStream, typename T>
-__device__ __forceinline__ T load(const T* p) {
-  if constexpr (kStream) return __builtin_nontemporal_load(p);
-  else return *p;
-}
-template <bool kStream, typename T, typename V>
-__device__ __forceinline__ void store(T* p, V v) {
-  if constexpr (kStream) __builtin_nontemporal_store(static_cast<T>(v), p);
-  else *p = v;
-}
-
 // A unit as it was read.
 template <bool kF32, int kU>
 struct Raw {
@@ -42,7 +31,8 @@ __device__ __forceinline__ Raw<kF32, kU> read(const void* base, int64_t at, int 
   if constexpr (kF32) {
     const uint32_t* p = static_cast<const uint32_t*>(base) + at;
     if (left >= 4) {
-      const u32x4 a = load<kStream>(reinterpret_cast<const u32x4_at4*>(p));
+      const auto* q = reinterpret_cast<const u32x4_at4*>(p);
+      const u32x4 a = kStream ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
       for (int i = 0; i < 4; ++i) r.w[i] = a[i];
     } else {
@@ -54,11 +44,13 @@ __device__ __forceinline__ Raw<kF32, kU> read(const void* base, int64_t at, int 
     const uint16_t* p = static_cast<const uint16_t*>(base) + at;
     if (left >= kU) {
       if constexpr (kU == 8) {
-        const u32x4 a = load<kStream>(reinterpret_cast<const u32x4_at2*>(p));
+        const auto* q = reinterpret_cast<const u32x4_at2*>(p);
+        const u32x4 a = kStream ? __builtin_nontemporal_load(q) : *q;
 #pragma unroll
         for (int i = 0; i < 4; ++i) r.w[i] = a[i];
       } else {
-        const u32x2 a = load<kStream>(reinterpret_cast<const u32x2_at2*>(p));
+        const auto* q = reinterpret_cast<const u32x2_at2*>(p);
+        const u32x2 a = kStream ? __builtin_nontemporal_load(q) : *q;
         r.w[0] = a.x;
         r.w[1] = a.y;
       }
@@ -90,8 +82,10 @@ __device__ __forceinline__ void put(void* base, int64_t at, const float (&v)[kU]
   if constexpr (kF32) {
     float* p = static_cast<float*>(base) + at;
     if (left >= 4) {
-      store<kStream>(reinterpret_cast<u32x4_at4*>(p), (u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]),
-                                                             __float_as_uint(v[2]), __float_as_uint(v[3])}));
+      auto* q = reinterpret_cast<u32x4_at4*>(p);
+      const u32x4_at4 a = u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+      if constexpr (kStream) __builtin_nontemporal_store(a, q);
+      else *q = a;
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -103,8 +97,17 @@ __device__ __forceinline__ void put(void* base, int64_t at, const float (&v)[kU]
 #pragma unroll
     for (int i = 0; i < kU / 2; ++i) w[i] = tm_act::pack_bf16(v[2 * i], v[2 * i + 1]);
     if (left >= kU) {
-      if constexpr (kU == 8) store<kStream>(reinterpret_cast<u32x4_at2*>(p), (u32x4{w[0], w[1], w[2], w[3]}));
-      else store<kStream>(reinterpret_cast<u32x2_at2*>(p), (u32x2{w[0], w[1]}));
+      if constexpr (kU == 8) {
+        auto* q = reinterpret_cast<u32x4_at2*>(p);
+        const u32x4_at2 a = u32x4{w[0], w[1], w[2], w[3]};
+        if constexpr (kStream) __builtin_nontemporal_store(a, q);
+        else *q = a;
+      } else {
+        auto* q = reinterpret_cast<u32x2_at2*>(p);
+        const u32x2_at2 a = u32x2{w[0], w[1]};
+        if constexpr (kStream) __builtin_nontemporal_store(a, q);
+        else *q = a;
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < kU; ++i)
