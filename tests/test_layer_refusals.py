@@ -172,3 +172,41 @@ def test_embedding_checks_without_gpu():
     big = (1 << 30, 100, 1 << 12)
     args = [FAKE, 0, 1 << 12, FAKE, 0, 1 << 12, FAKE, 1, *big, 1.0, -1, 0, FAKE, lib.tm_embed_grad_workspace_bytes(*big), None]
     assert lib.tm_embed_grad(*args) < 0 and b"too large" in lib.tm_last_error()
+
+
+def test_adamw_state_bits():
+    p = torch.nn.Parameter(torch.zeros(4))
+    for bits in (16, 4, 0, "8", None, 8.5):
+        with pytest.raises(ValueError, match="state_bits"):
+            ta.AdamW([p], state_bits=bits)
+    for seed in (-1, 1 << 64):
+        with pytest.raises(ValueError, match="seed"):
+            ta.AdamW([p], state_bits=8, seed=seed)
+    for seed in (1.5, "1", None):
+        with pytest.raises(TypeError):
+            ta.AdamW([p], state_bits=8, seed=seed)
+    opt = ta.AdamW([p], state_bits=8, seed=(1 << 64) - 1)
+    with pytest.raises(RuntimeError, match="no param has state"):
+        opt.flat_moments()
+    with pytest.raises(RuntimeError, match="state_bits=32"):
+        ta.AdamW([p]).flat_moments()
+
+
+def test_8_bit_moments_checks_without_gpu():
+    lib = _native.lib()
+    for n, size in ((-1, 0), (0, 0), (1, 260), (256, 260), (257, 520), (1 << 33, (1 << 33) * 65 // 64)):
+        assert lib.tm_moments8_bytes(n) == size
+    groups = (_native.TmHyper * 2)()
+    #       tensors n  chunks n  elems
+    table = [FAKE, 3, FAKE, 5, 65536]
+    wrong = ((0, None), (1, -1), (1, 1 << 32), (2, None), (3, -1), (3, 1 << 32), (4, 0), (4, -256), (4, 65537), (4, 1 << 31))
+    for name, rest in (("tm_adamw8_step", [groups, 2, None, 7, FAKE, None]), ("tm_moments8_read", [None]), ("tm_moments8_write", [None])):
+        for at, bad in wrong:
+            args = table + rest
+            args[at] = bad
+            assert getattr(lib, name)(*args) < 0 and name.encode() in lib.tm_last_error(), (name, at, bad)
+            assert b"launch" not in lib.tm_last_error(), (name, at, bad)
+    for at, bad in ((5, None), (6, 0), (6, -1), (6, _native.TM_MAX_GROUPS + 1), (9, None)):
+        args = table + [groups, 2, None, 7, FAKE, None]
+        args[at] = bad
+        assert lib.tm_adamw8_step(*args) < 0 and b"tm_adamw8_step" in lib.tm_last_error(), (at, bad)

@@ -39,6 +39,8 @@ into both.
 
 from __future__ import annotations
 
+import operator
+
 import numpy as np
 import torch
 import weakref
@@ -162,12 +164,13 @@ class AdamW(torch.optim.Optimizer):
         }
         if state_bits not in (8, 32):
             raise ValueError(f"torchure_amd.AdamW: state_bits must be 32 or 8, got {state_bits!r}")
-        if not 0 <= int(seed) < 1 << 64:
+        seed = operator.index(seed)
+        if not 0 <= seed < 1 << 64:
             raise ValueError(f"torchure_amd.AdamW: seed must be in [0, 2^64), got {seed}")
         self.chunk_elems = tables.check_chunk_elems(chunk_elems)
         self.defer_clip = bool(defer_clip)
         self.state_bits = int(state_bits)
-        self.seed = int(seed)
+        self.seed = seed
         self._pending = None  # (coef device tensor, _ClipRecord)
         self._uploader = tables.TableUploader()
         self._uploader_read = tables.TableUploader()  # flat_moments' tables
