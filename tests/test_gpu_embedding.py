@@ -118,6 +118,13 @@ def test_many_tokens(kind):
     check(ids_of(kind, 150_001, 4096, g), 4096, 64, scale=0.5)
 
 
+@pytest.mark.parametrize("n", [2047, 2049, 4097, 8191, 8193, 20000])
+@pytest.mark.parametrize("vocab", [1, 2, 300])
+def test_more_of_an_id_than_wait_at_once(vocab, n):
+    g = torch.Generator(device=DEV).manual_seed(n)
+    check(ids_of("text", n, vocab, g), vocab, 40, BF16, padding=vocab - 1 if vocab > 2 else None, seed=n)
+
+
 @pytest.mark.parametrize("scale", [0.0, -1.0, 1e-3, 32.0, 27.875])
 def test_scales(scale):
     g = torch.Generator(device=DEV).manual_seed(6)

@@ -7,10 +7,12 @@
 // so that its bits are the same every time:
 //
 //   1. Tokens by id. Workgroup b has the ids with id % B = b (so that a vocabulary's frequent, low ids spread over
-//      all of them). It reads all ids twice: first it counts, in LDS, its own ids and the tokens of the workgroups before it,
-//      which places its part of the list; then it puts its tokens' positions there in order, 1024 ids at a time: those that
-//      match wait in a queue in their order, and a queue's entry goes behind as many as there are equal ones before it.
-//      An id that is out of range or the padding's is on no list.
+//      all of them). It reads all ids twice, eight a lane on their way together (one after the other they took 49 latencies
+//      each time of 50,001 tokens): first it counts, in LDS, its own ids and the tokens of the workgroups before it, which places its
+//      part of the list; then those that match wait in a queue in their order. Of 64 neighbours in a queue a wave finds each one's
+//      equals by ballots, and the 64s take their places from the ids' cursors one after the other (ranked by comparing
+//      with all before, 50,001 tokens of which an eighth had one id took the workgroup that has it 104 us; so 40). An id that is out of
+//      range or the padding's is on no list.
 //   2. Sums. A wave takes 32 entries of the list and one panel of columns, adds rows in order, and writes a
 //      sum out where the id changes: to the table if all of the id's entries are its own, else to a partial sum. The other workgroups of
 //      the launch fill the rows of ids that do not occur with zeros, which is most of the bytes.
@@ -96,7 +98,12 @@ __global__ __launch_bounds__(256) void lookup_kernel(Lookup a) {
 
 // ---------------------------------------------------------------- 1. tokens by id
 
-constexpr int kGroupThreads = 1024, kMostLocal = 8192, kQueue = 2048;
+constexpr int kGroupThreads = 1024, kGroupWaves = kGroupThreads / kWave, kMostLocal = 8192;
+constexpr int kIds = 8;                                // ids a lane has on their way
+constexpr int kQueue = 2048;                             // entries that wait for their places
+constexpr int kPartWaves = kQueue / (kIds * kWave);    // waves of a round that surely fit
+constexpr int kParts = kGroupWaves / kPartWaves;
+static_assert(kQueue % kGroupThreads == 0 && kGroupWaves % kPartWaves == 0 && kMostLocal <= 1 << 16, "whole parts, 16-bit ids");
 
 struct Segment {
   int32_t start, count;
@@ -126,7 +133,7 @@ __device__ __forceinline__ int wave_before(int v) {
   return s - v;
 }
 
-// ... of the workgroup's threads, and of all in `sum`. `room`: 17 words; two barriers.
+// ... of the workgroup's threads, and of all in `sum`. `room`: a word a wave; two barriers.
 __device__ __forceinline__ int block_before(int v, int* room, int& sum) {
   const int wave = threadIdx.x >> 6, before = wave_before(v);
   __syncthreads();
@@ -135,7 +142,7 @@ __device__ __forceinline__ int block_before(int v, int* room, int& sum) {
   int base = 0;
   sum = 0;
 #pragma unroll
-  for (int i = 0; i < kGroupThreads / kWave; ++i) {
+  for (int i = 0; i < kGroupWaves; ++i) {
     const int s = room[i];
     if (i < wave) base += s;
     sum += s;
@@ -147,20 +154,33 @@ template <typename Id>
 __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(const Id* __restrict__ ids, int32_t n, int64_t vocab,
                                                                     int64_t padding, Lists t) {
   __shared__ int cursor[kMostLocal];
-  __shared__ int room[kGroupThreads / kWave];
+  __shared__ int room[kGroupWaves];
   __shared__ int queue_pos[kQueue];
-  __shared__ alignas(16) uint16_t queue_local[kQueue];
-  const int mask = (1 << t.log2_b) - 1, b = blockIdx.x, tid = threadIdx.x;
+  __shared__ uint16_t queue_local[kQueue];
+  constexpr int kRound = kGroupThreads * kIds;
+  const int mask = (1 << t.log2_b) - 1, b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   for (int i = tid; i < t.locals; i += kGroupThreads) cursor[i] = 0;
   __syncthreads();
   auto wanted = [&](int64_t id) { return static_cast<uint64_t>(id) < static_cast<uint64_t>(vocab) && id != padding; };
+  // The ids of one round, 512 neighbours a wave, all on their way together.
+  auto load = [&](int64_t (&id)[kIds], int64_t round) {
+#pragma unroll
+    for (int k = 0; k < kIds; ++k) {
+      const int64_t i = round + (wave * kIds + k) * kWave + l;
+      id[k] = i < n ? static_cast<int64_t>(ids[i]) : -1;
+    }
+  };
   int before = 0;
-  for (int i = tid; i < n; i += kGroupThreads) {
-    const int64_t id = ids[i];
-    if (!wanted(id)) continue;
-    const int bucket = static_cast<int>(id) & mask;
-    before += bucket < b;
-    if (bucket == b) atomicAdd(&cursor[static_cast<int>(id) >> t.log2_b], 1);
+  for (int64_t round = 0; round < n; round += kRound) {
+    int64_t id[kIds];
+    load(id, round);
+#pragma unroll
+    for (int k = 0; k < kIds; ++k) {
+      if (!wanted(id[k])) continue;
+      const int bucket = static_cast<int>(id[k]) & mask;
+      before += bucket < b;
+      if (bucket == b) atomicAdd(&cursor[static_cast<int>(id[k]) >> t.log2_b], 1);
+    }
   }
   int base = 0;
   block_before(before, room, base);  // (its barriers are behind the counts, too)
@@ -187,61 +207,98 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(const Id* __
   if (!all) return;  // (of the whole workgroup)
   __syncthreads();
 
-  // A queue's entries behind the equal ones before them.
+  // Puts a queue's entries in their places. Of 64 neighbours in it a wave finds each one's equals before it; the 64s then take their
+  // places from the cursors one after the other.
   int queued = 0;
   auto drain = [&] {
-    int dest[kQueue / kGroupThreads];
+    constexpr int kMine = kQueue / kGroupThreads;
+    int local[kMine], pos[kMine], rank[kMine], equal[kMine], dest[kMine];
 #pragma unroll
-    for (int k = 0; k < kQueue / kGroupThreads; ++k) {
-      const int q = tid + k * kGroupThreads;
-      dest[k] = -1;
-      if (q < queued) {
-        const uint32_t mine = queue_local[q];
-        int rank = 0, j = 0;
-        for (; j + 8 <= q; j += 8) {
-          const tm_act::u32x4 w = *reinterpret_cast<const tm_act::u32x4*>(queue_local + j);
-#pragma unroll
-          for (int h = 0; h < 4; ++h) rank += ((w[h] & 0xFFFFu) == mine) + ((w[h] >> 16) == mine);
+    for (int k = 0; k < kMine; ++k) {
+      const int q = (k * kGroupWaves + wave) * kWave + l;
+      const bool in = q < queued;
+      local[k] = in ? queue_local[q] : -1;
+      pos[k] = in ? queue_pos[q] : 0;
+      rank[k] = equal[k] = dest[k] = 0;
+      uint64_t left = __ballot(in);
+      while (left) {  // of the wave's lanes those of one id at a time
+        const int key = __builtin_amdgcn_readlane(local[k], __ffsll(static_cast<unsigned long long>(left)) - 1);
+        const uint64_t same = __ballot(local[k] == key);
+        if (local[k] == key) {
+          rank[k] = __popcll(same & ((uint64_t(1) << l) - 1));
+          equal[k] = __popcll(same);
         }
-        for (; j < q; ++j) rank += queue_local[j] == mine;
-        dest[k] = cursor[mine] + rank;
+        left &= ~same;
       }
     }
-    __syncthreads();
+    const int groups = (queued + kWave - 1) / kWave;
 #pragma unroll
-    for (int k = 0; k < kQueue / kGroupThreads; ++k) {
-      const int q = tid + k * kGroupThreads;
-      if (dest[k] >= 0) {
-        t.order[dest[k]] = queue_pos[q];
-        t.id[dest[k]] = (queue_local[q] << t.log2_b) | b;
-        atomicAdd(&cursor[queue_local[q]], 1);
+    for (int k = 0; k < kMine; ++k) {
+      const int end = min(groups, (k + 1) * kGroupWaves);
+      for (int g = k * kGroupWaves; g < end; ++g) {
+        if (g == k * kGroupWaves + wave && local[k] >= 0) {
+          const int at = cursor[local[k]];
+          dest[k] = at + rank[k];
+          if (rank[k] == 0) cursor[local[k]] = at + equal[k];
+        }
+        __syncthreads();
       }
     }
-    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      if (local[k] >= 0) {
+        t.order[dest[k]] = pos[k];
+        t.id[dest[k]] = (local[k] << t.log2_b) | b;
+      }
+    }
     queued = 0;
   };
-  for (int64_t tile = 0; tile < n; tile += kGroupThreads) {
-    const int64_t i = tile + tid;
-    const int64_t id = i < n ? static_cast<int64_t>(ids[i]) : -1;
-    const bool match = wanted(id) && (static_cast<int>(id) & mask) == b;
-    const uint64_t ballot = __ballot(match);
-    const int wave = tid >> 6, in_wave = __popcll(ballot & ((uint64_t(1) << (tid & 63)) - 1));
-    if ((tid & 63) == 0) room[wave] = __popcll(ballot);
-    __syncthreads();
-    int at = queued, found = 0;
+  for (int64_t round = 0; round < n; round += kRound) {
+    int64_t id[kIds];
+    load(id, round);
+    int local[kIds], in_wave[kIds], mine = 0;
 #pragma unroll
-    for (int w = 0; w < kGroupThreads / kWave; ++w) {
+    for (int k = 0; k < kIds; ++k) {
+      local[k] = wanted(id[k]) && (static_cast<int>(id[k]) & mask) == b ? static_cast<int>(id[k]) >> t.log2_b : -1;
+      const uint64_t ballot = __ballot(local[k] >= 0);
+      in_wave[k] = mine + __popcll(ballot & ((uint64_t(1) << l) - 1));
+      mine += __popcll(ballot);
+    }
+    if (l == 0) room[wave] = mine;
+    __syncthreads();
+    // the waves before this one, and those of each part: a part always fits an empty queue
+    int ahead = 0, part[kParts] = {}, found = 0;
+#pragma unroll
+    for (int w = 0; w < kGroupWaves; ++w) {
       const int s = room[w];
-      if (w < wave) at += s;
+      if (w < wave) ahead += s;
+      part[w / kPartWaves] += s;
       found += s;
     }
-    if (match) {
-      queue_pos[at + in_wave] = static_cast<int>(i);
-      queue_local[at + in_wave] = static_cast<uint16_t>(static_cast<int>(id) >> t.log2_b);
+    auto put_in = [&](int at) {
+#pragma unroll
+      for (int k = 0; k < kIds; ++k) {
+        if (local[k] >= 0) {
+          queue_pos[at + in_wave[k]] = static_cast<int>(round) + (wave * kIds + k) * kWave + l;
+          queue_local[at + in_wave[k]] = static_cast<uint16_t>(local[k]);
+        }
+      }
+    };
+    if (queued + found <= kQueue) {
+      put_in(queued + ahead);
+      queued += found;
+      __syncthreads();
+    } else {
+      if (queued) drain();
+#pragma unroll
+      for (int p = 0; p < kParts; ++p) {
+        if (wave / kPartWaves == p) put_in(ahead);
+        ahead -= part[p];
+        queued = part[p];
+        __syncthreads();
+        if (queued) drain();
+      }
     }
-    queued += found;
-    __syncthreads();
-    if (queued > kQueue - kGroupThreads) drain();
   }
   if (queued) drain();
 }
