@@ -17,6 +17,9 @@
 //      sum out where the id changes: to the table if all of the id's entries are its own, else to a partial sum. The other workgroups of
 //      the launch fill the rows of ids that do not occur with zeros, which is most of the bytes.
 //   3. Ids with entries in several waves: their partial sums, in order.
+//
+// Measured: 8192 tokens of 151,936 ids x 1024 in fp32: lookup 9 us, the three launches 10, 125 (656 MB at 5.2 TB/s; stores of zeros
+// alone reach 6.7) and 5. 50,001 of 4096 x 777 in bf16: 21; 40, 23 and 15.
 
 #include <hip/hip_runtime.h>
 
