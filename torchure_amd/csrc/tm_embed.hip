@@ -11,7 +11,7 @@
 //      each time of 50,001 tokens): first it counts, in LDS, its own ids and the tokens of the workgroups before it, which places its
 //      part of the list; then those that match wait in a queue in their order. Of 64 neighbours in a queue a wave finds each one's
 //      equals by ballots, and the 64s take their places from the ids' cursors one after the other (ranked by comparing
-//      with all before, 50,001 tokens of which an eighth had one id took the workgroup that has it 104 us; so 40). An id that is out of
+//      with all before, 50,001 tokens of which an eighth had one id took the workgroup that has it 104 us; so 37). An id that is out of
 //      range or the padding's is on no list.
 //   2. Sums. A wave takes 32 entries of the list and one panel of columns, adds rows in order, and writes a
 //      sum out where the id changes: to the table if all of the id's entries are its own, else to a partial sum. The other workgroups of
@@ -19,7 +19,7 @@
 //   3. Ids with entries in several waves: their partial sums, in order.
 //
 // Measured: 8192 tokens of 151,936 ids x 1024 in fp32: lookup 9 us, the three launches 10, 125 (656 MB at 5.2 TB/s; stores of zeros
-// alone reach 6.7) and 5. 50,001 of 4096 x 777 in bf16: 21; 40, 23 and 15.
+// alone reach 6.7) and 5. 50,001 of 4096 x 777 in bf16: 21; 37, 23 and 14.
 
 #include <hip/hip_runtime.h>
 
@@ -164,26 +164,28 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(const Id* __
   const int mask = (1 << t.log2_b) - 1, b = blockIdx.x, tid = threadIdx.x, wave = tid >> 6, l = tid & 63;
   for (int i = tid; i < t.locals; i += kGroupThreads) cursor[i] = 0;
   __syncthreads();
-  auto wanted = [&](int64_t id) { return static_cast<uint64_t>(id) < static_cast<uint64_t>(vocab) && id != padding; };
-  // The ids of one round, 512 neighbours a wave, all on their way together.
-  auto load = [&](int64_t (&id)[kIds], int64_t round) {
+  // A round's ids, 512 neighbours a wave, all on their way together (past the last token its id again: no branch, which would
+  // have each waited for by itself: 50,001 32-bit ids 55 us for 39); then f(k, id, whether it is on the list).
+  auto load = [&](Id (&id)[kIds], int round) {
+#pragma unroll
+    for (int k = 0; k < kIds; ++k) id[k] = ids[min(round + (wave * kIds + k) * kWave + l, n - 1)];
+  };
+  auto each = [&](const Id (&id)[kIds], int round, auto&& f) {
 #pragma unroll
     for (int k = 0; k < kIds; ++k) {
-      const int64_t i = round + (wave * kIds + k) * kWave + l;
-      id[k] = i < n ? static_cast<int64_t>(ids[i]) : -1;
+      const int i = round + (wave * kIds + k) * kWave + l;
+      const int64_t v = id[k];
+      f(k, static_cast<int>(v), i < n && static_cast<uint64_t>(v) < static_cast<uint64_t>(vocab) && v != padding);
     }
   };
   int before = 0;
-  for (int64_t round = 0; round < n; round += kRound) {
-    int64_t id[kIds];
+  for (int round = 0; round < n; round += kRound) {
+    Id id[kIds];
     load(id, round);
-#pragma unroll
-    for (int k = 0; k < kIds; ++k) {
-      if (!wanted(id[k])) continue;
-      const int bucket = static_cast<int>(id[k]) & mask;
-      before += bucket < b;
-      if (bucket == b) atomicAdd(&cursor[static_cast<int>(id[k]) >> t.log2_b], 1);
-    }
+    each(id, round, [&](int, int v, bool wanted) {
+      before += wanted && (v & mask) < b;
+      if (wanted && (v & mask) == b) atomicAdd(&cursor[v >> t.log2_b], 1);
+    });
   }
   int base = 0;
   block_before(before, room, base);  // (its barriers are behind the counts, too)
@@ -256,17 +258,16 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(const Id* __
     }
     queued = 0;
   };
-  for (int64_t round = 0; round < n; round += kRound) {
-    int64_t id[kIds];
+  for (int round = 0; round < n; round += kRound) {
+    Id id[kIds];
     load(id, round);
     int local[kIds], in_wave[kIds], mine = 0;
-#pragma unroll
-    for (int k = 0; k < kIds; ++k) {
-      local[k] = wanted(id[k]) && (static_cast<int>(id[k]) & mask) == b ? static_cast<int>(id[k]) >> t.log2_b : -1;
+    each(id, round, [&](int k, int v, bool wanted) {
+      local[k] = wanted && (v & mask) == b ? v >> t.log2_b : -1;
       const uint64_t ballot = __ballot(local[k] >= 0);
       in_wave[k] = mine + __popcll(ballot & ((uint64_t(1) << l) - 1));
       mine += __popcll(ballot);
-    }
+    });
     if (l == 0) room[wave] = mine;
     __syncthreads();
     // the waves before this one, and those of each part: a part always fits an empty queue
@@ -282,17 +283,17 @@ __global__ __launch_bounds__(kGroupThreads) void embed_group_kernel(const Id* __
 #pragma unroll
       for (int k = 0; k < kIds; ++k) {
         if (local[k] >= 0) {
-          queue_pos[at + in_wave[k]] = static_cast<int>(round) + (wave * kIds + k) * kWave + l;
+          queue_pos[at + in_wave[k]] = round + (wave * kIds + k) * kWave + l;
           queue_local[at + in_wave[k]] = static_cast<uint16_t>(local[k]);
         }
       }
     };
+    if (queued && queued + found > kQueue) drain();
     if (queued + found <= kQueue) {
       put_in(queued + ahead);
       queued += found;
       __syncthreads();
     } else {
-      if (queued) drain();
 #pragma unroll
       for (int p = 0; p < kParts; ++p) {
         if (wave / kPartWaves == p) put_in(ahead);
