@@ -18,7 +18,7 @@
 //      the launch fill the rows of ids that do not occur with zeros, which is most of the bytes.
 //   3. Ids with entries in several waves: their partial sums, in order.
 //
-// Measured: 8192 tokens of 151,936 ids x 1024 in fp32: lookup 9 us, the three launches 10, 125 (656 MB at 5.2 TB/s; stores of zeros
+// Measured: 8192 tokens of 151,936 ids x 1024 in fp32: lookup 9 us, the three launches 10, 122 (656 MB at 5.4 TB/s; stores of zeros
 // alone reach 6.7) and 5. 50,001 of 4096 x 777 in bf16: 21; 37, 23 and 14.
 
 #include <hip/hip_runtime.h>
@@ -346,12 +346,14 @@ template <bool kW32, bool kY32, bool kAdd>
 __global__ __launch_bounds__(256) void embed_sum_kernel(Sums a) {
   constexpr int kU = kW32 || kY32 ? 4 : 8, kAhead = 8;
   const int l = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (blockIdx.x >= a.sum_blocks) {  // rows that do not occur
+  // Rows that do not occur: one to a wave, through the caches (8192 tokens of 151,936 x 1024 in bf16 61 us; past them and four rows to a wave
+  // 83. A row of 1024 in fp32 to a workgroup, a store a thread, 8% slower.)
+  if (blockIdx.x >= a.sum_blocks) {
     const int64_t blocks = gridDim.x - a.sum_blocks;
     const float none[kU] = {};
     for (int64_t v = (blockIdx.x - a.sum_blocks) * 4 + wave; v < a.vocab; v += blocks * 4) {
       if (a.t.segments[segment_at(a.t, static_cast<int32_t>(v))].count) continue;
-      for (int c = kU * l; c < a.cols; c += kU * kWave) put<kW32, kU, true>(a.dw, v * a.ldw + c, none, a.cols - c);
+      for (int c = kU * l; c < a.cols; c += kU * kWave) put<kW32, kU>(a.dw, v * a.ldw + c, none, a.cols - c);
     }
     return;
   }
@@ -538,7 +540,7 @@ int tm_embed_grad(void* d_dw, int w_f32, int64_t ldw, const void* d_dy, int y_f3
   const bool wide = w_f32 || y_f32;
   const int64_t units = (cols + (wide ? 4 : 8) - 1) / (wide ? 4 : 8), panels = (units + kWave - 1) / kWave;
   const int64_t chunks = chunks_of(tokens), sum_blocks = (chunks * panels + 3) / 4;
-  const int64_t fill_blocks = add ? 0 : std::min<int64_t>((vocab + 15) / 16, 1 << 16);
+  const int64_t fill_blocks = add ? 0 : std::min<int64_t>((vocab + 3) / 4, 1 << 20);
   const int64_t join_panels = (cols + 4 * kWave - 1) / (4 * kWave);
   if (sum_blocks + fill_blocks >= int64_t(1) << 24 || (chunks - 1) * join_panels >= int64_t(1) << 24)  // of 256: less than 2^32 a launch
     return fail(TM_EINVAL, "%s: %lld tokens x %lld columns are too large for a launch", who, (long long)tokens, (long long)cols);
