@@ -108,6 +108,7 @@ def embedding_grad_(
     if grad.requires_grad:
         raise RuntimeError(f"{who}: grad requires a gradient itself and cannot be changed in place")
     padding = _padding(who, padding_idx, rows)
+    _refuse_tangents(who, grad, dy)
     if ids.numel() == 0:
         return grad
     if not _apart(grad, dy):
