@@ -507,11 +507,18 @@ class AdamW(torch.optim.Optimizer):
         param's device, as fp32, by the first step."""
         self._verified.clear()
         self._plan = None
-        super().load_state_dict(state_dict)
+        saved = {}
+        look = self.register_load_state_dict_pre_hook(lambda _, given: saved.update(given))  # behind the program's own
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            look.remove()
         for group in self.param_groups:
             group["fused"] = True
             group["foreach"] = None
-        self._repack_states()
+        keys = [k for group in saved["param_groups"] for k in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        self._repack_states({id(p) for k, p in zip(keys, params) if _of_bytes(saved["state"].get(k))})
 
     def _as_held(self, p: torch.Tensor, m: torch.Tensor, v: torch.Tensor):
         """``p``'s moments as this optimizer holds them, from either width."""
@@ -532,11 +539,11 @@ class AdamW(torch.optim.Optimizer):
         _convert_moments("tm_moments8_write", list(zip(out, wide)), p)
         return tuple(out)
 
-    def _repack_states(self) -> None:
+    def _repack_states(self, of_bytes: set) -> None:
         """Moments loaded from a checkpoint (separate tensors, or views of a loaded storage)
         are copied into this optimizer's pooled layout, as if created by its first step; those of the other width
         are converted. (torch's loader casts byte moments to the param's fp32: whole numbers up to 255,
-        cast back here.)"""
+        cast back here for the params whose ids are in ``of_bytes``: their moments were saved as bytes.)"""
         held = []
         for group in self.param_groups:
             for p in group["params"]:
@@ -547,7 +554,7 @@ class AdamW(torch.optim.Optimizer):
                 if not (isinstance(m, torch.Tensor) and isinstance(v, torch.Tensor)):
                     continue
                 size = held_bytes(p.numel())
-                if p.numel() and m.numel() == size and v.numel() == size:
+                if id(p) in of_bytes and m.numel() == size and v.numel() == size:
                     m, v = (t.to(dtype=torch.uint8, device=p.device) for t in (m, v))
                 elif not (m.numel() == p.numel() and v.numel() == p.numel() and m.dtype == v.dtype == torch.float32
                           and m.device == v.device == p.device):
@@ -898,6 +905,12 @@ def pooled_held_moments(params, zero: bool = True):
         for p, o, n in zip(ps, offs, sizes):
             out[id(p)] = tuple(pool[o: o + n] for pool in pools)
     return [(p, *out[id(p)]) for p in params]
+
+
+def _of_bytes(state) -> bool:
+    """Whether a saved state's moments are bytes."""
+    moments = [state.get(k) for k in ("exp_avg", "exp_avg_sq")] if isinstance(state, dict) else [None]
+    return all(isinstance(t, torch.Tensor) and t.dtype == torch.uint8 for t in moments)
 
 
 def _launch_moments(name: str, rows, device, upload) -> None:
