@@ -57,3 +57,22 @@ def test_bytes_that_a_hook_puts_in(bits):
         assert torch.equal(opt.flat_moments()[1].float().square(), wide["exp_avg_sq"])
     other.step()
     assert len(other._optimizer_load_state_dict_pre_hooks) == 1  # the program's
+
+
+def test_negative_zeros():
+    """A second moment of -0.0 is zero, and stays its own element's."""
+    n = 520
+    v = torch.linspace(0.1, 1.0, n, device=DEV).square_()
+    v[::3] = 0.0
+    p, opt = optimizer(n, 8)
+    state = {"step": torch.tensor(1.0), "exp_avg": torch.zeros(n, device=DEV)}
+    saved = opt.state_dict()
+    held = []
+    for zero in (0.0, -0.0):
+        values = torch.where(v == 0.0, torch.full_like(v, zero), v)
+        saved["state"] = {0: {**state, "exp_avg_sq": values}}
+        opt.load_state_dict(copy.deepcopy(saved))
+        held.append(opt.state[p]["exp_avg_sq"].clone())
+        _, root = opt.flat_moments()
+        assert not root[::3].any() and not torch.signbit(root).any()
+    assert torch.equal(*held)

@@ -113,6 +113,7 @@ __device__ __forceinline__ uint32_t hold_m(float m, uint32_t me, uint32_t bits) 
   const uint32_t c = (up >> 24 & 0x80u) | (up >> 20 & 0x7Fu);
   return kAny && !finite(m) ? 0x7Fu : c;
 }
+// A root has no sign, which would reach the next element's code.
 template <bool kAny>
 __device__ __forceinline__ uint32_t hold_root(float r, uint32_t re, uint32_t bits) {
   const uint32_t up = __float_as_uint(scale_root(r, re)) + ((bits >> 13 & ~7u) | 4u);
@@ -412,7 +413,7 @@ __device__ __forceinline__ void move_moments(const tm_tensor_t& d, int64_t start
       load_f32<kWhole>(m, d.master, e, left);
       load_f32<kWhole>(r, d.grad, e, left);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = sqrtf(r[j]);
+      for (int j = 0; j < 4; ++j) r[j] = fabsf(sqrtf(r[j]));  // (the root of -0 is -0)
       const uint32_t half[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
       store_codes(d, codes, e, hold4(m, r, half));
     }
