@@ -1,4 +1,4 @@
-"""The embedding's gradient by sums that are exact, so that every token counts once."""
+"""The embedding's gradient by sums that are exact, so that every token counts once, and on the stream that it is called on."""
 
 from __future__ import annotations
 
@@ -50,3 +50,41 @@ def test_every_token_counts_once(kind, vocab, n, w, out):
 @pytest.mark.parametrize("n,vocab", [(8192, 151_936), (50_001, 4096), (50_001, 300)])
 def test_padded_batches_of_odd_widths(n, vocab, cols, w, out):
     check("text", n, vocab, cols, w, out, padding=3, id_type=torch.int32 if cols == 520 else torch.int64)
+
+
+def beside():
+    """A stream whose work runs beside the current one's (streams share the few hardware queues)."""
+    for _ in range(8):
+        s, done = torch.cuda.Stream(), torch.cuda.Event()
+        torch.cuda._sleep(20_000_000)  # a bounded spin
+        done.record()
+        with torch.cuda.stream(s):
+            torch.ones(1, device=DEV)
+        s.synchronize()
+        free = not done.query()
+        torch.cuda.synchronize()
+        if free:
+            return s
+    pytest.skip("no stream runs beside the current one")
+
+
+def test_node_called_on_another_stream():
+    """A node that is called directly runs where it is called, not where its forward pass ran."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    ids = ids_of("text", 3000, 500, g)
+    weight = torch.randn(500, 256, generator=g, device=DEV).requires_grad_()
+    dy = torch.randn(3000, 256, generator=g, device=DEV)
+    want, = torch.autograd.grad(ta.embedding(ids, weight), weight, dy)
+    y = ta.embedding(ids, weight)
+    torch.cuda.synchronize()
+    s = beside()
+    with torch.cuda.stream(s):
+        spoilt = torch.full_like(want, float("nan"))
+    s.synchronize()
+    del spoilt  # (its block is the result's)
+    torch.cuda._sleep(100_000_000)  # the forward pass's stream is busy
+    with torch.no_grad(), torch.cuda.stream(s):
+        got = next(v for v in y.grad_fn(dy) if v is not None).clone()
+    s.synchronize()
+    assert torch.equal(got, want)
+    torch.cuda.synchronize()

@@ -1,4 +1,4 @@
-"""The norms' backward pass where the sums over rows can be checked exactly."""
+"""The norms' backward pass where the sums over rows can be checked exactly, and what it keeps, reads and runs on."""
 
 from __future__ import annotations
 
@@ -49,3 +49,47 @@ def test_every_row_counts_once(rows, cols, layer, x):
     assert torch.equal(got["weight"].double(), (dy.double() * t["x"].double()).sum(0))
     if layer:
         assert torch.equal(got["bias"].double(), dy.double().sum(0))
+
+
+# ---------------------------------------------------------------------------- streams
+
+
+def beside():
+    """A stream whose work runs beside the current one's (streams share the few hardware queues)."""
+    for _ in range(8):
+        s, done = torch.cuda.Stream(), torch.cuda.Event()
+        torch.cuda._sleep(20_000_000)  # a bounded spin
+        done.record()
+        with torch.cuda.stream(s):
+            torch.ones(1, device=DEV)
+        s.synchronize()
+        free = not done.query()
+        torch.cuda.synchronize()
+        if free:
+            return s
+    pytest.skip("no stream runs beside the current one")
+
+
+@pytest.mark.parametrize("layer", [True, False])
+def test_node_called_on_another_stream(layer):
+    """A node that is called directly runs where it is called, not where its forward pass ran."""
+    g = torch.Generator(device=DEV).manual_seed(2)
+    t = {"x": torch.randn(400, 1000, generator=g, device=DEV).requires_grad_(), "weight": torch.randn(1000, generator=g, device=DEV).requires_grad_(),
+         "bias": torch.randn(1000, generator=g, device=DEV).requires_grad_() if layer else None}
+    dy = torch.randn(400, 1000, generator=g, device=DEV)
+    keys = [k for k in t if t[k] is not None]
+    want = torch.autograd.grad(call(t, layer), [t[k] for k in keys], dy)
+    y = call(t, layer)
+    torch.cuda.synchronize()
+    s = beside()
+    with torch.cuda.stream(s):
+        spoilt = [torch.full_like(w, float("nan")) for w in want]
+    s.synchronize()
+    del spoilt  # (its blocks are the results')
+    torch.cuda._sleep(100_000_000)  # the forward pass's stream is busy
+    with torch.no_grad(), torch.cuda.stream(s):
+        got = [v.clone() for v in y.grad_fn(dy)[: len(keys)]]
+    s.synchronize()
+    for k, a, b in zip(keys, want, got):
+        assert torch.equal(a, b), k
+    torch.cuda.synchronize()

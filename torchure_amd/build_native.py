@@ -67,8 +67,9 @@ def host_command(output: str) -> list[str]:
         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_tm_host", "-DTORCH_API_INCLUDE_EXTENSION_H",
         f"-I{tdir}/include", f"-I{tdir}/include/torch/csrc/api/include",
         f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
+        "-D__HIP_PLATFORM_AMD__", f"-I{os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(hipcc()))), 'include')}",
         *HOST_SOURCES,
-        f"-L{tdir}/lib", "-lc10", "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{tdir}/lib",
+        f"-L{tdir}/lib", "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python", f"-Wl,-rpath,{tdir}/lib",
         "-o", output,
     ]
 

@@ -4,6 +4,7 @@
 // from norm.py and embed.py.
 
 #include <torch/extension.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/Exceptions.h>
 
@@ -79,6 +80,10 @@ struct OnDevice {
   explicit OnDevice(const Tensor& t) : guard(t.device()) {}
 };
 
+// The stream that a backward pass runs on: the engine makes the forward pass's the current one, and a node that is called
+// directly runs where its caller is.
+void* current_stream(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
 // What a backward pass returned, in a pass that records itself (create_graph): a second derivative is refused, where a
 // result without a graph would drop it.
 variable_list once(variable_list grads) {
@@ -119,7 +124,6 @@ Tensor norm_forward(const Tensor& x, const Opt& weight, const Opt& bias, const N
   return y;
 }
 
-// The engine runs a node's backward pass on the stream that its forward pass ran on, so the handle is kept.
 struct NormFunction : torch::autograd::Function<NormFunction> {
   enum : i64 { kLayer = 1, kWeight = 2, kWeightF32 = 4, kBias = 8, kBiasF32 = 16 };
 
@@ -129,7 +133,6 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     ctx->save_for_backward(std::move(kept));
     ctx->saved_data["flags"] = (n.layer ? kLayer : 0) | (weight ? kWeight | (is_f32(*weight) ? kWeightF32 : 0) : 0) |
                                (bias ? kBias | (is_f32(*bias) ? kBiasF32 : 0) : 0);
-    ctx->saved_data["stream"] = reinterpret_cast<i64>(n.stream);
     return y;
   }
 
@@ -156,7 +159,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
       const float* rstd = s.data_ptr<float>();
       check(abi().norm_backward(ptr(dx), ptr(dw), ptr(db), f32_if(db), ptr(d.t), is_f32(d.t), d.ld, ptr(r.t), is_f32(r.t), r.ld,
                                 rstd, layer ? rstd + r.n : nullptr, ptr(w), f32_if(w), f32_if(dw), layer, r.n, r.d, ptr(ws),
-                                need, reinterpret_cast<void*>(ctx->saved_data["stream"].toInt())),
+                                need, current_stream(dy)),
             "tm_norm_backward");
     }
     return once({dx, dw, db, Tensor()});
@@ -229,7 +232,6 @@ struct EmbedFunction : torch::autograd::Function<EmbedFunction> {
     ctx->saved_data["f32"] = is_f32(weight);
     ctx->saved_data["scale"] = e.scale;
     ctx->saved_data["padding"] = e.padding;
-    ctx->saved_data["stream"] = reinterpret_cast<i64>(e.stream);
     return lookup(kept, weight, e);
   }
 
@@ -241,7 +243,7 @@ struct EmbedFunction : torch::autograd::Function<EmbedFunction> {
       const at::AutoGradMode no_grad(false);
       dw = room(dy, {ctx->saved_data["vocab"].toInt(), dy.size(-1)}, type_of(ctx->saved_data["f32"].toBool()));
       table_grad(dw, dw.size(1), dy, ids, ctx->saved_data["scale"].toDouble(), ctx->saved_data["padding"].toInt(), false,
-                 reinterpret_cast<void*>(ctx->saved_data["stream"].toInt()));
+                 current_stream(dy));
     }
     return once({Tensor(), dw, Tensor()});
   }
