@@ -542,7 +542,8 @@ int tm_moments8_write(const tm_tensor_t* d_tensors, int64_t n_tensors, const tm_
  *   tm_norm_forward    d_rstd and d_mean (rows values each, mean for layer norm only): written where given, for the backward pass.
  *   tm_norm_backward   d_dx (x's type, rows cols apart), d_dw (dw_f32) and d_db (b_f32, layer norm only), each or NULL, from dy
  *                      (y's type, rows lddy apart). With d_dw or d_db, d_ws holds tm_norm_workspace_bytes bytes. Sums over
- *                      rows are made in a fixed order.
+ *                      rows are made in a fixed order. d_x, d_rstd and d_mean are read for dx and dw only, d_w for dx only, and may be
+ *                      NULL without (x_f32 still says x's type, which the workspace goes by).
  * Limits: cols <= 16384, rows <= 2^40.
  */
 int tm_norm_forward(void* d_y, int y_f32, float* d_rstd, float* d_mean, const void* d_x, int x_f32, int64_t ldx,

@@ -1,4 +1,4 @@
-"""The norms' backward pass where the sums over rows can be checked exactly, and what it keeps, reads and runs on."""
+"""The norms' backward pass where the sums over rows can be checked exactly, and what it keeps and runs on."""
 
 from __future__ import annotations
 
@@ -49,6 +49,40 @@ def test_every_row_counts_once(rows, cols, layer, x):
     assert torch.equal(got["weight"].double(), (dy.double() * t["x"].double()).sum(0))
     if layer:
         assert torch.equal(got["bias"].double(), dy.double().sum(0))
+
+
+# ---------------------------------------------------------------------------- what is kept
+
+
+@pytest.mark.parametrize("layer", [True, False])
+def test_kept_for_what_is_wanted(layer):
+    g = torch.Generator(device=DEV).manual_seed(1)
+    rows, cols = 37, 200
+    values = {"x": torch.randn(rows, cols, generator=g, device=DEV).to(BF16), "weight": torch.randn(cols, generator=g, device=DEV),
+              "bias": torch.randn(cols, generator=g, device=DEV) if layer else None}
+    dy = torch.randn(rows, cols, generator=g, device=DEV).to(BF16)
+    names = [k for k, v in values.items() if v is not None]
+    every = {k: v if v is None else v.clone().requires_grad_() for k, v in values.items()}
+    full = dict(zip(names, torch.autograd.grad(call(every, layer), [every[k] for k in names], dy)))
+    stats = (2 if layer else 1, rows)
+    for bits in range(1, 1 << len(names)):
+        keys = [k for i, k in enumerate(names) if bits >> i & 1]
+        t = {k: v if v is None else v.clone().requires_grad_(k in keys) for k, v in values.items()}
+        kept = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda v: kept.append(tuple(v.shape)) or v, lambda v: v):
+            y = call(t, layer)
+        want = []
+        if "x" in keys or "weight" in keys:
+            want += [(rows, cols), stats]
+        if "x" in keys:
+            want.append((cols,))
+        assert sorted(kept) == sorted(want), (keys, kept)
+        with torch.no_grad():  # what is not kept may change
+            for k, needed in (("x", "x" in keys or "weight" in keys), ("weight", "x" in keys), ("bias", False)):
+                if t[k] is not None and not needed:
+                    t[k].add_(1.0)
+        for k, got in zip(keys, torch.autograd.grad(y, [t[k] for k in keys], dy)):
+            assert got.dtype == values[k].dtype and torch.equal(got, full[k]), (keys, k)
 
 
 # ---------------------------------------------------------------------------- streams

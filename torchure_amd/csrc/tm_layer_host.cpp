@@ -125,13 +125,16 @@ Tensor norm_forward(const Tensor& x, const Opt& weight, const Opt& bias, const N
 }
 
 struct NormFunction : torch::autograd::Function<NormFunction> {
-  enum : i64 { kLayer = 1, kWeight = 2, kWeightF32 = 4, kBias = 8, kBiasF32 = 16 };
+  enum : i64 { kLayer = 1, kWeight = 2, kWeightF32 = 4, kBias = 8, kBiasF32 = 16, kXF32 = 32 };
 
+  // Kept are, for x's gradient, x, the statistics and the weight; for the weight's, x and the statistics; for the bias's nothing.
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Opt& weight, const Opt& bias, const Norm& n) {
-    variable_list kept;
-    const Tensor y = norm_forward(x, weight, bias, n, &kept);
+    const bool for_x = wants_grad(x), for_weight = weight && wants_grad(*weight);
+    variable_list kept(3);
+    const Tensor y = norm_forward(x, weight, bias, n, for_x || for_weight ? &kept : nullptr);
+    if (!for_x) kept[2] = Tensor();
     ctx->save_for_backward(std::move(kept));
-    ctx->saved_data["flags"] = (n.layer ? kLayer : 0) | (weight ? kWeight | (is_f32(*weight) ? kWeightF32 : 0) : 0) |
+    ctx->saved_data["flags"] = (n.layer ? kLayer : 0) | (is_f32(x) ? kXF32 : 0) | (weight ? kWeight | (is_f32(*weight) ? kWeightF32 : 0) : 0) |
                                (bias ? kBias | (is_f32(*bias) ? kBiasF32 : 0) : 0);
     return y;
   }
@@ -141,25 +144,25 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     const Tensor& dy = grads[0];
     const variable_list kept = ctx->get_saved_variables();
     const i64 flags = ctx->saved_data["flags"].toInt();
-    const bool layer = flags & kLayer, has_w = flags & kWeight, has_b = flags & kBias;
+    const bool layer = flags & kLayer, has_w = flags & kWeight, has_b = flags & kBias, x_f32 = flags & kXF32;
     const bool need_x = ctx->needs_input_grad(0), need_w = has_w && ctx->needs_input_grad(1),
                need_b = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
     Tensor dx, dw, db;
     {
       const at::AutoGradMode no_grad(false);
       const OnDevice on(dy);
-      const Rows r = rows_of(kept[0]), d = rows_of(dy);
-      const Tensor s = kept[1].contiguous(), w = kept[2].defined() ? kept[2].contiguous() : Tensor();
-      if (need_x) dx = room(dy, dy.sizes(), r.t.scalar_type());
-      if (need_w) dw = room(dy, {r.d}, type_of(flags & kWeightF32));
-      if (need_b) db = room(dy, {r.d}, type_of(flags & kBiasF32));
-      const size_t need = need_w || need_b ? abi().norm_bytes(r.n, r.d, is_f32(r.t), is_f32(d.t), layer) : 0;
+      const Rows d = rows_of(dy), r = kept[0].defined() ? rows_of(kept[0]) : Rows{Tensor(), d.n, d.d, d.d};
+      const Tensor s = kept[1].defined() ? kept[1].contiguous() : Tensor(), w = kept[2].defined() ? kept[2].contiguous() : Tensor();
+      if (need_x) dx = room(dy, dy.sizes(), type_of(x_f32));
+      if (need_w) dw = room(dy, {d.d}, type_of(flags & kWeightF32));
+      if (need_b) db = room(dy, {d.d}, type_of(flags & kBiasF32));
+      const size_t need = need_w || need_b ? abi().norm_bytes(d.n, d.d, x_f32, is_f32(d.t), layer) : 0;
       Tensor ws;
       if (need) ws = room(dy, {static_cast<i64>(need)}, at::kByte);
-      const float* rstd = s.data_ptr<float>();
-      check(abi().norm_backward(ptr(dx), ptr(dw), ptr(db), f32_if(db), ptr(d.t), is_f32(d.t), d.ld, ptr(r.t), is_f32(r.t), r.ld,
-                                rstd, layer ? rstd + r.n : nullptr, ptr(w), f32_if(w), f32_if(dw), layer, r.n, r.d, ptr(ws),
-                                need, current_stream(dy)),
+      const float* rstd = s.defined() ? s.data_ptr<float>() : nullptr;
+      check(abi().norm_backward(ptr(dx), ptr(dw), ptr(db), f32_if(db), ptr(d.t), is_f32(d.t), d.ld, ptr(r.t), x_f32, r.ld, rstd,
+                                layer && rstd ? rstd + d.n : nullptr, ptr(w), f32_if(w), f32_if(dw), layer, d.n, d.d, ptr(ws), need,
+                                current_stream(dy)),
             "tm_norm_backward");
     }
     return once({dx, dw, db, Tensor()});

@@ -251,7 +251,7 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
   Row<S, kY32> next_dy;
   auto load = [&](int64_t r) {
     const int cols = r < a.rows ? a.cols : 0;
-    next_x.load(a.x, r * a.ldx, l, cols);
+    next_x.load(a.x, r * a.ldx, l, a.x ? cols : 0);
     next_dy.load(a.dy, r * a.lddy, l, cols);
   };
   if constexpr (kAhead) load(r0 + mine);
@@ -266,7 +266,8 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
   for (; r0 < a.rows; r0 += step) {
     const int64_t r = r0 + mine;
     const int cols = r < a.rows ? a.cols : 0;
-    const float rstd = cols ? a.rstd[r] : 0.0f, mean = kLayer && cols ? a.mean[r] : 0.0f;
+    const bool there = cols && a.x;  // (x is left out where db alone is wanted)
+    const float rstd = there ? a.rstd[r] : 0.0f, mean = kLayer && there ? a.mean[r] : 0.0f;
     if constexpr (!kAhead) load(r);
     const Row<S, kX32> row_x = next_x;
     const Row<S, kY32> row_dy = next_dy;
@@ -511,9 +512,11 @@ int tm_norm_backward(void* d_dx, void* d_dw, void* d_db, int b_f32, const void* 
   const char* who = "tm_norm_backward";
   if (int rc = check_sizes(who, rows, cols)) return rc;
   if (rows == 0) return fail(TM_EINVAL, "%s: no rows", who);
-  if (!d_dy || !d_x || !d_rstd || (layer && !d_mean)) return fail(TM_EINVAL, "%s: null input", who);
+  if (!d_dy) return fail(TM_EINVAL, "%s: null input", who);
+  if ((d_dx || d_dw) && (!d_x || !d_rstd || (layer && !d_mean))) return fail(TM_EINVAL, "%s: null input", who);
   if (!layer && d_db) return fail(TM_EINVAL, "%s: an RMS norm has no bias", who);
-  if ((ldx < cols || lddy < cols) && rows > 1)
+  if (!d_dx && !d_dw) d_x = nullptr;
+  if (((d_x && ldx < cols) || lddy < cols) && rows > 1)
     return fail(TM_EINVAL, "%s: rows %lld and %lld elements apart", who, (long long)ldx, (long long)lddy);
   if (odd(d_dx, x_f32) || odd(d_dw, dw_f32) || odd(d_db, b_f32) || odd(d_dy, y_f32) || odd(d_x, x_f32) || odd(d_w, w_f32) ||
       odd(d_rstd, true) || odd(d_mean, true))

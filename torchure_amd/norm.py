@@ -72,8 +72,8 @@ def rms_norm(
     dtype: torch.dtype | None = None,
 ) -> torch.Tensor:
     """``x / sqrt(mean(x^2) + eps) * weight`` over the last dimension, in ``dtype`` (bf16 or fp32; x's by default). All
-    gradients, in their tensors' types; what no gradient needs is neither kept nor computed. Kept for the backward
-    pass are x and one fp32 value a row. Differentiable once, in reverse mode."""
+    gradients, in their tensors' types. Kept for the backward pass are x and one fp32 value a row, for x's and the
+    weight's gradient, and for x's the weight; what no gradient needs is not kept. Differentiable once, in reverse mode."""
     return _norm("rms_norm", x, weight, None, False, eps, dtype)
 
 
@@ -86,5 +86,5 @@ def layer_norm(
 ) -> torch.Tensor:
     """``(x - mean(x)) / sqrt(var(x) + eps) * weight + bias`` over the last dimension (var: the mean squared distance from the
     mean), in ``dtype`` (bf16 or fp32; x's by default). Gradients and what is kept as for ``rms_norm``, with two fp32
-    values a row."""
+    values a row; for the bias's gradient nothing is."""
     return _norm("layer_norm", x, weight, bias, True, eps, dtype)
