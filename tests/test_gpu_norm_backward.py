@@ -1,4 +1,4 @@
-"""The norms' backward pass where the sums over rows can be checked exactly, and what it keeps and runs on."""
+"""The norms' backward pass where the sums over rows can be checked exactly, and what it keeps, reads and runs on."""
 
 from __future__ import annotations
 
@@ -11,6 +11,7 @@ import torchure_amd as ta
 pytestmark = pytest.mark.gpu
 
 DEV, BF16, F32 = "cuda", torch.bfloat16, torch.float32
+U = 2.0 ** -24
 
 
 def call(t, layer, eps=1e-5):
@@ -49,6 +50,37 @@ def test_every_row_counts_once(rows, cols, layer, x):
     assert torch.equal(got["weight"].double(), (dy.double() * t["x"].double()).sum(0))
     if layer:
         assert torch.equal(got["bias"].double(), dy.double().sum(0))
+
+
+# ---------------------------------------------------------------------------- rows far from zero
+
+
+@pytest.mark.parametrize("out", [BF16, F32])
+@pytest.mark.parametrize("cols", [1, 2, 4, 8, 16, 32])
+def test_constant_rows_far_from_zero(cols, out):
+    """A row of one large number has xhat of 0, and dx = (g - mean(g)) / sqrt(eps), also where mean times rstd is past
+    fp32: what lies past a row's end has no part in it. (Of 2^k equal numbers the mean is exact in fp32.)"""
+    eps = 1e-5
+    g = torch.Generator(device=DEV).manual_seed(cols)
+    x = torch.randn(7, cols, generator=g, device=DEV)
+    x[2], x[5] = 2.0 ** 121, -(2.0 ** 121)
+    t = {"x": x.to(out).requires_grad_(), "weight": torch.ones(cols, device=DEV, requires_grad=True),
+         "bias": torch.zeros(cols, device=DEV, requires_grad=True)}
+    dy = torch.randn(7, cols, generator=g, device=DEV).to(out)
+    y = call(t, True, eps)
+    assert not y[2].any() and not y[5].any()
+    dx, dw, db = torch.autograd.grad(y, [t["x"], t["weight"], t["bias"]], dy)
+    d = dy.double()
+    for r in (2, 5):
+        want = (d[r] - d[r].mean()) / eps ** 0.5
+        # a sum at most 80 additions deep, its scaling, the difference; eps, its root and reciprocal; the product; the result
+        bound = (84 * U * d[r].abs().mean() + U * (d[r] - d[r].mean()).abs()) / eps ** 0.5 + 5 * U * want.abs()
+        bound = bound + {BF16: 2.0 ** -8, F32: U}[out] * (want.abs() + bound)
+        assert bool(((dx[r].double() - want).abs() <= bound).all()), r
+    keep = torch.tensor([0, 1, 3, 4, 6], device=DEV)
+    rest = {"x": t["x"].detach()[keep].requires_grad_(), "weight": t["weight"], "bias": t["bias"]}
+    same, part, _ = torch.autograd.grad(call(rest, True, eps), [rest["x"], t["weight"], t["bias"]], dy[keep])
+    assert torch.equal(dx[keep], same) and bool(torch.isfinite(dw).all())
 
 
 # ---------------------------------------------------------------------------- what is kept

@@ -40,6 +40,7 @@ int fail(int code, const char* fmt, A... args) {
 
 constexpr int kWave = 64;
 constexpr int kCus = 256;
+constexpr float kMost = 0x1.fffffep127f;
 // Results go past the caches: 8192 x 2560 forward 16.7 us for 20.9, fp32 8192 x 1024 backward 14.7 for 18.1; a product of 9728 columns
 // behind the first takes the same time with it either way (338-341 us).
 constexpr bool kStream = true;
@@ -268,6 +269,9 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
     const int cols = r < a.rows ? a.cols : 0;
     const bool there = cols && a.x;  // (x is left out where db alone is wanted)
     const float rstd = there ? a.rstd[r] : 0.0f, mean = kLayer && there ? a.mean[r] : 0.0f;
+    // Where mean rstd passes fp32 (both finite), all of the row is its mean: a distance of even 2^-48 of it would make rstd less. Its
+    // xhat is 0, but past its end, where x is read as 0, it would be -inf, and times a g of 0 NaN.
+    const float hat = kLayer && fabsf(mean * rstd) > kMost && fabsf(mean) <= kMost && rstd <= kMost ? 0.0f : rstd;
     if constexpr (!kAhead) load(r);
     const Row<S, kX32> row_x = next_x;
     const Row<S, kY32> row_dy = next_dy;
@@ -284,7 +288,7 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
       values(dy, row_dy.u[k]);
 #pragma unroll
       for (int i = 0; i < S::kU; ++i) {
-        const float xhat = (x[i] - mean) * rstd, g = dy[i] * w[i];
+        const float xhat = (x[i] - mean) * hat, g = dy[i] * w[i];
         if constexpr (kParams) {
           dw[k][i] = fmaf(dy[i], xhat, dw[k][i]);
           if constexpr (kLayer) db[k][i] += dy[i];
@@ -304,7 +308,7 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
         values(x, row_x.u[k]);
         values(dy, row_dy.u[k]);
 #pragma unroll
-        for (int i = 0; i < S::kU; ++i) dx[i] = (fmaf(dy[i], w[i], -mid) - (x[i] - mean) * rstd * along) * rstd;
+        for (int i = 0; i < S::kU; ++i) dx[i] = (fmaf(dy[i], w[i], -mid) - (x[i] - mean) * hat * along) * rstd;
         put<kX32, S::kU, kStream>(a.dx, r * a.cols + c, dx, cols - c);
       }
     }
