@@ -270,8 +270,8 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
     const bool there = cols && a.x;  // (x is left out where db alone is wanted)
     const float rstd = there ? a.rstd[r] : 0.0f, mean = kLayer && there ? a.mean[r] : 0.0f;
     // Where mean rstd passes fp32 (both finite), all of the row is its mean: a distance of even 2^-48 of it would make rstd less. Its
-    // xhat is 0, but past its end, where x is read as 0, it would be -inf, and times a g of 0 NaN.
-    const float hat = kLayer && fabsf(mean * rstd) > kMost && fabsf(mean) <= kMost && rstd <= kMost ? 0.0f : rstd;
+    // xhat is 0, but past its end, where x is read as 0, it is -inf, and times a g of 0 NaN.
+    const bool far = kLayer && fabsf(mean * rstd) > kMost && fabsf(mean) <= kMost && rstd <= kMost;
     if constexpr (!kAhead) load(r);
     const Row<S, kX32> row_x = next_x;
     const Row<S, kY32> row_dy = next_dy;
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
       values(dy, row_dy.u[k]);
 #pragma unroll
       for (int i = 0; i < S::kU; ++i) {
-        const float xhat = (x[i] - mean) * hat, g = dy[i] * w[i];
+        const float xhat = (x[i] - mean) * rstd, g = dy[i] * w[i];
         if constexpr (kParams) {
           dw[k][i] = fmaf(dy[i], xhat, dw[k][i]);
           if constexpr (kLayer) db[k][i] += dy[i];
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
       }
     }
     row_sum(v);
-    const float along = v[0] * a.inv_cols, mid = kLayer ? v[kLayer ? 1 : 0] * a.inv_cols : 0.0f;
+    const float along = far ? 0.0f : v[0] * a.inv_cols, mid = kLayer ? v[kLayer ? 1 : 0] * a.inv_cols : 0.0f;
     if (a.dx) {
 #pragma unroll
       for (int k = 0; k < S::kVec; ++k) {
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(S::kBackwardThreads) void norm_backward_kernel(Back
         values(x, row_x.u[k]);
         values(dy, row_dy.u[k]);
 #pragma unroll
-        for (int i = 0; i < S::kU; ++i) dx[i] = (fmaf(dy[i], w[i], -mid) - (x[i] - mean) * hat * along) * rstd;
+        for (int i = 0; i < S::kU; ++i) dx[i] = (fmaf(dy[i], w[i], -mid) - (x[i] - mean) * rstd * along) * rstd;
         put<kX32, S::kU, kStream>(a.dx, r * a.cols + c, dx, cols - c);
       }
     }
