@@ -107,6 +107,8 @@ def embedding_grad_(
         raise RuntimeError(f"{who}: grad of strides {grad.stride()}, its rows must lie apart, each in one piece")
     if grad.requires_grad:
         raise RuntimeError(f"{who}: grad requires a gradient itself and cannot be changed in place")
+    if grad.is_inference() and not torch.is_inference_mode_enabled():
+        raise RuntimeError(f"{who}: grad is an inference tensor and cannot be changed in place outside inference mode")
     padding = _padding(who, padding_idx, rows)
     _refuse_tangents(who, grad, dy)
     if ids.numel() == 0:
