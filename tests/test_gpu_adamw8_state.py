@@ -76,3 +76,61 @@ def test_negative_zeros():
         _, root = opt.flat_moments()
         assert not root[::3].any() and not torch.signbit(root).any()
     assert torch.equal(*held)
+
+
+# ---------------------------------------------------------------------------- every root as 64 bits hold it
+
+
+MASK = (1 << 32) - 1
+
+
+def mix(z):
+    z = ((z ^ (z >> 16)) * 0x8C2549D1) & MASK
+    z = ((z ^ (z >> 15)) * 0xD406A25D) & MASK
+    return z ^ (z >> 16)
+
+
+def high_halves(n, seed, step):
+    z = (torch.arange(n, device=DEV) * 0x9E3779B1 + mix((step + mix(mix(seed))) & MASK)) & MASK
+    z = ((z ^ (z >> 16)) * 0x8C2549D1) & MASK
+    return (z ^ (z >> 15)) >> 16
+
+
+def two_to(e):
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def roots(held, n):
+    """The values of n roots' bytes (n a multiple of 256), in 64 bits."""
+    c, e = held[:n].long(), held[n:].long() - 145
+    values = torch.where(c < 16, c, (16 + c % 16) << (c // 16 - 1).clamp(min=0)).double()
+    return (values.view(-1, 64) * two_to(e)[:, None]).view(-1)
+
+
+@pytest.mark.parametrize("std", [1e-3, 1.0])
+def test_roots_turn_where_64_bits_say(std):
+    """Of 2^24 roots each is the neighbour that its value in 64 bits and its random bits ask for: where it turns is a number that fp32
+    holds, and a root rounded onto it from below stays below. (Blocks whose largest root is within fp32 of where their power of two
+    changes, and roots on the format's constant steps, may go either way.)"""
+    n, seed, betas = 1 << 24, 3, (0.9, 0.95)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    p = torch.nn.Parameter(torch.zeros(n, device=DEV))
+    opt = ta.AdamW([p], lr=1e-3, betas=betas, weight_decay=0.0, state_bits=8, seed=seed)
+    for step in (1, 2, 3):
+        before = roots(opt.state[p]["exp_avg_sq"], n) if step > 1 else torch.zeros(n, dtype=torch.float64, device=DEV)
+        p.grad = torch.randn(n, generator=g, device=DEV) * std
+        opt.step()
+        v = betas[1] * before.square() + (1.0 - betas[1]) * p.grad.double().square()
+        r = v.sqrt().view(-1, 64)
+        most = r.amax(1)
+        e = torch.frexp(most / (30.0 * 2.0 ** 14))  # most <= 30 2^14 2^x
+        power = two_to(e.exponent - (e.mantissa == 0.5).int())[:, None]
+        off = (most / (30.0 * 2.0 ** 14 * power.view(-1)) - torch.tensor([[0.5], [1.0]], device=DEV, dtype=torch.float64)).abs().amin(0)
+        y = r / power
+        place = two_to(torch.frexp(y).exponent - 5)
+        u = (high_halves(n, seed, step).double().view(-1, 64) + 0.5) / 65536.0
+        want = torch.floor(y / place + u) * place * power
+        sure = (y >= 16.0) & (off > 2.0 ** -22)[:, None]
+        got = roots(opt.state[p]["exp_avg_sq"], n).view(-1, 64)
+        assert float(sure.double().mean()) > 0.99
+        assert int((got != want)[sure].sum()) == 0, step

@@ -12,9 +12,9 @@
 // 5e-4 of itself). Rounded up with the probability of the part that lies above, what is held has the right mean.
 // The random bits are a hash of (seed, step, element): the same run gives the same bits, on any launch shape.
 //
-// The new moments are summed in fp64 as in the 32-bit step and rounded to fp32 once (fp64 costs the step nothing, 5.95 TB/s
-// either way; sums in fp32 turned three times as many of the roundings the other way); the rest is fp32. The step uses the moments
-// before they are held again.
+// The new moments are summed in fp64 as in the 32-bit step and rounded to fp32 once (sums in fp32 turned three times as many of the
+// roundings the other way); the rest is fp32. Which way a root is rounded goes by its sum in fp64 too: 1-1.6% of the step's time. The
+// step uses the moments before they are held again.
 //
 // Bound by memory: 16.06 bytes a param with bf16 grads and copies (28 with 32-bit moments). The codes were computed with per-value
 // tests, selects and e4m3 conversions first, 300 vector instructions a wave, which bound the step at 5.5 TB/s; as float's own denormals
@@ -113,10 +113,12 @@ __device__ __forceinline__ uint32_t hold_m(float m, uint32_t me, uint32_t bits) 
   const uint32_t c = (up >> 24 & 0x80u) | (up >> 20 & 0x7Fu);
   return kAny && !finite(m) ? 0x7Fu : c;
 }
-// A root has no sign, which would reach the next element's code.
+// A root has no sign, which would reach the next element's code. `past`: -1 where r is past the root that it was rounded
+// from, else 0: the places at which a root turns are fp32 numbers, and half of those just below one are rounded onto it (510 to 560 of
+// 574e6 were held otherwise than in 64 bits, none so).
 template <bool kAny>
-__device__ __forceinline__ uint32_t hold_root(float r, uint32_t re, uint32_t bits) {
-  const uint32_t up = __float_as_uint(scale_root(r, re)) + ((bits >> 13 & ~7u) | 4u);
+__device__ __forceinline__ uint32_t hold_root(float r, int past, uint32_t re, uint32_t bits) {
+  const uint32_t up = __float_as_uint(scale_root(r, re)) + ((bits >> 13 & ~7u) | 4u) + past;
   const uint32_t c = max(up >> 19, min(__float_as_uint(r), 1u));
   return kAny && !finite(r) ? 255u : c;
 }
@@ -131,12 +133,12 @@ struct Codes {
 };
 
 template <bool kAny>
-__device__ __forceinline__ void codes4(Codes& c, const float* m, const float* r, const uint32_t* bits) {
+__device__ __forceinline__ void codes4(Codes& c, const float* m, const float* r, const int* past, const uint32_t* bits) {
   c.m = c.r = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     c.m |= hold_m<kAny>(m[j], c.me, bits[j]) << (8 * j);
-    c.r |= hold_root<kAny>(r[j], c.re, bits[j]) << (8 * j);
+    c.r |= hold_root<kAny>(r[j], past[j], c.re, bits[j]) << (8 * j);
   }
 }
 
@@ -145,7 +147,7 @@ __device__ __forceinline__ uint32_t most4(const float* x) {
              max(__float_as_uint(x[2]) & 0x7FFFFFFFu, __float_as_uint(x[3]) & 0x7FFFFFFFu));
 }
 
-__device__ __forceinline__ Codes hold4(const float* m, const float* r, const uint32_t* bits) {
+__device__ __forceinline__ Codes hold4(const float* m, const float* r, const int* past, const uint32_t* bits) {
   Codes c;
   uint32_t most_m = most4(m), most_r = most4(r);
   // a wave with an m past all blocks' range, an infinity or a NaN looks at each value
@@ -158,8 +160,8 @@ __device__ __forceinline__ Codes hold4(const float* m, const float* r, const uin
   most_r = tm_act::row_max(most_r);
   c.me = static_cast<uint32_t>(tm_act::block_exponent(most_m) + 127);
   c.re = max((most_r + 0x000FFFFFu) >> 23, static_cast<uint32_t>(kRootLow));
-  if (any) codes4<true>(c, m, r, bits);
-  else codes4<false>(c, m, r, bits);
+  if (any) codes4<true>(c, m, r, past, bits);
+  else codes4<false>(c, m, r, past, bits);
   return c;
 }
 
@@ -338,6 +340,7 @@ __device__ __forceinline__ void update(const tm_tensor_t& d, const Scal& s, floa
     float m[4], r[4];
     read4(was[k], m, r);
     uint32_t bits[4];
+    int past[4];
     const uint32_t z = static_cast<uint32_t>(e) * kHashA + s.key;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -345,11 +348,14 @@ __device__ __forceinline__ void update(const tm_tensor_t& d, const Scal& s, floa
       const float pj = (s.flags & kDecay) ? fmaf(s.neg_lrwd, p[k][j], p[k][j]) : p[k][j];
       const double gd = gj;
       m[j] = static_cast<float>(fma(s.beta1, static_cast<double>(m[j]), s.omb1 * gd));
-      r[j] = sqrtf(static_cast<float>(fma(s.beta2, static_cast<double>(r[j] * r[j]), s.omb2 * gd * gd)));
+      const double v = fma(s.beta2, static_cast<double>(r[j] * r[j]), s.omb2 * gd * gd);
+      r[j] = sqrtf(static_cast<float>(v));
+      const double rd = r[j];
+      past[j] = __double2hiint(fma(-rd, rd, v)) >> 31;
       p[k][j] = pj - s.step_size * m[j] / fmaf(r[j], s.inv_bc2s, s.eps);
       bits[j] = element_bits(z + j * kHashA);
     }
-    const Codes now = hold4(m, r, bits);
+    const Codes now = hold4(m, r, past, bits);
     const int left = kWhole ? 4 : left_of(d.numel, e);
     store_f32<kWhole>(d.master, e, left, p[k]);
     store_codes(d, codes, e, now);
@@ -415,7 +421,8 @@ __device__ __forceinline__ void move_moments(const tm_tensor_t& d, int64_t start
 #pragma unroll
       for (int j = 0; j < 4; ++j) r[j] = fabsf(sqrtf(r[j]));  // (the root of -0 is -0)
       const uint32_t half[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-      store_codes(d, codes, e, hold4(m, r, half));
+      const int past[4] = {};
+      store_codes(d, codes, e, hold4(m, r, past, half));
     }
   }
 }
