@@ -521,7 +521,7 @@ int tm_lin(const tm_lin_t* h_desc, void* d_ws, size_t ws_bytes, void* stream);
  * (all zero is too). The other fields, tables, groups and the workspace (tm_workspace_bytes) are tm_adamw_step's;
  * masters, grads and copies need their elements' alignment only.
  *   tm_adamw8_step     step += 1, the update in fp32 from what is held, and the new moments held again: rounded up or down by a
- *                      hash of seed, step and element, so that the mean is kept. Infinite and NaN moments are held as NaN.
+ *                      hash of seed, step and element (not of the tensor), so that the mean is kept. Infinite and NaN moments are held as NaN.
  *   tm_moments8_read   master[] = exp_avg's values and grad[] = the root's, as bf16 (exact), or, with TM_GRAD_F32 in a record's
  *                      flags, exp_avg's and exp_avg_sq's (the root's square) as fp32.
  *   tm_moments8_write  holds the fp32 values at master (exp_avg) and grad (exp_avg_sq), to the nearest.

@@ -10,7 +10,8 @@
 // Rounding is stochastic: a moment moves by (1 - beta) of its distance to the new gradient in a step, less than half a
 // step of 8 bits (2^-4 of m, 2^-5 of r) for most, and to the nearest it would stay where it is for ever (beta2 = 0.999: r moves by
 // 5e-4 of itself). Rounded up with the probability of the part that lies above, what is held has the right mean.
-// The random bits are a hash of (seed, step, element): the same run gives the same bits, on any launch shape.
+// The random bits are a hash of (seed, step, element): the same run gives the same bits, on any launch shape. The tensor has no part in
+// it: elements i of all tensors are rounded by the same bits in a step.
 //
 // The new moments are summed in fp64 as in the 32-bit step and rounded to fp32 once (sums in fp32 turned three times as many of the
 // roundings the other way); the rest is fp32. Which way a root is rounded goes by its sum in fp64 too: 1-1.6% of the step's time. The
@@ -18,7 +19,8 @@
 //
 // Bound by memory: 16.06 bytes a param with bf16 grads and copies (28 with 32-bit moments). The codes were computed with per-value
 // tests, selects and e4m3 conversions first, 300 vector instructions a wave, which bound the step at 5.5 TB/s; as float's own denormals
-// (below) it runs at 5.95, in-order streams of 256 to 1024 bytes a wave.
+// (below) it ran at 5.95, with the roots' test at 5.6-5.8 (0.6B shape, many launches in a row; 5.6-5.85 without it in turn), in-order
+// streams of 256 to 1024 bytes a wave.
 
 #include <hip/hip_runtime.h>
 
@@ -75,6 +77,8 @@ __device__ __forceinline__ void store_bytes(uint8_t* p, uint32_t v) {
 
 // ---------------------------------------------------------------- random bits
 
+// A: the prime nearest to 2^32 over the golden ratio. B and C: of 400 random odd pairs the one with which, where a bit of the input turns,
+// each bit of the output turns nearest to half the time.
 constexpr uint32_t kHashA = 0x9E3779B1u, kHashB = 0x8C2549D1u, kHashC = 0xD406A25Du;
 
 __device__ __forceinline__ uint32_t mix(uint32_t z) {

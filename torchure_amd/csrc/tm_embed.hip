@@ -18,8 +18,9 @@
 //      the launch fill the rows of ids that do not occur with zeros, which is most of the bytes.
 //   3. Ids with entries in several waves: their partial sums, in order.
 //
-// Measured: 8192 tokens of 151,936 ids x 1024 in fp32: lookup 9 us, the three launches 10, 122 (656 MB at 5.4 TB/s; stores of zeros
-// alone reach 6.7) and 5. 50,001 of 4096 x 777 in bf16: 21; 37, 23 and 14.
+// Measured: 8192 tokens of 151,936 ids x 1024 in fp32: lookup 19 us (its rows out of the caches, as after a gradient's zeros; 7.5 in
+// them), the three launches 10, 118 (656 MB at 5.6 TB/s; stores of zeros alone reach 6.7) and 6. 50,001 of 4096 x 777 in bf16: 22; 37,
+// 23 (too few bytes on their way: rows of 512 are read at 2.1 TB/s in as many tokens and at 4.2 in four times as many) and 14.
 
 #include <hip/hip_runtime.h>
 
