@@ -14,13 +14,12 @@
 // it: elements i of all tensors are rounded by the same bits in a step.
 //
 // The new moments are summed in fp64 as in the 32-bit step and rounded to fp32 once (sums in fp32 turned three times as many of the
-// roundings the other way); the rest is fp32. Which way a root is rounded goes by its sum in fp64 too: 1-1.6% of the step's time. The
-// step uses the moments before they are held again.
+// roundings the other way); the rest is fp32. Which way a root is rounded goes by its sum in fp64 too. The step uses the moments before
+// they are held again.
 //
 // Bound by memory: 16.06 bytes a param with bf16 grads and copies (28 with 32-bit moments). The codes were computed with per-value
 // tests, selects and e4m3 conversions first, 300 vector instructions a wave, which bound the step at 5.5 TB/s; as float's own denormals
-// (below) it ran at 5.95, with the roots' test at 5.6-5.8 (0.6B shape, many launches in a row; 5.6-5.85 without it in turn), in-order
-// streams of 256 to 1024 bytes a wave.
+// (below) it runs at 5.7-5.95, in-order streams of 256 to 1024 bytes a wave.
 
 #include <hip/hip_runtime.h>
 
@@ -117,12 +116,12 @@ __device__ __forceinline__ uint32_t hold_m(float m, uint32_t me, uint32_t bits) 
   const uint32_t c = (up >> 24 & 0x80u) | (up >> 20 & 0x7Fu);
   return kAny && !finite(m) ? 0x7Fu : c;
 }
-// A root has no sign, which would reach the next element's code. `past`: -1 where r is past the root that it was rounded
-// from, else 0: the places at which a root turns are fp32 numbers, and half of those just below one are rounded onto it (510 to 560 of
-// 574e6 were held otherwise than in 64 bits, none so).
+// A root has no sign, which would reach the next element's code. `up`: its code and the bits below, the random ones added.
+__device__ __forceinline__ uint32_t root_up(float r, uint32_t re, uint32_t bits) {
+  return __float_as_uint(scale_root(r, re)) + ((bits >> 13 & ~7u) | 4u);
+}
 template <bool kAny>
-__device__ __forceinline__ uint32_t hold_root(float r, int past, uint32_t re, uint32_t bits) {
-  const uint32_t up = __float_as_uint(scale_root(r, re)) + ((bits >> 13 & ~7u) | 4u) + past;
+__device__ __forceinline__ uint32_t hold_root(float r, uint32_t up) {
   const uint32_t c = max(up >> 19, min(__float_as_uint(r), 1u));
   return kAny && !finite(r) ? 255u : c;
 }
@@ -136,13 +135,24 @@ struct Codes {
   uint32_t me, re;   // the exponents' bytes
 };
 
-template <bool kAny>
-__device__ __forceinline__ void codes4(Codes& c, const float* m, const float* r, const int* past, const uint32_t* bits) {
+// past(j): whether r[j] is past the root that it was rounded from. The places at which a root turns are fp32 numbers, and half of those
+// just below one are rounded onto it (510 to 560 of 574e6 were held otherwise than in 64 bits, none so). Looked at where a root lies on one,
+// which one wave in 2000 sees: for each root it cost the step 1-1.6%, so nothing; exp_avg's values (14-25 of 37e6 with fp32 gradients, none
+// with bf16 ones) in the same way 1-2%, for want of registers.
+template <bool kAny, class Past>
+__device__ __forceinline__ void codes4(Codes& c, const float* m, const float* r, const uint32_t* bits, Past&& past) {
+  uint32_t up[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) up[j] = root_up(r[j], c.re, bits[j]);
+  if (min(min(up[0] << 13, up[1] << 13), min(up[2] << 13, up[3] << 13)) == 0) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) up[j] -= past(j);
+  }
   c.m = c.r = 0;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     c.m |= hold_m<kAny>(m[j], c.me, bits[j]) << (8 * j);
-    c.r |= hold_root<kAny>(r[j], past[j], c.re, bits[j]) << (8 * j);
+    c.r |= hold_root<kAny>(r[j], up[j]) << (8 * j);
   }
 }
 
@@ -151,7 +161,8 @@ __device__ __forceinline__ uint32_t most4(const float* x) {
              max(__float_as_uint(x[2]) & 0x7FFFFFFFu, __float_as_uint(x[3]) & 0x7FFFFFFFu));
 }
 
-__device__ __forceinline__ Codes hold4(const float* m, const float* r, const int* past, const uint32_t* bits) {
+template <class Past>
+__device__ __forceinline__ Codes hold4(const float* m, const float* r, const uint32_t* bits, Past&& past) {
   Codes c;
   uint32_t most_m = most4(m), most_r = most4(r);
   // a wave with an m past all blocks' range, an infinity or a NaN looks at each value
@@ -164,8 +175,8 @@ __device__ __forceinline__ Codes hold4(const float* m, const float* r, const int
   most_r = tm_act::row_max(most_r);
   c.me = static_cast<uint32_t>(tm_act::block_exponent(most_m) + 127);
   c.re = max((most_r + 0x000FFFFFu) >> 23, static_cast<uint32_t>(kRootLow));
-  if (any) codes4<true>(c, m, r, past, bits);
-  else codes4<false>(c, m, r, past, bits);
+  if (any) codes4<true>(c, m, r, bits, past);
+  else codes4<false>(c, m, r, bits, past);
   return c;
 }
 
@@ -344,7 +355,7 @@ __device__ __forceinline__ void update(const tm_tensor_t& d, const Scal& s, floa
     float m[4], r[4];
     read4(was[k], m, r);
     uint32_t bits[4];
-    int past[4];
+    double v[4];
     const uint32_t z = static_cast<uint32_t>(e) * kHashA + s.key;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -352,14 +363,12 @@ __device__ __forceinline__ void update(const tm_tensor_t& d, const Scal& s, floa
       const float pj = (s.flags & kDecay) ? fmaf(s.neg_lrwd, p[k][j], p[k][j]) : p[k][j];
       const double gd = gj;
       m[j] = static_cast<float>(fma(s.beta1, static_cast<double>(m[j]), s.omb1 * gd));
-      const double v = fma(s.beta2, static_cast<double>(r[j] * r[j]), s.omb2 * gd * gd);
-      r[j] = sqrtf(static_cast<float>(v));
-      const double rd = r[j];
-      past[j] = __double2hiint(fma(-rd, rd, v)) >> 31;
+      v[j] = fma(s.beta2, static_cast<double>(r[j] * r[j]), s.omb2 * gd * gd);
+      r[j] = sqrtf(static_cast<float>(v[j]));
       p[k][j] = pj - s.step_size * m[j] / fmaf(r[j], s.inv_bc2s, s.eps);
       bits[j] = element_bits(z + j * kHashA);
     }
-    const Codes now = hold4(m, r, past, bits);
+    const Codes now = hold4(m, r, bits, [&](int j) { return fma(-static_cast<double>(r[j]), static_cast<double>(r[j]), v[j]) < 0.0; });
     const int left = kWhole ? 4 : left_of(d.numel, e);
     store_f32<kWhole>(d.master, e, left, p[k]);
     store_codes(d, codes, e, now);
@@ -425,8 +434,7 @@ __device__ __forceinline__ void move_moments(const tm_tensor_t& d, int64_t start
 #pragma unroll
       for (int j = 0; j < 4; ++j) r[j] = fabsf(sqrtf(r[j]));  // (the root of -0 is -0)
       const uint32_t half[4] = {0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
-      const int past[4] = {};
-      store_codes(d, codes, e, hold4(m, r, past, half));
+      store_codes(d, codes, e, hold4(m, r, half, [](int) { return false; }));
     }
   }
 }
